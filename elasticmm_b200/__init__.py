@@ -8,6 +8,7 @@ GPU; moving KV data does, and there is no CPU fallback.
 from . import _lib
 from ._lib import EmmError
 from .kv_pool import Context, KVPool, compact_plan, get_context
+from .kv_pool_q4 import KVPoolQ4, ScorePool
 
-__all__ = ["Context", "KVPool", "EmmError", "compact_plan", "get_context", "_lib"]
+__all__ = ["Context", "KVPool", "KVPoolQ4", "ScorePool", "EmmError", "compact_plan", "get_context", "_lib"]
 __version__ = "0.1.0"

@@ -48,6 +48,11 @@ OPT_WAIT_LIMIT_NS = 9
 OPT_PDL = 10
 
 
+# enum emm_dtype
+DTYPE_FP16, DTYPE_BF16 = 0, 1
+MAX_QUERY_GROUP = 64
+
+
 class PoolDesc(C.Structure):
     """struct emm_pool_desc."""
 
@@ -122,6 +127,24 @@ SIGNATURES = {
     "emm_append_bound": (C.c_int, [_P, C.c_int32, _P]),
     "emm_append_unbind": (C.c_int, [_P]),
     "emm_upload_ids": (C.c_int, [_P, _P, C.c_int32, _P, _P]),
+    "emm_q4_row_bytes": (C.c_int, [C.c_int32]),
+    "emm_q4_append": (C.c_int, [_P] + [C.c_int32] * 4 + [_P, _P] + [C.c_int64] * 4 + [_P, C.c_int32, _P]),
+    "emm_q4_read": (C.c_int, [_P] + [C.c_int32] * 4 + [_P, _P] + [C.c_int64] * 4 + [_P, C.c_int32, _P]),
+    "emm_q4_attend_workspace": (C.c_int, [_P] + [C.c_int32] * 4 + [C.POINTER(C.c_uint64)]),
+    "emm_q4_attend": (
+        C.c_int,
+        [_P, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, _P, C.c_int64, _P, C.c_int64, C.c_int32, _P, C.c_int32,
+         C.c_int32, C.c_int32, C.c_double, _P, _P, C.c_uint64, _P],
+    ),
+    "emm_select_tokens": (
+        C.c_int,
+        [_P, _P, C.c_int64, C.c_int32, _P, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P],
+    ),
+    "emm_keep_tokens": (
+        C.c_int,
+        [_P, _P, C.c_int32, C.c_int32, _P, C.c_int64, C.c_int32, _P, C.c_int32, _P],
+    ),
+    "emm_reset_scores": (C.c_int, [_P, _P, C.c_int32, _P]),
     "emm_compact_plan": (C.c_int, [_I64P, C.c_int64, C.c_int64, _I64P, _I64P, _I64P, _I64P]),
     "emm_nccl_unique_id": (C.c_int, [C.c_char_p]),
     "emm_nccl_comm_init": (C.c_int, [_P, C.c_char_p, C.c_int, C.c_int, C.POINTER(_P)]),

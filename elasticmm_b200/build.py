@@ -19,7 +19,8 @@ REPO_DIR = PKG_DIR.parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libemm_kv.so"
 SOURCES = [CSRC / "emm_kv.cu"]
-HEADERS = [CSRC / "page_copy.cuh", CSRC / "append.cuh", REPO_DIR / "include" / "emm_kv.h"]
+HEADERS = [*(CSRC / f"{n}.cuh" for n in ("page_copy", "append", "q4", "attend", "evict", "cache_ops")),
+           REPO_DIR / "include" / "emm_kv.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -1,0 +1,359 @@
+// C entries of the 4-bit cache (append, read, decode attention) and of token eviction. Included once, at the end of
+// emm_kv.cu, whose contexts, pools and error helpers it uses. Kernels: q4.cuh, attend.cuh, evict.cuh.
+#pragma once
+#include "attend.cuh"
+#include "evict.cuh"
+#include "q4.cuh"
+
+namespace {
+
+bool q4_dim(int32_t D) { return D == 64 || D == 128 || D == 256; }
+
+// A pool whose rows are 4-bit rows of head_dim channels, in this GPU's memory, every row on a 16-byte boundary.
+int check_q4_pool(const emm_pool *p, int32_t head_dim, const char *what) {
+  if (!p) return fail(EMM_ERR_BAD_ARG, "%s: null pool", what);
+  if (!q4_dim(head_dim)) return fail(EMM_ERR_BAD_ARG, "%s: head dimension %d not in {64, 128, 256}", what, head_dim);
+  const emm_pool_desc &d = p->desc;
+  if (p->planes != 2 || d.elem_size != 1 || d.head_size != emm::q4_row_bytes(head_dim))
+    return fail(EMM_ERR_BAD_ARG, "%s: needs a two-plane pool of bytes with %d bytes per head row, got %d x %d bytes", what,
+                emm::q4_row_bytes(head_dim), d.head_size, d.elem_size);
+  if (!p->device_local) return fail(EMM_ERR_BAD_ARG, "%s: the pool is not in this GPU's memory", what);
+  if (p->align < 16 || d.token_stride % 16 || d.head_stride % 16)
+    return fail(EMM_ERR_ALIGN, "%s: rows of the pool must lie on 16-byte boundaries", what);
+  return EMM_OK;
+}
+
+int check_dtype(int32_t dtype, const char *what) {
+  if (dtype != EMM_DTYPE_FP16 && dtype != EMM_DTYPE_BF16)
+    return fail(EMM_ERR_BAD_ARG, "%s: dtype %d is neither EMM_DTYPE_FP16 nor EMM_DTYPE_BF16", what, dtype);
+  return EMM_OK;
+}
+
+emm::TokenSide token_side(const emm_pool *p) {
+  emm::TokenSide s;
+  s.layers = p->d_layers;
+  s.plane_stride = (uint64_t)p->desc.plane_stride;
+  s.block_stride = (uint64_t)p->desc.block_stride;
+  s.token_stride = (uint64_t)p->desc.token_stride;
+  s.head_stride = (uint64_t)p->desc.head_stride;
+  s.num_blocks = (uint32_t)p->desc.num_blocks;
+  s.block_size = (uint32_t)p->desc.block_size;
+  return s;
+}
+
+// A single-plane pool of fp32 [NB, H, BS] (accumulated attention weights).
+int check_score_pool(const emm_pool *p, const char *what) {
+  if (!p) return fail(EMM_ERR_BAD_ARG, "%s: null score pool", what);
+  const emm_pool_desc &d = p->desc;
+  if (p->planes != 1 || d.elem_size != 4 || p->page_bytes == 0)
+    return fail(EMM_ERR_BAD_ARG, "%s: weights are a single-plane pool of fp32 [NB, heads, block size] with dense blocks", what);
+  if (!p->device_local) return fail(EMM_ERR_BAD_ARG, "%s: the score pool is not in this GPU's memory", what);
+  return EMM_OK;
+}
+
+int check_tables(const int32_t *tables, int64_t stride, int32_t width, const int32_t *lens, int32_t B, const char *what) {
+  if (B < 0 || width < 0) return fail(EMM_ERR_BAD_ARG, "%s: negative count", what);
+  if (B > 0 && (!lens || (width > 0 && !tables))) return fail(EMM_ERR_BAD_ARG, "%s: null pointer", what);
+  if (B > 1 && stride < width) return fail(EMM_ERR_BAD_ARG, "%s: table stride smaller than its width", what);
+  return EMM_OK;
+}
+
+int q4_rows_impl(emm_pool *pool, bool append, int32_t D, int32_t dtype, int32_t layer_begin, int32_t layer_count,
+                 const void *key, const void *value, int64_t kls, int64_t kts, int64_t vls, int64_t vts,
+                 const int64_t *slots, int32_t T, void *stream) {
+  const char *what = append ? "q4_append" : "q4_read";
+  if (int rc = check_q4_pool(pool, D, what)) return rc;
+  if (int rc = check_dtype(dtype, what)) return rc;
+  if (int rc = check_layer_range(pool, layer_begin, layer_count)) return rc;
+  if (T < 0) return fail(EMM_ERR_BAD_ARG, "%s: negative token count", what);
+  if (T == 0 || layer_count == 0) return EMM_OK;
+  if (!key || !value || !slots) return fail(EMM_ERR_BAD_ARG, "%s: null pointer", what);
+  const int64_t row = (int64_t)pool->desc.num_kv_heads * D * 2;
+  if (kts < row || vts < row)
+    return fail(EMM_ERR_BAD_ARG, "%s: token stride smaller than a token row (%lld bytes)", what, (long long)row);
+  if (layer_count > 1 && (kls < (int64_t)(T - 1) * kts + row || vls < (int64_t)(T - 1) * vts + row))
+    return fail(EMM_ERR_BAD_ARG, "%s: layer stride smaller than one layer of rows", what);
+  uint32_t align = 256;
+  const uint64_t parts[] = {(uint64_t)key, (uint64_t)value, (uint64_t)kts, (uint64_t)vts,
+                            layer_count > 1 ? (uint64_t)kls : 0, layer_count > 1 ? (uint64_t)vls : 0};
+  for (uint64_t v : parts) align = std::min(align, pow2_align(v));
+  if (align < 2) return fail(EMM_ERR_ALIGN, "%s: key/value not aligned to their elements", what);
+  const uint64_t units = (uint64_t)T * (uint64_t)pool->desc.num_kv_heads * (uint64_t)(D / 4);
+  const uint64_t blocks = (units + 255) / 256;
+  if ((uint64_t)T * (uint64_t)pool->desc.num_kv_heads > 0xffffffffull || blocks > 0x7fffffffull || layer_count > 32767)
+    return fail(EMM_ERR_TOO_LARGE, "%s: %d layers x %d tokens", what, layer_count, T);
+
+  emm::Q4RowsArgs a;
+  a.pool = token_side(pool);
+  a.layer_begin = (uint32_t)layer_begin;
+  a.num_tokens = (uint32_t)T;
+  a.heads = (uint32_t)pool->desc.num_kv_heads;
+  a.key = (uint64_t)key;
+  a.value = (uint64_t)value;
+  a.key_layer_stride = (uint64_t)kls;
+  a.key_token_stride = (uint64_t)kts;
+  a.value_layer_stride = (uint64_t)vls;
+  a.value_token_stride = (uint64_t)vts;
+  a.slots = slots;
+  a.status = pool->ctx->d_status;
+  DeviceGuard guard(pool->ctx->device);
+  if (!guard.ok()) return fail(EMM_ERR_CUDA, "cannot select device %d", pool->ctx->device);
+  const dim3 grid((unsigned)blocks, (unsigned)layer_count * 2);
+  cudaStream_t st = (cudaStream_t)stream;
+#define EMM_Q4_ROWS(T_, D_)                                                                     \
+  do {                                                                                          \
+    if (append) {                                                                               \
+      if (align >= 8) emm::q4_append<T_, D_, true><<<grid, 256, 0, st>>>(a);                    \
+      else emm::q4_append<T_, D_, false><<<grid, 256, 0, st>>>(a);                              \
+    } else {                                                                                    \
+      if (align >= 8) emm::q4_read<T_, D_, true><<<grid, 256, 0, st>>>(a);                      \
+      else emm::q4_read<T_, D_, false><<<grid, 256, 0, st>>>(a);                                \
+    }                                                                                           \
+  } while (0)
+  if (dtype == EMM_DTYPE_FP16) {
+    if (D == 64) EMM_Q4_ROWS(__half, 64);
+    else if (D == 128) EMM_Q4_ROWS(__half, 128);
+    else EMM_Q4_ROWS(__half, 256);
+  } else {
+    if (D == 64) EMM_Q4_ROWS(__nv_bfloat16, 64);
+    else if (D == 128) EMM_Q4_ROWS(__nv_bfloat16, 128);
+    else EMM_Q4_ROWS(__nv_bfloat16, 256);
+  }
+#undef EMM_Q4_ROWS
+  EMM_CUDA(cudaGetLastError());
+  pool->ctx->launches += 1;
+  return EMM_OK;
+}
+
+uint64_t attend_workspace(const emm_pool *pool, int32_t B, int32_t Hq, int32_t max_len) {
+  return (uint64_t)B * (uint64_t)Hq * (uint64_t)max_len * sizeof(float);
+}
+
+}  // namespace
+
+extern "C" {
+
+int emm_q4_row_bytes(int32_t head_dim) { return q4_dim(head_dim) ? emm::q4_row_bytes(head_dim) : 0; }
+
+int emm_q4_append(emm_pool *pool, int32_t head_dim, int32_t dtype, int32_t layer_begin, int32_t layer_count,
+                  const void *d_key, const void *d_value, int64_t key_layer_stride, int64_t key_token_stride,
+                  int64_t value_layer_stride, int64_t value_token_stride, const int64_t *d_slot_mapping,
+                  int32_t num_tokens, void *stream) {
+  return q4_rows_impl(pool, true, head_dim, dtype, layer_begin, layer_count, d_key, d_value, key_layer_stride,
+                      key_token_stride, value_layer_stride, value_token_stride, d_slot_mapping, num_tokens, stream);
+}
+
+int emm_q4_read(emm_pool *pool, int32_t head_dim, int32_t dtype, int32_t layer_begin, int32_t layer_count, void *d_key,
+                void *d_value, int64_t key_layer_stride, int64_t key_token_stride, int64_t value_layer_stride,
+                int64_t value_token_stride, const int64_t *d_slot_mapping, int32_t num_tokens, void *stream) {
+  return q4_rows_impl(pool, false, head_dim, dtype, layer_begin, layer_count, d_key, d_value, key_layer_stride,
+                      key_token_stride, value_layer_stride, value_token_stride, d_slot_mapping, num_tokens, stream);
+}
+
+int emm_q4_attend_workspace(emm_pool *pool, int32_t num_seqs, int32_t num_heads, int32_t max_len, int32_t with_scores,
+                            uint64_t *bytes) {
+  if (!pool || !bytes) return fail(EMM_ERR_BAD_ARG, "q4_attend_workspace: null argument");
+  if (num_seqs < 0 || num_heads <= 0 || max_len < 0 || num_heads % pool->desc.num_kv_heads)
+    return fail(EMM_ERR_BAD_ARG, "q4_attend_workspace: %d sequences, %d heads, length %d", num_seqs, num_heads, max_len);
+  (void)with_scores;
+  *bytes = attend_workspace(pool, num_seqs, num_heads, max_len);
+  return EMM_OK;
+}
+
+int emm_q4_attend(emm_pool *pool, int32_t head_dim, int32_t dtype, int32_t layer, const void *d_query,
+                  int64_t query_seq_stride, void *d_out, int64_t out_seq_stride, const int32_t *d_block_tables,
+                  int64_t table_stride, int32_t table_width, const int32_t *d_seq_lens, int32_t num_seqs,
+                  int32_t num_heads, int32_t max_len, double scale, emm_pool *scores, void *d_workspace,
+                  uint64_t workspace_bytes, void *stream) {
+  const char *what = "q4_attend";
+  if (int rc = check_q4_pool(pool, head_dim, what)) return rc;
+  if (int rc = check_dtype(dtype, what)) return rc;
+  if (int rc = check_layer_range(pool, layer, 1)) return rc;
+  if (int rc = check_tables(d_block_tables, table_stride, table_width, d_seq_lens, num_seqs, what)) return rc;
+  const emm_pool_desc &d = pool->desc;
+  if (num_heads <= 0 || num_heads % d.num_kv_heads || num_heads / d.num_kv_heads > EMM_MAX_QUERY_GROUP)
+    return fail(EMM_ERR_BAD_ARG, "%s: %d query heads on %d KV heads (a multiple of them, at most %d each)", what, num_heads,
+                d.num_kv_heads, EMM_MAX_QUERY_GROUP);
+  if (max_len < 0 || (int64_t)max_len > (int64_t)table_width * d.block_size)
+    return fail(EMM_ERR_LENGTH, "%s: max_len %d needs more than %d blocks of %d tokens", what, max_len, table_width,
+                d.block_size);
+  if (!(scale - scale == 0.0)) return fail(EMM_ERR_BAD_ARG, "%s: the scale is not finite", what);
+  if (scores) {
+    if (int rc = check_score_pool(scores, what)) return rc;
+    if (scores->ctx != pool->ctx) return fail(EMM_ERR_BAD_ARG, "%s: pools of different contexts", what);
+    if (scores->desc.num_layers != d.num_layers || scores->desc.num_blocks != d.num_blocks ||
+        scores->desc.block_size != d.num_kv_heads || scores->desc.head_size != d.block_size)
+      return fail(EMM_ERR_LENGTH, "%s: the score pool must be [%d, %d, %d] in each of %d layers", what, d.num_blocks,
+                  d.num_kv_heads, d.block_size, d.num_layers);
+  }
+  if (num_seqs == 0) return EMM_OK;
+  if (!d_query || !d_out) return fail(EMM_ERR_BAD_ARG, "%s: null pointer", what);
+  const int64_t row = (int64_t)num_heads * head_dim * 2;
+  if (num_seqs > 1 && (query_seq_stride < row || out_seq_stride < row))
+    return fail(EMM_ERR_BAD_ARG, "%s: sequence stride smaller than a row of heads (%lld bytes)", what, (long long)row);
+  uint32_t align = 256;
+  const uint64_t parts[] = {(uint64_t)d_query, (uint64_t)d_out, num_seqs > 1 ? (uint64_t)query_seq_stride : 0,
+                            num_seqs > 1 ? (uint64_t)out_seq_stride : 0};
+  for (uint64_t v : parts) align = std::min(align, pow2_align(v));
+  if (align < 2) return fail(EMM_ERR_ALIGN, "%s: query/out not aligned to their elements", what);
+  const uint64_t want = attend_workspace(pool, num_seqs, num_heads, max_len);
+  if (workspace_bytes < want || (want && !d_workspace))
+    return fail(EMM_ERR_LENGTH, "%s: workspace of %llu bytes, %llu needed", what, (unsigned long long)workspace_bytes,
+                (unsigned long long)want);
+  if ((uint64_t)num_seqs * d.num_kv_heads > 0x7fffffffull) return fail(EMM_ERR_TOO_LARGE, "%s: %d sequences", what, num_seqs);
+
+  emm::AttendArgs a;
+  a.pool = token_side(pool);
+  a.layer_base = pool->h_layers[layer];
+  a.query = (uint64_t)d_query;
+  a.out = (uint64_t)d_out;
+  a.query_seq_stride = (uint64_t)query_seq_stride;
+  a.out_seq_stride = (uint64_t)out_seq_stride;
+  a.tables = d_block_tables;
+  a.table_stride = (uint64_t)table_stride;
+  a.lens = d_seq_lens;
+  a.num_seqs = (uint32_t)num_seqs;
+  a.kv_heads = (uint32_t)d.num_kv_heads;
+  a.group = (uint32_t)(num_heads / d.num_kv_heads);
+  a.max_len = (uint32_t)max_len;
+  a.scale_log2 = (float)(scale * 1.4426950408889634);
+  a.score_base = scores ? scores->h_layers[layer] : 0;
+  a.score_block_stride = scores ? (uint64_t)scores->desc.block_stride : 0;
+  a.logits = (float *)d_workspace;
+  a.status = pool->ctx->d_status;
+  DeviceGuard guard(pool->ctx->device);
+  if (!guard.ok()) return fail(EMM_ERR_CUDA, "cannot select device %d", pool->ctx->device);
+  cudaStream_t st = (cudaStream_t)stream;
+  const unsigned grid = (unsigned)num_seqs * (unsigned)d.num_kv_heads;
+  if (dtype == EMM_DTYPE_FP16) {
+    if (head_dim == 64) emm::attend_q4<__half, 64><<<grid, 256, 0, st>>>(a);
+    else if (head_dim == 128) emm::attend_q4<__half, 128><<<grid, 256, 0, st>>>(a);
+    else emm::attend_q4<__half, 256><<<grid, 256, 0, st>>>(a);
+  } else {
+    if (head_dim == 64) emm::attend_q4<__nv_bfloat16, 64><<<grid, 256, 0, st>>>(a);
+    else if (head_dim == 128) emm::attend_q4<__nv_bfloat16, 128><<<grid, 256, 0, st>>>(a);
+    else emm::attend_q4<__nv_bfloat16, 256><<<grid, 256, 0, st>>>(a);
+  }
+  EMM_CUDA(cudaGetLastError());
+  pool->ctx->launches += 1;
+  return EMM_OK;
+}
+
+int emm_select_tokens(emm_pool *scores, const int32_t *d_block_tables, int64_t table_stride, int32_t table_width,
+                      const int32_t *d_seq_lens, int32_t num_seqs, int32_t keep, int32_t recent, int32_t sink,
+                      int32_t *d_index, int32_t *d_new_lens, void *stream) {
+  const char *what = "select_tokens";
+  if (int rc = check_score_pool(scores, what)) return rc;
+  if (int rc = check_tables(d_block_tables, table_stride, table_width, d_seq_lens, num_seqs, what)) return rc;
+  if (keep <= 0 || recent < 0 || sink < 0 || (int64_t)recent + sink > keep)
+    return fail(EMM_ERR_BAD_ARG, "%s: keep %d must be positive and cover recent %d + sink %d", what, keep, recent, sink);
+  if (num_seqs == 0) return EMM_OK;
+  if (!d_index || !d_new_lens) return fail(EMM_ERR_BAD_ARG, "%s: null pointer", what);
+  const emm_pool_desc &d = scores->desc;
+  if ((uint64_t)num_seqs * d.block_size > 0x7fffffffull || d.num_layers > 65535 ||
+      (int64_t)table_width * d.head_size > 0x7fffffffll)
+    return fail(EMM_ERR_TOO_LARGE, "%s: %d layers x %d sequences of %d blocks", what, d.num_layers, num_seqs, table_width);
+  emm::SelectArgs a;
+  a.layers = scores->d_layers;
+  a.block_stride = (uint64_t)d.block_stride;
+  a.num_blocks = (uint32_t)d.num_blocks;
+  a.block_size = (uint32_t)d.head_size;
+  a.tables = d_block_tables;
+  a.table_stride = (uint64_t)table_stride;
+  a.table_width = (uint32_t)table_width;
+  a.lens = d_seq_lens;
+  a.num_seqs = (uint32_t)num_seqs;
+  a.heads = (uint32_t)d.block_size;
+  a.keep = (uint32_t)keep;
+  a.recent = (uint32_t)recent;
+  a.sink = (uint32_t)sink;
+  a.index = d_index;
+  a.new_lens = d_new_lens;
+  a.status = scores->ctx->d_status;
+  DeviceGuard guard(scores->ctx->device);
+  if (!guard.ok()) return fail(EMM_ERR_CUDA, "cannot select device %d", scores->ctx->device);
+  const dim3 grid((unsigned)num_seqs * (unsigned)d.block_size, (unsigned)d.num_layers);
+  emm::select_tokens<<<grid, emm::kSelectThreads, 0, (cudaStream_t)stream>>>(a);
+  EMM_CUDA(cudaGetLastError());
+  scores->ctx->launches += 1;
+  return EMM_OK;
+}
+
+int emm_keep_tokens(emm_pool *pool, const int32_t *d_index, int32_t index_heads, int32_t keep,
+                    const int32_t *d_block_tables, int64_t table_stride, int32_t table_width, const int32_t *d_seq_lens,
+                    int32_t num_seqs, void *stream) {
+  const char *what = "keep_tokens";
+  if (!pool) return fail(EMM_ERR_BAD_ARG, "%s: null pool", what);
+  if (int rc = check_tables(d_block_tables, table_stride, table_width, d_seq_lens, num_seqs, what)) return rc;
+  if (!pool->device_local) return fail(EMM_ERR_BAD_ARG, "%s: the pool is not in this GPU's memory", what);
+  if (keep <= 0) return fail(EMM_ERR_BAD_ARG, "%s: keep %d must be positive", what, keep);
+  const emm_pool_desc &d = pool->desc;
+  emm::KeepArgs a;
+  a.pool = token_side(pool);
+  if (pool->planes == 1) {
+    // A score pool [NB, H, BS]: a token's row of a head is one element.
+    if (int rc = check_score_pool(pool, what)) return rc;
+    a.heads = (uint32_t)d.block_size;
+    a.row_bytes = (uint32_t)d.elem_size;
+    a.pool.block_size = (uint32_t)d.head_size;
+    a.pool.token_stride = (uint64_t)d.elem_size;
+    a.pool.head_stride = (uint64_t)d.token_stride;
+  } else {
+    a.heads = (uint32_t)d.num_kv_heads;
+    a.row_bytes = (uint32_t)(d.head_size * d.elem_size);
+  }
+  if (index_heads != (int32_t)a.heads)
+    return fail(EMM_ERR_LENGTH, "%s: index of %d heads, the pool has %u", what, index_heads, a.heads);
+  if (num_seqs == 0) return EMM_OK;
+  if (!d_index) return fail(EMM_ERR_BAD_ARG, "%s: null pointer", what);
+  if ((uint64_t)num_seqs * a.heads * pool->planes > 0x7fffffffull || d.num_layers > 65535 ||
+      (int64_t)table_width * a.pool.block_size > 0x7fffffffll)
+    return fail(EMM_ERR_TOO_LARGE, "%s: %d layers x %d sequences of %d blocks", what, d.num_layers, num_seqs, table_width);
+  a.planes = (uint32_t)pool->planes;
+  a.tables = d_block_tables;
+  a.table_stride = (uint64_t)table_stride;
+  a.table_width = (uint32_t)table_width;
+  a.lens = d_seq_lens;
+  a.num_seqs = (uint32_t)num_seqs;
+  a.keep = (uint32_t)keep;
+  a.index = d_index;
+  a.status = pool->ctx->d_status;
+  uint32_t align = pow2_align(a.row_bytes);
+  for (uint64_t p : pool->h_layers) align = std::min(align, pow2_align(p));
+  const uint64_t strides[] = {a.pool.plane_stride, a.pool.block_stride, a.pool.token_stride, a.pool.head_stride};
+  for (uint64_t v : strides) align = std::min(align, pow2_align(v));
+  DeviceGuard guard(pool->ctx->device);
+  if (!guard.ok()) return fail(EMM_ERR_CUDA, "cannot select device %d", pool->ctx->device);
+  const dim3 grid((unsigned)num_seqs * a.heads * a.planes, (unsigned)d.num_layers);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (align >= 16) emm::keep_rows<uint4><<<grid, emm::kKeepThreads, 0, st>>>(a);
+  else if (align >= 8) emm::keep_rows<uint2><<<grid, emm::kKeepThreads, 0, st>>>(a);
+  else if (align >= 4) emm::keep_rows<uint32_t><<<grid, emm::kKeepThreads, 0, st>>>(a);
+  else if (align >= 2) emm::keep_rows<uint16_t><<<grid, emm::kKeepThreads, 0, st>>>(a);
+  else emm::keep_rows<uint8_t><<<grid, emm::kKeepThreads, 0, st>>>(a);
+  EMM_CUDA(cudaGetLastError());
+  pool->ctx->launches += 1;
+  return EMM_OK;
+}
+
+int emm_reset_scores(emm_pool *scores, const int64_t *d_slot_mapping, int32_t num_tokens, void *stream) {
+  const char *what = "reset_scores";
+  if (int rc = check_score_pool(scores, what)) return rc;
+  if (num_tokens < 0) return fail(EMM_ERR_BAD_ARG, "%s: negative token count", what);
+  if (num_tokens == 0) return EMM_OK;
+  if (!d_slot_mapping) return fail(EMM_ERR_BAD_ARG, "%s: null pointer", what);
+  const emm_pool_desc &d = scores->desc;
+  const uint64_t total = (uint64_t)num_tokens * (uint64_t)d.block_size;
+  const uint64_t blocks = (total + 255) / 256;
+  if (blocks > 0x7fffffffull || d.num_layers > 65535) return fail(EMM_ERR_TOO_LARGE, "%s: %d tokens", what, num_tokens);
+  DeviceGuard guard(scores->ctx->device);
+  if (!guard.ok()) return fail(EMM_ERR_CUDA, "cannot select device %d", scores->ctx->device);
+  emm::reset_scores<<<dim3((unsigned)blocks, (unsigned)d.num_layers), 256, 0, (cudaStream_t)stream>>>(
+      scores->d_layers, (uint64_t)d.block_stride, (uint32_t)d.num_blocks, (uint32_t)d.head_size, (uint32_t)d.block_size,
+      d_slot_mapping, (uint64_t)num_tokens, scores->ctx->d_status);
+  EMM_CUDA(cudaGetLastError());
+  scores->ctx->launches += 1;
+  return EMM_OK;
+}
+
+}  // extern "C"

@@ -1672,3 +1672,5 @@ int emm_gather_noalloc(int device, const emm_pool_desc *desc, const void *const 
 }
 
 }  // extern "C"
+
+#include "cache_ops.cuh"

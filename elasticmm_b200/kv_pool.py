@@ -643,6 +643,24 @@ class KVPool:
             key.stride(0) * e, key.stride(1) * e, value.stride(0) * e, value.stride(1) * e,
             C.c_void_p(slot_mapping.data_ptr()), T, C.c_void_p(_stream_ptr(self.device))))
 
+    # -- token eviction ------------------------------------------------------------
+    def keep_tokens(self, index: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor) -> None:
+        """Moves the kept rows to the first places of their sequences, in all layers, planes and heads.
+
+        `index` [L, B, H, keep] (int32, from ScorePool.select_tokens) holds each head's kept positions in ascending
+        order, `seq_lens` the lengths before the eviction. Position j receives the row of position index[.., j];
+        sequences of at most keep tokens, and everything from position keep on, stay as they are. On a ScorePool the
+        weights follow their tokens. A block may belong to one of the sequences only.
+        """
+        B, width = check_block_tables(self, block_tables, seq_lens)
+        heads = self.num_kv_heads if self.num_planes == 2 else self.block_size
+        if (index.dtype != torch.int32 or index.dim() != 4 or index.device != self.device or not index.is_contiguous()
+                or tuple(index.shape[:3]) != (self.num_layers, B, heads)):
+            raise ValueError(f"index must be a contiguous int32 device tensor [{self.num_layers}, {B}, {heads}, keep]")
+        _lib.check(self.ctx._lib.emm_keep_tokens(
+            self._h, index.data_ptr(), heads, index.shape[3], block_tables.data_ptr(), block_tables.stride(0), width,
+            seq_lens.data_ptr(), B, _stream_ptr(self.device)))
+
     def close(self) -> None:
         if getattr(self, "_h", None) is not None and self._h:
             self.ctx._lib.emm_pool_destroy(self._h)
@@ -653,6 +671,18 @@ class KVPool:
             self.close()
         except Exception:
             pass
+
+
+def check_block_tables(pool: KVPool, block_tables: torch.Tensor, seq_lens: torch.Tensor) -> Tuple[int, int]:
+    """(B, width) of int32 device tables [B, width] and lengths [B]."""
+    if (block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.device != pool.device
+            or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1)
+            or (block_tables.shape[0] > 1 and block_tables.stride(0) < block_tables.shape[1])):
+        raise ValueError("block_tables must be int32 [B, blocks] on the pool's device, each row contiguous")
+    if (seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or seq_lens.device != pool.device
+            or not seq_lens.is_contiguous() or seq_lens.numel() != block_tables.shape[0]):
+        raise ValueError("seq_lens must be a contiguous int32 device tensor with one entry per block table")
+    return block_tables.shape[0], block_tables.shape[1]
 
 
 def compact_plan(table_ids: Sequence[int], num_blocks: int) -> Tuple[np.ndarray, np.ndarray, np.ndarray]:

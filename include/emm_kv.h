@@ -329,6 +329,110 @@ int emm_append_bind(emm_pool *pool, const void *d_key, const void *d_value, int6
 int emm_append_bound(emm_append_binding *binding, int32_t layer, void *stream);
 int emm_append_unbind(emm_append_binding *binding);
 
+/* ---- 4-bit cache ------------------------------------------------------- */
+
+/* A 4-bit pool is an ordinary two-plane pool of BYTES whose head row is one
+ * 4-bit row: elem_size 1, head_size emm_q4_row_bytes(D), D = 64, 128 or 256
+ * channels. Gather, scatter, block copy, migration and compaction move its
+ * pages as they move any other; the entries below write, read and attend to
+ * its rows. No counterpart in the reference, whose cache is 16-bit.
+ *
+ * Row of D channels in D/32 groups of 32, each with a scale s and an offset o
+ * (fp16); channel x is the code c in 0..15 that stands for o + s*(c - 8):
+ *   lo, hi = smallest, largest of the group, clamped to +-65504
+ *   s = fp16((hi - lo) / 15), o = fp16(lo + 8*s)
+ *   c = clamp(rint((x - o) / s) + 8, 0, 15)   (s == 0: c = 8; a NaN in the
+ *       group makes s and o NaN, and the whole group reads back as NaN)
+ * in fp32, each operation rounded to nearest even. Bytes: D/2 of codes, the
+ * D/32 scales, the D/32 offsets, zeros up to a multiple of 16 (48, 80 and 160
+ * bytes for the three D). The codes come in units of two bytes, four
+ * channels, the lower nibble first; the unit of channels 32r + 4u .. +3 is at
+ * byte 2*(u*D/32 + r). Every row must start on a 16-byte boundary. */
+enum emm_dtype { EMM_DTYPE_FP16 = 0, EMM_DTYPE_BF16 = 1 }; /* of keys, values, queries and outputs */
+#define EMM_MAX_QUERY_GROUP 64 /* most query heads on one KV head */
+
+/* Bytes of a 4-bit row of head_dim channels; 0 if that dimension is not supported. */
+int emm_q4_row_bytes(int32_t head_dim);
+
+/* emm_append / emm_append_all_layers with quantisation: 16-bit key/value rows
+ * [layer_count, T, H, D] (heads dense, strides in bytes) go to their slots in
+ * layers [layer_begin, layer_begin + layer_count). slot < 0 is skipped, a slot
+ * outside the pool recorded in the status word and skipped; when a slot
+ * appears twice, groups of either row may win. */
+int emm_q4_append(emm_pool *pool, int32_t head_dim, int32_t dtype, int32_t layer_begin, int32_t layer_count,
+                  const void *d_key, const void *d_value, int64_t key_layer_stride, int64_t key_token_stride,
+                  int64_t value_layer_stride, int64_t value_token_stride, const int64_t *d_slot_mapping,
+                  int32_t num_tokens, void *stream);
+
+/* The inverse: o + s*(c - 8), rounded once to `dtype` (fp16 saturates at
+ * +-65504), into d_key / d_value [layer_count, T, H, D]. A negative slot, or one outside the pool (recorded),
+ * gives a row of zeros. */
+int emm_q4_read(emm_pool *pool, int32_t head_dim, int32_t dtype, int32_t layer_begin, int32_t layer_count, void *d_key,
+                void *d_value, int64_t key_layer_stride, int64_t key_token_stride, int64_t value_layer_stride,
+                int64_t value_token_stride, const int64_t *d_slot_mapping, int32_t num_tokens, void *stream);
+
+/* Decode attention over one layer of a 4-bit pool, one query token per
+ * sequence: out[b,h] = sum_t softmax_t(scale * q[b,h] . K[t]) V[t] over the
+ * seq_lens[b] tokens of sequence b, whose position t lies in block
+ * block_tables[b][t / BS] at place t % BS. Query head h reads KV head
+ * h / (num_heads / H). query and out are [num_seqs, num_heads, D] of `dtype`,
+ * heads dense, with a stride in bytes between sequences. Tables and lengths
+ * are DEVICE int32; table_stride counts entries; entries behind a sequence's
+ * last block are not read. A sequence of length 0 gives zeros. A length
+ * outside [0, max_len] is recorded (EMM_ERR_LENGTH) and clamped; a block id
+ * outside the pool is recorded and its tokens are left out. max_len bounds the
+ * workspace and must not exceed table_width * BS.
+ *
+ * With `scores` (a single-plane pool of fp32 [NB, H, BS] with the KV pool's
+ * layers, emm_pool_desc_blocks(L, NB, H, BS, 4)) each token's weight, summed
+ * over the query heads of its KV head, is added to its entry of that layer.
+ * No block may then belong to two of the call's sequences (each block has one
+ * owner, as V0BlockManager hands them out).
+ *
+ * The workspace (emm_q4_attend_workspace bytes, 16-byte aligned) is scratch of
+ * this call: calls that may overlap on the GPU need one each. */
+int emm_q4_attend_workspace(emm_pool *pool, int32_t num_seqs, int32_t num_heads, int32_t max_len, int32_t with_scores,
+                            uint64_t *bytes);
+int emm_q4_attend(emm_pool *pool, int32_t head_dim, int32_t dtype, int32_t layer, const void *d_query,
+                  int64_t query_seq_stride, void *d_out, int64_t out_seq_stride, const int32_t *d_block_tables,
+                  int64_t table_stride, int32_t table_width, const int32_t *d_seq_lens, int32_t num_seqs,
+                  int32_t num_heads, int32_t max_len, double scale, emm_pool *scores, void *d_workspace,
+                  uint64_t workspace_bytes, void *stream);
+
+/* ---- token eviction by accumulated weight ------------------------------- */
+
+/* Which tokens of each sequence stay, per layer and KV head. `scores` is a
+ * score pool (see emm_q4_attend). A sequence of n > keep tokens keeps its
+ * first `sink`, its last `recent` and, of the others, those with the largest
+ * weights up to `keep` in all; of equal weights the earlier token stays, and
+ * a NaN counts as -infinity. d_index [L, num_seqs, H, keep] (int32) receives
+ * their positions in ascending order; for n <= keep it is 0 .. n-1 and then
+ * -1. d_new_lens [num_seqs] (int32) receives min(n, keep). The scores are not
+ * changed. A length outside [0, table_width * BS] is recorded
+ * (EMM_ERR_LENGTH) and taken as 0; a block id outside the pool is recorded and
+ * its tokens have the lowest weight. The reference evicts whole requests only
+ * (elasticmm/engine/v0/block_manager.py:247-256). */
+int emm_select_tokens(emm_pool *scores, const int32_t *d_block_tables, int64_t table_stride, int32_t table_width,
+                      const int32_t *d_seq_lens, int32_t num_seqs, int32_t keep, int32_t recent, int32_t sink,
+                      int32_t *d_index, int32_t *d_new_lens, void *stream);
+
+/* Moves the kept rows to the first places of their sequence, in every layer,
+ * plane and head: position j receives the row of position d_index[l][b][h][j].
+ * Sequences of at most `keep` tokens are left alone, and so is everything from
+ * position `keep` on. `pool` is any pool with heads (16-bit or 4-bit), or a
+ * score pool, whose entries then follow their tokens. d_seq_lens are the
+ * lengths BEFORE the eviction. The rows of one head of one sequence must be
+ * ascending in d_index (as emm_select_tokens writes them); an entry that does
+ * not lie behind its place, or not inside the sequence, is skipped. No block
+ * may belong to two of the call's sequences. */
+int emm_keep_tokens(emm_pool *pool, const int32_t *d_index, int32_t index_heads, int32_t keep,
+                    const int32_t *d_block_tables, int64_t table_stride, int32_t table_width, const int32_t *d_seq_lens,
+                    int32_t num_seqs, void *stream);
+
+/* Zeroes the weights of the tokens at these slots in every layer and head: for
+ * newly appended tokens, whose slots may have held evicted or freed ones. */
+int emm_reset_scores(emm_pool *scores, const int64_t *d_slot_mapping, int32_t num_tokens, void *stream);
+
 /* ---- compaction planning (host only) ---------------------------------- */
 
 /* Minimal-move defragmentation plan. `table_ids` holds the concatenated
