@@ -130,7 +130,7 @@ SIGNATURES = {
     "emm_q4_row_bytes": (C.c_int, [C.c_int32]),
     "emm_q4_append": (C.c_int, [_P] + [C.c_int32] * 4 + [_P, _P] + [C.c_int64] * 4 + [_P, C.c_int32, _P]),
     "emm_q4_read": (C.c_int, [_P] + [C.c_int32] * 4 + [_P, _P] + [C.c_int64] * 4 + [_P, C.c_int32, _P]),
-    "emm_q4_attend_workspace": (C.c_int, [_P] + [C.c_int32] * 4 + [C.POINTER(C.c_uint64)]),
+    "emm_q4_attend_workspace": (C.c_int, [_P] + [C.c_int32] * 5 + [C.POINTER(C.c_uint64)]),
     "emm_q4_attend": (
         C.c_int,
         [_P, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, _P, C.c_int64, _P, C.c_int64, C.c_int32, _P, C.c_int32,

@@ -2,12 +2,65 @@
 //
 //   l[t] = scale * q . k[t]      p = softmax(l) over the sequence's tokens      out = sum_t p[t] v[t]
 //   weights (optional): score[block of t][kv head][place of t] += sum of p[t] over the query heads of the kv head
+//
+// The work is one pass over the cached rows (160 bytes per token and KV head at D = 128), so HBM bounds it; what the
+// layout below is for is to spend few enough instructions per row to keep up (about 40 16-bit elements per clock and SM).
+//
+// Products. A warp owns one KV head and up to eight of its query heads, and takes 16 tokens at a time through
+// mma.m16n8k16 with the CACHE as the 16-row operand: S^T = K Q^T (rows tokens, columns heads), O^T = V^T P^T (rows
+// channels, columns heads). A tcgen05 tile has 64 rows at least, of which a decode step could fill eight, and takes
+// its operands from shared memory, where the codes would first have to be written out as 16-bit values.
+//
+// Codes are never converted. A nibble masked in place in a 16-bit lane IS an fp16 subnormal: c * 2^-24 from bits 0..3,
+// c * 2^-20 from bits 4..7, exact, and the tensor cores take subnormals at full rate. One AND (and half a shift) makes
+// two operand elements. The two powers of two are undone in q (keys) or when the result is written (values).
+//
+// Scales and offsets, x = o + s (c - 8), group r of 32 channels:
+//   l[t]   = sum_r s_r[t] (sum_d q_d c_d) + sum_r (o_r[t] - 8 s_r[t]) Q_r,    Q_r = sum of q over the group
+//            the first bracket is two MMAs per group; the last sum is one MMA (two at D = 256) with the offsets and
+//            scales as rows and Q split into two fp16 halves (22 bits).
+//   out[d] = sum_t (p s_r) c_d - 8 sum_t (p s_r) + sum_t p o_r
+//            p s_r is formed per group as the 16-bit operand; the two sums are one MMA each, with rows of ones (the SAME
+//            rounded p s_r, so rounding enters only through s (c - 8), not through s c) and of offsets.
+// p is held relative to a reference that only follows the running maximum when that outgrows it by 2^6, so the
+// accumulators are rarely rescaled and no maximum is taken across lanes in between. p is scaled by 2^8 (by 2^-4 from
+// the first scale >= 2 on), which keeps p s_r below 2^15 and above fp16's subnormals down to 2^-22 of the largest.
+// With fp16 outputs the rounding of p s_r (2^-12 on average as large as the output's own) is halved again: its
+// remainder, exact by an fma, goes through the same MMAs. bf16 outputs are 8 times coarser and skip that.
+// Logits, sums and accumulators are 32 bits.
+//
+// Work. A unit is 16 (x token subsets) tokens of one sequence for the KV heads of a CTA. The units of the whole batch,
+// counted on the device, are split evenly over the CTAs, whatever the lengths: a CTA finishes the sequences that
+// lie in its share and leaves a partial result (in the workspace) of the at most two that do not; attend_join adds those.
+// Rows come by cp.async.bulk into a ring of stages: per token (token-major pages: the heads of a CTA are one run) or
+// per run of tokens and head (head-major pages). The warps take turns at issuing a unit's copies; a warp of its own for
+// that would leave 96 instead of 128 registers to each of the others (18 instead of 16 warps on an SM), and spill.
 #pragma once
+#include <type_traits>
+
 #include "q4.cuh"
 
 namespace emm {
 
 constexpr int kStatusLength = 3;
+
+// Geometry of the split, chosen on the host (attend_shape in cache_ops.cuh).
+struct AttendShape {
+  uint32_t heads_cta;    // KV heads per CTA
+  uint32_t head_groups;  // CTAs' worth of heads: ceil(H / heads_cta)
+  uint32_t ntiles;       // tiles of eight query heads per KV head
+  uint32_t subsets;      // token subsets of a unit, one warp each
+  uint32_t tokens;       // tokens per unit: 16 * subsets
+  uint32_t warps;        // heads_cta * ntiles * subsets
+  uint32_t run;          // tokens per bulk copy
+  uint32_t copy_heads;   // head copies per token run: 1 (token-major) or heads_cta
+  uint32_t ts, hs;       // shared-memory strides of a token and of a head, bytes
+  uint32_t plane_bytes;  // of one plane of a stage
+  uint32_t stages;
+  uint32_t grid;         // CTAs
+  uint32_t min_units;    // least units worth a CTA
+  uint32_t items;        // num_seqs * head_groups
+};
 
 struct AttendArgs {
   TokenSide pool;
@@ -24,9 +77,19 @@ struct AttendArgs {
   uint32_t group;             // query heads per kv head
   uint32_t max_len;
   float scale_log2;           // softmax scale * log2(e)
+  uint32_t align;             // common alignment of query and out
   uint64_t score_base;        // [NB, H, BS] fp32, or 0
   uint64_t score_block_stride;
-  float *logits;              // workspace [B, Hq, max_len]
+  uint64_t wait_limit_ns;
+  AttendShape sh;
+  // workspace
+  float *part_o;              // [2 * grid][heads_cta * group][D]
+  float2 *part_ml;            // [2 * grid][heads_cta * group]: reference, sum
+  int2 *item_span;            // [items]: first and last CTA of an item
+  int *cta_item;              // [grid]: the split item that this CTA finished, or -1
+  float *lse;                 // [B, Hq], with scores
+  float *logits;              // [B, Hq, logit_stride], with scores
+  uint64_t logit_stride;
   int *status;
 };
 
@@ -39,105 +102,807 @@ __device__ __forceinline__ uint32_t seq_length(const AttendArgs &a, uint32_t b, 
   return (uint32_t)n;
 }
 
-// Block of position t, or -1 (reported) for an id outside the pool.
-__device__ __forceinline__ int32_t block_of(const AttendArgs &a, uint32_t b, uint32_t t, bool reporter) {
-  const int32_t id = a.tables[b * a.table_stride + t / a.pool.block_size];
-  if ((uint32_t)id >= a.pool.num_blocks) {
-    if (reporter) report(a.status, kStatusIdRange, id);
-    return -1;
+__device__ __forceinline__ uint32_t seq_units(const AttendArgs &a, uint32_t n) {
+  return n == 0 ? 1u : (n + a.sh.tokens - 1) / a.sh.tokens;  // an empty sequence has one empty unit: its zeros
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void mma_k16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1, const float (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  uint32_t y;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+  return y;
+}
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
+  uint32_t y;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+__device__ __forceinline__ uint32_t fma_half2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t y;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(a), "r"(b), "r"(c));
+  return y;
+}
+__device__ __forceinline__ float2 unpack_half2(uint32_t x) {
+  return __half22float2(*reinterpret_cast<const __half2 *>(&x));
+}
+
+// Two 16-bit values of a word.
+template <typename T>
+__device__ __forceinline__ void unpack2(uint32_t w, float &lo, float &hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const float2 f = unpack_half2(w);
+    lo = f.x;
+    hi = f.y;
+  } else {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xffff0000u);
   }
-  return id;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    uint32_t y;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+    return y;
+  } else {
+    uint32_t y;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+    return y;
+  }
 }
 
-template <int D>
-__device__ __forceinline__ float q4_value(const uint8_t *row, uint32_t d) {
-  constexpr uint32_t G = q4_groups(D);
-  const uint32_t r = d / 32, u = d % 32 / 4, i = d % 4;
-  const uint32_t code = *reinterpret_cast<const uint16_t *>(row + 2 * (u * G + r));
-  const float s = __half2float(*reinterpret_cast<const __half *>(row + D / 2 + 2 * r));
-  const float o = __half2float(*reinterpret_cast<const __half *>(row + D / 2 + 2 * G + 2 * r));
-  return o + s * ((float)(int)((code >> (4 * i)) & 15u) - 8.f);
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t a) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+  return v;
+}
+// N words from consecutive addresses (8- or 16-byte aligned as the row format guarantees).
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t (&w)[N], uint32_t a) {
+  if constexpr (N == 1) {
+    w[0] = lds32(a);
+  } else if constexpr (N == 2) {
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3])
+                   : "r"(a + 4 * i));
+  }
 }
 
-// One CTA per (sequence, kv head): logits into the workspace, then the weights, then the weighted sum by channel.
+// Raises the transaction count of the barrier's current phase without arriving.
+__device__ __forceinline__ void mbar_expect_bytes(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+constexpr uint32_t kNib0 = 0x000f000fu, kNib1 = 0x00f000f0u;
+constexpr uint32_t kLoHalves = 0x5410u, kHiHalves = 0x7632u;  // prmt selectors: low / high halves of two words
+constexpr float kFirstRef = -1e30f;                            // reference before any token
+
+// Where a CTA's share of the units begins, found by all threads together.
+struct Share {
+  uint32_t b, hg, unit;  // first unit: sequence, head group, unit within the item
+  uint32_t count;        // units
+  uint32_t grid;         // CTAs that have a share
+  uint64_t total;        // units of the batch
+  uint64_t first;        // index of the first unit in the batch
+};
+
+// Decode attention; see the top of the file. kPrecise: carry the remainder of p s_r (fp16 outputs).
 template <typename T, int D>
-__global__ void __launch_bounds__(256) attend_q4(const __grid_constant__ AttendArgs a) {
-  __shared__ float qs[64 * 256 / 4];  // 16 heads of 256 channels at a time
-  __shared__ float red[8], stat[2 * 64];
-  const uint32_t b = blockIdx.x / a.kv_heads, h = blockIdx.x % a.kv_heads;
-  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const uint32_t n = seq_length(a, b, threadIdx.x == 0 && h == 0);
-  const uint32_t heads = a.kv_heads * a.group;
-  float *lg = a.logits + ((uint64_t)b * heads + h * a.group) * a.max_len;
-  auto row_of = [&](uint32_t t, int32_t id, uint32_t plane) {
-    return reinterpret_cast<const uint8_t *>(a.layer_base + plane * a.pool.plane_stride + (uint64_t)id * a.pool.block_stride +
-                                             (t % a.pool.block_size) * a.pool.token_stride + h * a.pool.head_stride);
-  };
-  for (uint32_t j0 = 0; j0 < a.group; j0 += 16) {
-    const uint32_t nj = min(16u, a.group - j0);
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attend_q4(const __grid_constant__ AttendArgs a) {
+  constexpr int G = q4_groups(D), R = q4_row_bytes(D);
+  constexpr int KW = D / 32;  // words of codes per lane and token, keys (two units of every group)
+  constexpr int VW = D / 64;  // words of codes per lane and token, values (one unit of every group)
+  constexpr int SW = (G + 1) / 2;  // words of a token's scales
+  constexpr bool kPrecise = sizeof(T) == 2 && std::is_same<T, __half>::value;
+  extern __shared__ __align__(128) unsigned char smem[];
+  constexpr uint32_t kMaxAttendStages = 16;
+  __shared__ __align__(8) uint64_t bar_full[kMaxAttendStages], bar_empty[kMaxAttendStages];
+  __shared__ uint32_t valid[kMaxAttendStages][4];  // which of a stage's tokens count
+  __shared__ uint32_t used[kMaxAttendStages];      // times a stage was filled
+  __shared__ Share share;
+  __shared__ uint64_t scan[10];
+  __shared__ int aborted;
+
+  const AttendShape &sh = a.sh;
+  const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const uint32_t stage_bytes = 2 * sh.plane_bytes;
+  grid_launch_dependents();
+
+  if (tid == 0) {
+    for (uint32_t s = 0; s < sh.stages; ++s) {
+      mbar_init(smem_u32(&bar_full[s]), 1);
+      mbar_init(smem_u32(&bar_empty[s]), sh.warps);
+      used[s] = 0;
+    }
+    mbar_init_fence();
+    aborted = 0;
+    a.cta_item[blockIdx.x] = -1;
+  }
+  // The batch's units and this CTA's share of them. A thread takes a run of consecutive sequences.
+  {
+    const uint32_t per = (a.num_seqs + blockDim.x - 1) / blockDim.x;
+    const uint32_t b0 = min(a.num_seqs, tid * per), b1 = min(a.num_seqs, b0 + per);
+    uint64_t mine = 0;
+    for (uint32_t b = b0; b < b1; ++b) mine += seq_units(a, seq_length(a, b, blockIdx.x == 0)) * (uint64_t)sh.head_groups;
+    uint64_t upto = mine;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+      const uint64_t other = __shfl_up_sync(0xffffffffu, upto, m);
+      if (lane >= m) upto += other;
+    }
+    if (lane == 31) scan[warp] = upto;
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < nj * D; i += 256)
-      qs[i] = to_f32<T>(reinterpret_cast<const T *>(a.query + b * a.query_seq_stride)[(h * a.group + j0) * D + i]);
+    uint64_t before = 0, total = 0;
+    for (uint32_t w = 0; w < blockDim.x / 32; ++w) {
+      if (w < warp) before += scan[w];
+      total += scan[w];
+    }
+    before += upto - mine;
+    const uint64_t worth = max((uint64_t)1, total / sh.min_units);
+    const uint32_t grid = (uint32_t)min((uint64_t)gridDim.x, worth);
+    const uint64_t first = blockIdx.x < grid ? total * blockIdx.x / grid : total;
+    const uint64_t end = blockIdx.x < grid ? total * (blockIdx.x + 1) / grid : total;
+    if (tid == 0) {
+      share.count = (uint32_t)(end - first);
+      share.grid = grid;
+      share.total = total;
+      share.first = first;
+    }
+    if (first < end && before <= first && first < before + mine) {
+      uint64_t at = before;
+      uint32_t b = b0;
+      for (;; ++b) {
+        const uint64_t u = seq_units(a, seq_length(a, b, false)) * (uint64_t)sh.head_groups;
+        if (first < at + u) break;
+        at += u;
+      }
+      const uint32_t units = seq_units(a, seq_length(a, b, false));
+      share.b = b;
+      share.hg = (uint32_t)((first - at) / units);
+      share.unit = (uint32_t)((first - at) % units);
+    }
     __syncthreads();
-    for (uint32_t t = warp; t < n; t += 8) {
-      const int32_t id = block_of(a, b, t, lane == 0);
-      float k[D / 32];
-      if (id >= 0)
-        for (uint32_t i = 0; i < D / 32; ++i) k[i] = q4_value<D>(row_of(t, id, 0), i * 32 + lane);
-      for (uint32_t j = 0; j < nj; ++j) {
-        float s = 0.f;
-        if (id >= 0)
-          for (uint32_t i = 0; i < D / 32; ++i) s += k[i] * qs[j * D + i * 32 + lane];
-        for (int m = 16; m; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-        if (lane == 0) lg[(uint64_t)(j0 + j) * a.max_len + t] = id < 0 ? -INFINITY : s * a.scale_log2;
+  }
+  uint32_t left = share.count;
+  if (left == 0) return;
+  uint32_t b = share.b, hg = share.hg, unit = share.unit;
+  bool ok = true;
+
+  // ---- loads: this warp's turns are units warp, warp + warps, .. of the share
+  const uint32_t ring = smem_u32(smem);
+  const uint32_t all = left, copies = sh.tokens / sh.run * sh.copy_heads;  // copies per plane
+  uint32_t turn = warp;                                                    // next unit this warp issues
+  uint32_t ib = b, ihg = hg, iunit = unit + warp, in = seq_length(a, b, false), iunits = seq_units(a, in);
+  auto issue = [&]() {
+    while (iunit >= iunits) {
+      iunit -= iunits;
+      if (++ihg == sh.head_groups) {
+        ihg = 0;
+        in = seq_length(a, ++ib, false);
+        iunits = seq_units(a, in);
       }
     }
+    const uint32_t use = turn / sh.stages, s = turn - use * sh.stages;
+    const uint32_t h0 = ihg * sh.heads_cta, heads = min(sh.heads_cta, a.kv_heads - h0);
+    const uint32_t full = smem_u32(&bar_full[s]), to = ring + s * stage_bytes;
+    if (use > 0) {
+      ok = mbar_wait_bounded(smem_u32(&bar_empty[s]), (use - 1) & 1, a.wait_limit_ns);
+      ok = __all_sync(0xffffffffu, ok) && !*(volatile int *)&aborted;
+      if (!ok) {
+        if (lane == 0) {
+          report(a.status, kStatusTimeout, (long long)blockIdx.x);
+          *(volatile int *)&aborted = 1;
+        }
+        turn = 0xffffffffu;
+        return;
+      }
+    }
+    uint32_t bits[4] = {0, 0, 0, 0};
+#pragma unroll 1
+    for (uint32_t c = lane; c < copies; c += 32) {
+      const uint32_t run = c / sh.copy_heads, head = c - run * sh.copy_heads;
+      const uint32_t t_rel = run * sh.run, t = iunit * sh.tokens + t_rel;
+      if (t >= in || head >= heads) continue;
+      const uint32_t blk = t / a.pool.block_size;
+      const int32_t id = a.tables[ib * a.table_stride + blk];
+      if ((uint32_t)id >= a.pool.num_blocks) {
+        report(a.status, kStatusIdRange, id);
+        continue;
+      }
+      const uint32_t count = min(sh.run, in - t);
+      const uint64_t src = a.layer_base + (uint64_t)id * a.pool.block_stride + (t - blk * a.pool.block_size) * a.pool.token_stride +
+                           (h0 + head) * a.pool.head_stride;
+      const uint32_t dst = to + t_rel * sh.ts + head * sh.hs;
+      const uint32_t len = (sh.copy_heads == 1 ? heads : 1u) * count * R;  // several heads (one token), or several tokens
+      mbar_expect_bytes(full, 2 * len);
+      bulk_load(dst, src, len, full);
+      bulk_load(dst + sh.plane_bytes, src + a.pool.plane_stride, len, full);
+      if (head == 0) {
+        const uint32_t m = ((1u << count) - 1u) << (t_rel % 32);
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          if (t_rel / 32 == w) bits[w] |= m;
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      if (w * 32 < (int)sh.tokens) {
+        const uint32_t m = __reduce_or_sync(0xffffffffu, bits[w]);
+        if (lane == 0) valid[s][w] = m;
+      }
+    __syncwarp();
+    if (lane == 0) {
+      used[s] = use + 1;
+      mbar_arrive(full);  // after every lane's expected bytes: the phase ends when they have landed
+    }
+    turn += sh.warps;
+    iunit += sh.warps;
+  };
+  while (turn < min(all, sh.stages)) issue();
+  uint32_t done = 0;  // units this warp has consumed
+
+  uint32_t stage = 0, parity = 0;
+  auto advance = [&]() {
+    if (++stage == sh.stages) {
+      stage = 0;
+      parity ^= 1;
+    }
+  };
+
+  const uint32_t hl = warp % sh.heads_cta;                       // KV head within the CTA
+  const uint32_t nt = warp / sh.heads_cta % sh.ntiles;           // tile of query heads
+  const uint32_t sub = warp / (sh.heads_cta * sh.ntiles);        // token subset
+  const uint32_t g = lane / 4, q4 = lane % 4;
+  // Tokens of fragment rows: with a token stride of 32 * odd bytes (token-major) rows 2i, 2i + 1 are two tokens apart
+  // and even (odd) rows cover all residues mod 4; with 16 * odd (head-major) even rows are even tokens. Either way the
+  // value loads, and in the first case the key loads too, touch every bank once.
+  auto token_of = [&](uint32_t r) -> uint32_t {
+    if (sh.ts % 32) return r;
+    return r < 4 ? (r >> 1) + 2 * (r & 1) : (r < 6 ? 6 - 2 * (r & 1) : 7 - 2 * (r & 1));
+  };
+  const uint32_t tk = token_of(g);                            // key rows g and g + 8: tokens tk, tk + 8
+  const uint32_t tv0 = token_of(2 * q4), tv1 = token_of(2 * q4 + 1);
+  const uint32_t t_sub = sub * 16;
+  const uint32_t k_off = (t_sub + tk) * sh.ts + hl * sh.hs;
+  const uint32_t v_off0 = sh.plane_bytes + (t_sub + tv0) * sh.ts + hl * sh.hs;
+  const uint32_t v_off1 = sh.plane_bytes + (t_sub + tv1) * sh.ts + hl * sh.hs;
+  float *merge = reinterpret_cast<float *>(smem + sh.stages * stage_bytes);  // [(warps - warps/subsets)][8][D + 2]
+
+  while (left > 0) {
+    const uint32_t n = seq_length(a, b, false), units = seq_units(a, n);
+    const uint32_t unit0 = unit, count = min(left, units - unit);
+    const uint32_t h = hg * sh.heads_cta + hl;
+    const bool active = h < a.kv_heads;
+    const uint32_t j0 = nt * 8;  // first query head of the tile, within the group
+
+    // ---- the queries of this tile as B fragments
+    uint32_t qf[G][4];
+    uint32_t qo[2], qc[2];  // Q_r and -8 Q_r as two halves: B fragments of the offsets' and scales' product
+    float c0, c1;       // logit factors of heads 2 q4, 2 q4 + 1
+    {
+      const bool mine = active && j0 + g < a.group;
+      const uint64_t src = a.query + b * a.query_seq_stride + ((uint64_t)(min(h, a.kv_heads - 1) * a.group + j0 + g) * D + 8 * q4) * 2;
+      auto load8 = [&](float (&x)[8], int r) {
+        if (!mine) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = 0.f;
+        } else if (a.align >= 16) {
+          const uint4 v = *reinterpret_cast<const uint4 *>(src + r * 64);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) unpack2<T>(w[i], x[2 * i], x[2 * i + 1]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(reinterpret_cast<const T *>(src + r * 64)[i]);
+        }
+      };
+      float top = 0.f;
+#pragma unroll
+      for (int r = 0; r < G; ++r) {
+        float x[8];
+        load8(x, r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // A power of two brings the head's largest |q| into [2^5, 2^6): 16 q (for the low nibbles) and 8 times a sum of 32
+      // stay below fp16's largest, and smaller ones keep 11 bits down to 2^-19 of it.
+      int ex = (int)((__float_as_uint(top) >> 23) & 255u) - 127 - 5;
+      ex = top == 0.f ? 0 : (ex < -110 ? -110 : (ex > 123 ? 123 : ex));
+      const float down = __uint_as_float((uint32_t)(127 - ex) << 23), up = __uint_as_float((uint32_t)(127 + ex) << 23);
+      // k index of the offset product: groups' high halves at 0 .. G-1, low halves at G .. 2G-1
+      const int r0 = G == 8 ? 2 * (int)q4 : (G == 4 ? 2 * (int)(q4 & 1) : 0);
+      const bool low = G == 4 ? q4 >= 2 : q4 == 1;
+      float pick0 = 0.f, pick1 = 0.f;
+#pragma unroll
+      for (int r = 0; r < G; ++r) {
+        float x[8], sum = 0.f;
+        load8(x, r);  // a second read, from L1, costs less than the registers
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[i] = __half2float(__float2half_rn(x[i] * down));
+          sum += x[i];
+        }
+        qf[r][0] = pack_half2(16.f * x[0], 16.f * x[4]);
+        qf[r][1] = pack_half2(x[1], x[5]);
+        qf[r][2] = pack_half2(16.f * x[2], 16.f * x[6]);
+        qf[r][3] = pack_half2(x[3], x[7]);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if (r == r0) pick0 = sum;
+        if (r == r0 + 1) pick1 = sum;
+      }
+      const uint32_t hi = pack_half2(pick0, pick1);
+      const float2 rounded = unpack_half2(hi);
+      const uint32_t rest = pack_half2(pick0 - rounded.x, pick1 - rounded.y);
+      const uint32_t eight = 0xc800c800u;  // -8, -8
+      if constexpr (G == 8) {
+        qo[0] = hi;
+        qo[1] = rest;
+        qc[0] = mul_half2(hi, eight);
+        qc[1] = mul_half2(rest, eight);
+      } else {  // one product: offsets in k 0 .. 7, scales in k 8 .. 15
+        qo[0] = G == 4 || q4 < 2 ? (low ? rest : hi) : 0u;
+        qo[1] = mul_half2(qo[0], eight);
+        qc[0] = qc[1] = 0;
+      }
+      const float c = up * a.scale_log2;
+      c0 = __shfl_sync(0xffffffffu, c, 8 * q4);
+      c1 = __shfl_sync(0xffffffffu, c, 8 * q4 + 4);
+    }
+
+    float acc[G][2][4], accx[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < G; ++r)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[r][i][k] = 0.f;
+    float ref0 = kFirstRef, ref1 = kFirstRef, sum0 = 0.f, sum1 = 0.f;
+    float lift = 8.f;  // p is held times 2^lift
+    float *lg = a.score_base && active
+                    ? a.logits + ((uint64_t)b * a.kv_heads * a.group + (uint64_t)h * a.group + j0 + 2 * q4) * a.logit_stride
+                    : nullptr;
+    const bool store0 = lg && j0 + 2 * q4 < a.group, store1 = lg && j0 + 2 * q4 + 1 < a.group;
+
+    // Moves the references of this lane's two heads and everything held relative to them.
+    auto rescale = [&](float to0, float to1) {
+      const float f0 = ex2(ref0 - to0), f1 = ex2(ref1 - to1);
+      ref0 = to0;
+      ref1 = to1;
+      sum0 *= f0;
+      sum1 *= f1;
+#pragma unroll
+      for (int r = 0; r < G; ++r)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          acc[r][i][0] *= f0;
+          acc[r][i][1] *= f1;
+          acc[r][i][2] *= f0;
+          acc[r][i][3] *= f1;
+        }
+      accx[0] *= f0;
+      accx[1] *= f1;
+      accx[2] *= f0;
+      accx[3] *= f1;
+    };
+
+    for (uint32_t k = 0; k < count; ++k) {
+      if (ok) {
+        ok = mbar_wait_bounded(smem_u32(&bar_full[stage]), parity, a.wait_limit_ns);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok && lane == 0) {
+          report(a.status, kStatusTimeout, (long long)blockIdx.x);
+          *(volatile int *)&aborted = 1;
+        }
+      }
+      const uint32_t mask = ok && active ? valid[stage][t_sub / 32] >> (t_sub % 32) & 0xffffu : 0u;
+      if (mask) {
+        const uint32_t base = ring + stage * stage_bytes;
+        // ---- logits of 16 tokens
+        float l[4];
+        {
+          uint32_t w0[KW], w1[KW], s0[SW], s1[SW];
+          const uint32_t ka = base + k_off, kb = ka + 8 * sh.ts;
+          lds_words(w0, ka + q4 * (D / 8));
+          lds_words(w1, kb + q4 * (D / 8));
+          lds_words(s0, ka + D / 2);
+          lds_words(s1, kb + D / 2);
+          float d0[4] = {0.f, 0.f, 0.f, 0.f};
+          {
+            const uint32_t wo = G == 8 ? q4 : (G == 4 ? (q4 & 1) : 0);  // word of two groups
+            const uint32_t o0 = lds32(ka + D / 2 + 2 * G + 4 * wo), o1 = lds32(kb + D / 2 + 2 * G + 4 * wo);
+            if constexpr (G == 8) {
+              const uint32_t e0 = lds32(ka + D / 2 + 4 * wo), e1 = lds32(kb + D / 2 + 4 * wo);
+              mma_k16(d0, o0, o1, o0, o1, qo[0], qo[1], d0);
+              mma_k16(d0, e0, e1, e0, e1, qc[0], qc[1], d0);
+            } else {
+              const uint32_t e0 = G == 4 && (q4 & 1) ? s0[SW - 1] : s0[0], e1 = G == 4 && (q4 & 1) ? s1[SW - 1] : s1[0];
+              mma_k16(d0, o0, o1, e0, e1, qo[0], qo[1], d0);
+            }
+          }
+          float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int r = 0; r < G; ++r) {
+            const uint32_t sel = r % 2 ? kHiHalves : kLoHalves;
+            const uint32_t u0 = __byte_perm(w0[r / 2], w0[KW / 2 + r / 2], sel), u1 = __byte_perm(w1[r / 2], w1[KW / 2 + r / 2], sel);
+            const uint32_t y0 = u0 >> 8, y1 = u1 >> 8;
+            float m[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_k16(m, u0 & kNib0, u1 & kNib0, u0 & kNib1, u1 & kNib1, qf[r][0], qf[r][1], m);
+            mma_k16(m, y0 & kNib0, y1 & kNib0, y0 & kNib1, y1 & kNib1, qf[r][2], qf[r][3], m);
+            const float2 f0 = unpack_half2(s0[r / 2]), f1 = unpack_half2(s1[r / 2]);
+            const float e0 = r % 2 ? f0.y : f0.x, e1 = r % 2 ? f1.y : f1.x;
+            x[0] = fmaf(e0, m[0], x[0]);
+            x[1] = fmaf(e0, m[1], x[1]);
+            x[2] = fmaf(e1, m[2], x[2]);
+            x[3] = fmaf(e1, m[3], x[3]);
+          }
+          l[0] = c0 * fmaf(x[0], 0x1p20f, d0[0]);
+          l[1] = c1 * fmaf(x[1], 0x1p20f, d0[1]);
+          l[2] = c0 * fmaf(x[2], 0x1p20f, d0[2]);
+          l[3] = c1 * fmaf(x[3], 0x1p20f, d0[3]);
+        }
+        if (mask != 0xffffu) {
+          if (!(mask >> tk & 1)) l[0] = l[1] = -INFINITY;
+          if (!(mask >> (tk + 8) & 1)) l[2] = l[3] = -INFINITY;
+        }
+        if (lg) {
+          const uint32_t t = (unit0 + k) * sh.tokens + t_sub + tk;
+          if (t < n) {
+            if (store0) lg[t] = l[0];
+            if (store1) lg[a.logit_stride + t] = l[1];
+          }
+          if (t + 8 < n) {
+            if (store0) lg[t + 8] = l[2];
+            if (store1) lg[a.logit_stride + t + 8] = l[3];
+          }
+        }
+        // ---- scales of the value rows; from the first one >= 2 (bit 14 of an fp16) p is held smaller
+        uint32_t sv[4][SW];  // tokens tv0, tv1, tv0 + 8, tv1 + 8
+        uint32_t ov[4];      // offsets of group g at the same tokens
+        const uint32_t va = base + v_off0, vb = base + v_off1;
+        lds_words(sv[0], va + D / 2);
+        lds_words(sv[1], vb + D / 2);
+        lds_words(sv[2], va + 8 * sh.ts + D / 2);
+        lds_words(sv[3], vb + 8 * sh.ts + D / 2);
+        const uint32_t oa = D / 2 + 2 * G + 2 * (g & (G - 1));
+        ov[0] = lds16(va + oa);
+        ov[1] = lds16(vb + oa);
+        ov[2] = lds16(va + 8 * sh.ts + oa);
+        ov[3] = lds16(vb + 8 * sh.ts + oa);
+        if (mask != 0xffffu) {
+          const uint32_t t[4] = {tv0, tv1, tv0 + 8, tv1 + 8};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!(mask >> t[i] & 1)) {
+              ov[i] = 0;
+#pragma unroll
+              for (int w = 0; w < SW; ++w) sv[i][w] = 0;
+            }
+        }
+        uint32_t big = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int w = 0; w < SW; ++w) big |= sv[i][w];
+        const bool lower = (big & 0x40004000u) != 0 && lift > 0.f;
+        // ---- weights; the reference follows the maximum only when it is left 2^6 behind
+        float p[4] = {l[0] - ref0, l[1] - ref1, l[2] - ref0, l[3] - ref1};
+        const float most = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
+        if (__any_sync(0xffffffffu, most > lift + 6.f || lower)) {
+          if (__any_sync(0xffffffffu, lower)) {
+            rescale(ref0 == kFirstRef ? ref0 : ref0 + lift + 4.f, ref1 == kFirstRef ? ref1 : ref1 + lift + 4.f);
+            lift = -4.f;
+          }
+          float m0 = fmaxf(l[0], l[2]), m1 = fmaxf(l[1], l[3]);
+#pragma unroll
+          for (int s = 4; s < 32; s <<= 1) {
+            m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, s));
+            m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, s));
+          }
+          rescale(fmaxf(ref0, m0 - lift), fmaxf(ref1, m1 - lift));
+          p[0] = l[0] - ref0;
+          p[1] = l[1] - ref1;
+          p[2] = l[2] - ref0;
+          p[3] = l[3] - ref1;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = ex2(p[i]);
+        sum0 += p[0] + p[2];
+        sum1 += p[1] + p[3];
+        const uint32_t h01 = pack_half2(p[0], p[1]), h23 = pack_half2(p[2], p[3]);
+        const uint32_t b0 = transpose8(h01), b1 = transpose8(h23);
+        uint32_t bl0 = 0, bl1 = 0;
+        if constexpr (kPrecise) {
+          const float2 r01 = unpack_half2(h01), r23 = unpack_half2(h23);
+          bl0 = transpose8(pack_half2(p[0] - r01.x, p[1] - r01.y));
+          bl1 = transpose8(pack_half2(p[2] - r23.x, p[3] - r23.y));
+        }
+        // ---- sum p o_r in rows 8 .. of accx
+        {
+          const uint32_t o01 = ov[0] | ov[1] << 16, o23 = ov[2] | ov[3] << 16;
+          mma_k16(accx, 0u, o01, 0u, o23, b0, b1, accx);
+          if constexpr (kPrecise) mma_k16(accx, 0u, o01, 0u, o23, bl0, bl1, accx);
+        }
+        // ---- values
+        uint32_t w[4][VW];
+        lds_words(w[0], va + g * (D / 16));
+        lds_words(w[1], vb + g * (D / 16));
+        lds_words(w[2], va + 8 * sh.ts + g * (D / 16));
+        lds_words(w[3], vb + 8 * sh.ts + g * (D / 16));
+#pragma unroll
+        for (int r = 0; r < G; ++r) {
+          const uint32_t sel = r % 2 ? kHiHalves : kLoHalves;
+          const uint32_t s01 = __byte_perm(sv[0][r / 2], sv[1][r / 2], sel), s23 = __byte_perm(sv[2][r / 2], sv[3][r / 2], sel);
+          const uint32_t e0 = mul_half2(b0, s01), e1 = mul_half2(b1, s23);
+          const uint32_t u01 = __byte_perm(w[0][r / 2], w[1][r / 2], sel), u23 = __byte_perm(w[2][r / 2], w[3][r / 2], sel);
+          const uint32_t y01 = u01 >> 8, y23 = u23 >> 8;
+          const uint32_t one = g == (uint32_t)r ? 0x3c003c00u : 0u;
+          mma_k16(acc[r][0], u01 & kNib0, u01 & kNib1, u23 & kNib0, u23 & kNib1, e0, e1, acc[r][0]);
+          mma_k16(acc[r][1], y01 & kNib0, y01 & kNib1, y23 & kNib0, y23 & kNib1, e0, e1, acc[r][1]);
+          mma_k16(accx, one, 0u, one, 0u, e0, e1, accx);
+          if constexpr (kPrecise) {
+            const uint32_t f0 = fma_half2(bl0, s01, fma_half2(b0, s01, e0 ^ 0x80008000u));
+            const uint32_t f1 = fma_half2(bl1, s23, fma_half2(b1, s23, e1 ^ 0x80008000u));
+            mma_k16(acc[r][0], u01 & kNib0, u01 & kNib1, u23 & kNib0, u23 & kNib1, f0, f1, acc[r][0]);
+            mma_k16(acc[r][1], y01 & kNib0, y01 & kNib1, y23 & kNib0, y23 & kNib1, f0, f1, acc[r][1]);
+            mma_k16(accx, one, 0u, one, 0u, f0, f1, accx);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bar_empty[stage]));
+      advance();
+      // Refill the stage of the unit before this one: the other warps have most likely left it.
+      ++done;
+      if (done >= 2 && turn == done + sh.stages - 2 && turn < all) issue();
+    }
+
+    // ---- the segment's result: o[r][i] of channel 32 r + 4 g + i, heads 2 q4 and 2 q4 + 1
+#pragma unroll
+    for (int s = 4; s < 32; s <<= 1) {
+      sum0 += __shfl_xor_sync(0xffffffffu, sum0, s);
+      sum1 += __shfl_xor_sync(0xffffffffu, sum1, s);
+    }
+#pragma unroll
+    for (int r = 0; r < G; ++r) {
+      const float x0 = __shfl_sync(0xffffffffu, accx[2], 4 * r + q4) - 8.f * __shfl_sync(0xffffffffu, accx[0], 4 * r + q4);
+      const float x1 = __shfl_sync(0xffffffffu, accx[3], 4 * r + q4) - 8.f * __shfl_sync(0xffffffffu, accx[1], 4 * r + q4);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        acc[r][i][0] = fmaf(acc[r][i][0], 0x1p24f, x0);
+        acc[r][i][1] = fmaf(acc[r][i][1], 0x1p24f, x1);
+        acc[r][i][2] = fmaf(acc[r][i][2], 0x1p20f, x0);
+        acc[r][i][3] = fmaf(acc[r][i][3], 0x1p20f, x1);
+      }
+    }
+    if (sh.subsets > 1) {
+      // The subsets' results meet in the first subset's warp, through shared memory, one after the other.
+      const uint32_t per = sh.heads_cta * sh.ntiles;
+      float *slot = merge + (uint64_t)(warp % per + (sub ? sub - 1 : 0) * per) * 8 * (D + 2);
+      if (sub) {
+#pragma unroll
+        for (int r = 0; r < G; ++r) {
+          float *o0 = slot + (2 * q4) * (D + 2) + 32 * r + 4 * g, *o1 = o0 + (D + 2);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            *reinterpret_cast<float2 *>(o0 + 2 * i) = make_float2(acc[r][i][0], acc[r][i][2]);
+            *reinterpret_cast<float2 *>(o1 + 2 * i) = make_float2(acc[r][i][1], acc[r][i][3]);
+          }
+        }
+        if (g == 0) {
+          *reinterpret_cast<float2 *>(slot + (2 * q4) * (D + 2) + D) = make_float2(ref0, sum0);
+          *reinterpret_cast<float2 *>(slot + (2 * q4 + 1) * (D + 2) + D) = make_float2(ref1, sum1);
+        }
+      }
+      __syncthreads();
+      if (sub == 0) {
+        for (uint32_t s = 1; s < sh.subsets; ++s) {
+          const float *from = merge + (uint64_t)(warp % per + (s - 1) * per) * 8 * (D + 2);
+          const float2 ml0 = *reinterpret_cast<const float2 *>(from + (2 * q4) * (D + 2) + D);
+          const float2 ml1 = *reinterpret_cast<const float2 *>(from + (2 * q4 + 1) * (D + 2) + D);
+          const float to0 = fmaxf(ref0, ml0.x), to1 = fmaxf(ref1, ml1.x);
+          const float a0 = ex2(ref0 - to0), a1 = ex2(ref1 - to1), f0 = ex2(ml0.x - to0), f1 = ex2(ml1.x - to1);
+          ref0 = to0;
+          ref1 = to1;
+          sum0 = sum0 * a0 + ml0.y * f0;
+          sum1 = sum1 * a1 + ml1.y * f1;
+#pragma unroll
+          for (int r = 0; r < G; ++r) {
+            const float *o0 = from + (2 * q4) * (D + 2) + 32 * r + 4 * g, *o1 = o0 + (D + 2);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float2 v0 = *reinterpret_cast<const float2 *>(o0 + 2 * i), v1 = *reinterpret_cast<const float2 *>(o1 + 2 * i);
+              acc[r][i][0] = acc[r][i][0] * a0 + v0.x * f0;
+              acc[r][i][2] = acc[r][i][2] * a0 + v0.y * f0;
+              acc[r][i][1] = acc[r][i][1] * a1 + v1.x * f1;
+              acc[r][i][3] = acc[r][i][3] * a1 + v1.y * f1;
+            }
+          }
+        }
+      }
+      __syncthreads();  // the buffer is free for the next segment
+    }
+    const bool whole = count == units;
+    if (sub == 0 && active && ok) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint32_t j = j0 + 2 * q4 + c;
+        if (j >= a.group) continue;
+        const float sum = c ? sum1 : sum0, ref = c ? ref1 : ref0;
+        const uint64_t head = (uint64_t)h * a.group + j;
+        if (whole) {
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no token counts: zeros
+          T *out = reinterpret_cast<T *>(a.out + b * a.out_seq_stride) + head * D + 4 * g;
+#pragma unroll
+          for (int r = 0; r < G; ++r) {
+            if (a.align >= 8) {
+              *reinterpret_cast<uint2 *>(out + 32 * r) = make_uint2(pack2<T>(acc[r][0][c] * inv, acc[r][0][2 + c] * inv),
+                                                                    pack2<T>(acc[r][1][c] * inv, acc[r][1][2 + c] * inv));
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) out[32 * r + i] = from_f32<T>(acc[r][i / 2][2 * (i % 2) + c] * inv);
+            }
+          }
+          if (lg && g == 0) a.lse[(uint64_t)b * a.kv_heads * a.group + head] = sum == 0.f ? INFINITY : ref + lg2(sum);
+        } else {
+          const uint64_t slot = 2ull * blockIdx.x + (unit0 == 0 ? 1 : 0);
+          const uint64_t row = slot * sh.heads_cta * a.group + hl * a.group + j;
+          float *o = a.part_o + row * D + 4 * g;
+#pragma unroll
+          for (int r = 0; r < G; ++r)
+            *reinterpret_cast<float4 *>(o + 32 * r) = make_float4(acc[r][0][c], acc[r][0][2 + c], acc[r][1][c], acc[r][1][2 + c]);
+          if (g == 0) a.part_ml[row] = make_float2(ref, sum);
+        }
+      }
+    }
+    if (tid == 0 && unit0 + count == units) {
+      // This CTA ends the item: say where it began.
+      const uint64_t end = share.first + (share.count - left) + count;          // units up to the item's end
+      const uint64_t begin = end - units;
+      const uint32_t from = (uint32_t)(((begin + 1) * share.grid - 1) / share.total);  // the CTA that has unit `begin`
+      const uint32_t item = b * sh.head_groups + hg;
+      a.item_span[item] = make_int2((int)from, (int)blockIdx.x);
+      if (!whole) a.cta_item[blockIdx.x] = (int)item;
+    }
+    left -= count;
+    unit = 0;
+    if (++hg == sh.head_groups) {
+      hg = 0;
+      ++b;
+    }
   }
   __syncthreads();
-  for (uint32_t j = 0; j < a.group; ++j) {
-    float m = -1e30f, z = 0.f;
-    for (uint32_t t = threadIdx.x; t < n; t += 256) m = fmaxf(m, lg[(uint64_t)j * a.max_len + t]);
-    for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-    if (lane == 0) red[warp] = m;
-    __syncthreads();
-    for (int k = 0; k < 8; ++k) m = fmaxf(m, red[k]);
-    __syncthreads();
-    for (uint32_t t = threadIdx.x; t < n; t += 256) z += exp2f(lg[(uint64_t)j * a.max_len + t] - m);
-    for (int k = 16; k; k >>= 1) z += __shfl_xor_sync(0xffffffffu, z, k);
-    if (lane == 0) red[warp] = z;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      z = 0.f;
-      for (int k = 0; k < 8; ++k) z += red[k];
-      stat[2 * j] = m;
-      stat[2 * j + 1] = z > 0.f ? 1.f / z : (z == 0.f ? 0.f : z);
-    }
-    __syncthreads();
-    for (uint32_t t = threadIdx.x; t < n; t += 256) {
-      float &l = lg[(uint64_t)j * a.max_len + t];
-      l = exp2f(l - stat[2 * j]) * stat[2 * j + 1];
-    }
+  if (aborted && tid == 0) {
+    // Loads may still be landing in this CTA's shared memory: one more bounded wait for each stage.
+    for (uint32_t s = 0; s < sh.stages; ++s)
+      if (used[s] && !mbar_wait_bounded(smem_u32(&bar_full[s]), (used[s] - 1) & 1, a.wait_limit_ns)) break;
   }
+}
+
+// Adds the partial results of an item that several CTAs worked on. grid.x: items, or (by_cta) the CTAs that finished
+// one; grid.y: query heads of an item. A warp takes every eighth part, four channels (or two) per lane.
+constexpr int kJoinWarps = 8;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinWarps * 32) attend_join(const __grid_constant__ AttendArgs a, const uint32_t by_cta) {
+  constexpr int C = D / 32;  // channels per lane
+  __shared__ float red[kJoinWarps][2];
+  __shared__ float o[kJoinWarps][D];
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, y = blockIdx.y;
+  int item = (int)blockIdx.x;
+  if (by_cta) item = a.cta_item[blockIdx.x];
+  if (item < 0) return;
+  const int2 span = a.item_span[item];
+  if (span.x == span.y) return;
+  const uint32_t b = item / a.sh.head_groups, hg = item % a.sh.head_groups;
+  const uint32_t h = hg * a.sh.heads_cta + y / a.group;
+  if (h >= a.kv_heads) return;
+  const uint32_t parts = (uint32_t)(span.y - span.x) + 1, rows = a.sh.heads_cta * a.group;
+  auto row_of = [&](uint32_t i) { return (2ull * (span.x + i) + (i == 0 ? 1 : 0)) * rows + y; };
+  float top = kFirstRef;
+  for (uint32_t i = threadIdx.x; i < parts; i += kJoinWarps * 32) top = fmaxf(top, a.part_ml[row_of(i)].x);
+#pragma unroll
+  for (int m = 16; m; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+  if (lane == 0) red[warp][0] = top;
   __syncthreads();
-  if (a.score_base) {
-    for (uint32_t t = threadIdx.x; t < n; t += 256) {
-      const int32_t id = block_of(a, b, t, false);
-      if (id < 0) continue;
-      float w = 0.f;
-      for (uint32_t j = 0; j < a.group; ++j) w += lg[(uint64_t)j * a.max_len + t];
-      float *sc = reinterpret_cast<float *>(a.score_base + (uint64_t)id * a.score_block_stride) + h * a.pool.block_size +
-                  t % a.pool.block_size;
-      *sc += w;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, red[w][0]);
+  float acc[C], sum = 0.f;
+#pragma unroll
+  for (int c = 0; c < C; ++c) acc[c] = 0.f;
+#pragma unroll 4
+  for (uint32_t i = warp; i < parts; i += kJoinWarps) {
+    const uint64_t row = row_of(i);
+    const float2 ml = a.part_ml[row];
+    const float f = ex2(ml.x - top);
+    sum = fmaf(ml.y, f, sum);
+    const float *src = a.part_o + row * D + lane * C;
+    float v[C];
+    if constexpr (C == 2) {
+      *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(src);
+    } else {
+#pragma unroll
+      for (int c = 0; c < C; c += 4) *reinterpret_cast<float4 *>(v + c) = *reinterpret_cast<const float4 *>(src + c);
     }
+#pragma unroll
+    for (int c = 0; c < C; ++c) acc[c] = fmaf(v[c], f, acc[c]);
   }
-  for (uint32_t i = threadIdx.x; i < a.group * D; i += 256) {
-    const uint32_t j = i / D, d = i % D;
-    float acc = 0.f;
-    for (uint32_t t = 0; t < n; ++t) {
-      const int32_t id = block_of(a, b, t, false);
-      if (id >= 0) acc += lg[(uint64_t)j * a.max_len + t] * q4_value<D>(row_of(t, id, 1), d);
-    }
-    reinterpret_cast<T *>(a.out + b * a.out_seq_stride)[(h * a.group + j) * D + d] = from_f32<T>(acc);
+#pragma unroll
+  for (int c = 0; c < C; ++c) o[warp][lane * C + c] = acc[c];
+  if (lane == 0) red[warp][1] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) sum += red[w][1];
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const uint64_t head = (uint64_t)h * a.group + y % a.group;
+  if (threadIdx.x < D) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) v += o[w][threadIdx.x];
+    reinterpret_cast<T *>(a.out + b * a.out_seq_stride)[head * D + threadIdx.x] = from_f32<T>(v * inv);
+  }
+  if (threadIdx.x == 0 && a.score_base)
+    a.lse[(uint64_t)b * a.kv_heads * a.group + head] = sum == 0.f ? INFINITY : top + lg2(sum);
+}
+
+// Adds every token's weight to its score. grid.x: chunks of 256 tokens, grid.y: (sequence, KV head) pairs.
+__global__ void __launch_bounds__(256) attend_scores(const __grid_constant__ AttendArgs a) {
+  __shared__ float lse[64];
+  grid_launch_dependents();
+  grid_dependency_wait();
+  for (uint32_t bh = blockIdx.y; bh < a.num_seqs * a.kv_heads; bh += gridDim.y) {
+    const uint32_t b = bh / a.kv_heads, h = bh % a.kv_heads;
+    const uint32_t n = seq_length(a, b, false), t = blockIdx.x * 256 + threadIdx.x;
+    if (blockIdx.x * 256 >= n) continue;
+    const uint64_t head = ((uint64_t)b * a.kv_heads + h) * a.group;
+    __syncthreads();
+    if (threadIdx.x < a.group) lse[threadIdx.x] = a.lse[head + threadIdx.x];
+    __syncthreads();
+    if (t >= n) continue;
+    const int32_t id = a.tables[b * a.table_stride + t / a.pool.block_size];
+    if ((uint32_t)id >= a.pool.num_blocks) continue;
+    float w = 0.f;
+    for (uint32_t j = 0; j < a.group; ++j) w += ex2(a.logits[(head + j) * a.logit_stride + t] - lse[j]);
+    float *sc = reinterpret_cast<float *>(a.score_base + (uint64_t)id * a.score_block_stride) +
+                (uint64_t)h * a.pool.block_size + t % a.pool.block_size;
+    *sc += w;
   }
 }
 

@@ -125,8 +125,123 @@ int q4_rows_impl(emm_pool *pool, bool append, int32_t D, int32_t dtype, int32_t 
   return EMM_OK;
 }
 
-uint64_t attend_workspace(const emm_pool *pool, int32_t B, int32_t Hq, int32_t max_len) {
-  return (uint64_t)B * (uint64_t)Hq * (uint64_t)max_len * sizeof(float);
+// How a call's work is laid out; see attend.cuh. A rule on heads and strides only.
+int attend_shape(const emm_pool *pool, int32_t D, int32_t B, int32_t group, int32_t max_len, emm::AttendShape *out,
+                 int *smem_out) {
+  const emm_pool_desc &d = pool->desc;
+  const uint32_t R = (uint32_t)emm::q4_row_bytes(D), H = (uint32_t)d.num_kv_heads;
+  emm::AttendShape s;
+  s.ntiles = (uint32_t)(group + 7) / 8;
+  // Eight warps at most: KV heads first (their rows of a token are one copy), equal shares of them, then
+  // the tokens of a unit in as many subsets as are left.
+  const uint32_t most = std::max(1u, 8u / s.ntiles);
+  s.head_groups = (H + most - 1) / most;
+  s.heads_cta = (H + s.head_groups - 1) / s.head_groups;
+  s.subsets = std::max(1u, 8u / (s.heads_cta * s.ntiles));
+  s.tokens = 16 * s.subsets;
+  s.warps = s.heads_cta * s.ntiles * s.subsets;
+  const bool token_major = d.head_stride == (int64_t)R && !(H == 1 && d.token_stride == (int64_t)R);
+  if (token_major) {
+    s.run = 1;
+    s.copy_heads = 1;
+    const uint32_t lines = (s.heads_cta * R + 31) / 32;
+    s.ts = 32 * (lines | 1u);  // 32 * odd: the fragment rows' loads fall into different banks
+    s.hs = R;
+    s.plane_bytes = s.tokens * s.ts;
+  } else {
+    s.run = 1;
+    if (d.token_stride == (int64_t)R)
+      while (s.run < 16 && d.block_size % (2 * (int)s.run) == 0) s.run *= 2;
+    s.copy_heads = s.heads_cta;
+    s.ts = R;
+    s.hs = s.tokens * R;
+    s.plane_bytes = s.heads_cta * s.hs;
+  }
+  const int per_sm = D == 256 ? 1 : 2;
+  const int budget = std::min(pool->ctx->max_smem_optin, 228 * 1024 / per_sm) - 4096;
+  const int merge = (int)((s.subsets - 1) * s.heads_cta * s.ntiles * 8 * (uint32_t)(D + 2) * 4);
+  s.stages = (uint32_t)std::min(16, (budget - merge) / (int)(2 * s.plane_bytes));
+  if (s.stages < 2) return fail(EMM_ERR_TOO_LARGE, "q4_attend: a unit of %u bytes does not fit shared memory", 2 * s.plane_bytes);
+  *smem_out = (int)(s.stages * 2 * s.plane_bytes) + merge;
+  s.items = (uint32_t)B * s.head_groups;
+  s.min_units = 2;
+  const uint64_t units = std::max<uint64_t>(1, ((uint64_t)max_len + s.tokens - 1) / s.tokens) * s.items;
+  s.grid = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(units / s.min_units, (uint64_t)pool->ctx->sm_count * per_sm));
+  *out = s;
+  return EMM_OK;
+}
+
+struct AttendWorkspace {
+  uint64_t part_o, part_ml, item_span, cta_item, lse, logits, logit_stride, bytes;
+};
+
+AttendWorkspace attend_workspace(const emm::AttendShape &s, int32_t D, int32_t B, int32_t Hq, int32_t group, int32_t max_len,
+                                 bool scores) {
+  AttendWorkspace w;
+  uint64_t at = 0;
+  auto take = [&](uint64_t bytes) {
+    const uint64_t p = at;
+    at += (bytes + 255) / 256 * 256;
+    return p;
+  };
+  const uint64_t rows = 2ull * s.grid * s.heads_cta * (uint32_t)group;
+  w.part_o = take(rows * (uint32_t)D * 4);
+  w.part_ml = take(rows * 8);
+  w.item_span = take((uint64_t)s.items * 8);
+  w.cta_item = take((uint64_t)s.grid * 4);
+  w.lse = take(scores ? (uint64_t)B * Hq * 4 : 0);
+  w.logit_stride = ((uint64_t)max_len + 7) / 8 * 8;
+  w.logits = take(scores ? (uint64_t)B * Hq * w.logit_stride * 4 : 0);
+  w.bytes = at;
+  return w;
+}
+
+// The kernel's dynamic shared memory is raised to the device's limit once per device.
+template <typename T, int D>
+int attend_smem(int device, int smem) {
+  static std::atomic<int> limit[kMaxTrackedDevices];
+  const bool tracked = device >= 0 && device < kMaxTrackedDevices;
+  if (tracked && limit[device].load(std::memory_order_acquire) >= smem) return EMM_OK;
+  int most = 0;
+  EMM_CUDA(cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, device));
+  cudaFuncAttributes fa;
+  EMM_CUDA(cudaFuncGetAttributes(&fa, emm::attend_q4<T, D>));
+  most -= (int)fa.sharedSizeBytes;
+  if (smem > most) return fail(EMM_ERR_TOO_LARGE, "q4_attend: %d bytes of shared memory, the device has %d", smem, most);
+  EMM_CUDA(cudaFuncSetAttribute(emm::attend_q4<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+  if (tracked) limit[device].store(most, std::memory_order_release);
+  return EMM_OK;
+}
+
+template <typename T, int D>
+int attend_launch(emm_ctx *ctx, const emm::AttendArgs &a, int smem, cudaStream_t st) {
+  if (int rc = attend_smem<T, D>(ctx->device, smem)) return rc;
+  emm::attend_q4<T, D><<<a.sh.grid, a.sh.warps * 32, smem, st>>>(a);
+  EMM_CUDA(cudaGetLastError());
+  ctx->launches += 1;
+  // The two small kernels behind it are placed while it drains.
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctx->pdl ? 1 : 0;
+  if (a.sh.grid > 1) {  // one CTA splits nothing
+    const bool by_cta = a.sh.items > a.sh.grid;
+    cfg.gridDim = dim3(by_cta ? a.sh.grid : a.sh.items, a.sh.heads_cta * a.group);
+    cfg.blockDim = dim3(emm::kJoinWarps * 32);
+    EMM_CUDA(cudaLaunchKernelEx(&cfg, emm::attend_join<T, D>, a, (uint32_t)by_cta));
+    ctx->launches += 1;
+  }
+  if (a.score_base && a.max_len > 0) {
+    const uint64_t pairs = (uint64_t)a.num_seqs * a.kv_heads;
+    cfg.gridDim = dim3((a.max_len + 255) / 256, (unsigned)std::min<uint64_t>(pairs, 65535));
+    cfg.blockDim = dim3(256);
+    EMM_CUDA(cudaLaunchKernelEx(&cfg, emm::attend_scores, a));
+    ctx->launches += 1;
+  }
+  return EMM_OK;
 }
 
 }  // namespace
@@ -150,13 +265,18 @@ int emm_q4_read(emm_pool *pool, int32_t head_dim, int32_t dtype, int32_t layer_b
                       key_token_stride, value_layer_stride, value_token_stride, d_slot_mapping, num_tokens, stream);
 }
 
-int emm_q4_attend_workspace(emm_pool *pool, int32_t num_seqs, int32_t num_heads, int32_t max_len, int32_t with_scores,
-                            uint64_t *bytes) {
-  if (!pool || !bytes) return fail(EMM_ERR_BAD_ARG, "q4_attend_workspace: null argument");
-  if (num_seqs < 0 || num_heads <= 0 || max_len < 0 || num_heads % pool->desc.num_kv_heads)
-    return fail(EMM_ERR_BAD_ARG, "q4_attend_workspace: %d sequences, %d heads, length %d", num_seqs, num_heads, max_len);
-  (void)with_scores;
-  *bytes = attend_workspace(pool, num_seqs, num_heads, max_len);
+int emm_q4_attend_workspace(emm_pool *pool, int32_t head_dim, int32_t num_seqs, int32_t num_heads, int32_t max_len,
+                            int32_t with_scores, uint64_t *bytes) {
+  const char *what = "q4_attend_workspace";
+  if (!bytes) return fail(EMM_ERR_BAD_ARG, "%s: null argument", what);
+  if (int rc = check_q4_pool(pool, head_dim, what)) return rc;
+  const int32_t H = pool->desc.num_kv_heads;
+  if (num_seqs < 0 || num_heads <= 0 || max_len < 0 || num_heads % H || num_heads / H > EMM_MAX_QUERY_GROUP)
+    return fail(EMM_ERR_BAD_ARG, "%s: %d sequences, %d heads, length %d", what, num_seqs, num_heads, max_len);
+  emm::AttendShape sh;
+  int smem = 0;
+  if (int rc = attend_shape(pool, head_dim, num_seqs, num_heads / H, max_len, &sh, &smem)) return rc;
+  *bytes = attend_workspace(sh, head_dim, num_seqs, num_heads, num_heads / H, max_len, with_scores != 0).bytes;
   return EMM_OK;
 }
 
@@ -196,13 +316,17 @@ int emm_q4_attend(emm_pool *pool, int32_t head_dim, int32_t dtype, int32_t layer
                             num_seqs > 1 ? (uint64_t)out_seq_stride : 0};
   for (uint64_t v : parts) align = std::min(align, pow2_align(v));
   if (align < 2) return fail(EMM_ERR_ALIGN, "%s: query/out not aligned to their elements", what);
-  const uint64_t want = attend_workspace(pool, num_seqs, num_heads, max_len);
-  if (workspace_bytes < want || (want && !d_workspace))
-    return fail(EMM_ERR_LENGTH, "%s: workspace of %llu bytes, %llu needed", what, (unsigned long long)workspace_bytes,
-                (unsigned long long)want);
   if ((uint64_t)num_seqs * d.num_kv_heads > 0x7fffffffull) return fail(EMM_ERR_TOO_LARGE, "%s: %d sequences", what, num_seqs);
-
+  const int32_t group = num_heads / d.num_kv_heads;
   emm::AttendArgs a;
+  int smem = 0;
+  if (int rc = attend_shape(pool, head_dim, num_seqs, group, max_len, &a.sh, &smem)) return rc;
+  const AttendWorkspace w = attend_workspace(a.sh, head_dim, num_seqs, num_heads, group, max_len, scores != nullptr);
+  if (workspace_bytes < w.bytes || !d_workspace)
+    return fail(EMM_ERR_LENGTH, "%s: workspace of %llu bytes, %llu needed", what, (unsigned long long)workspace_bytes,
+                (unsigned long long)w.bytes);
+  if (pow2_align((uint64_t)d_workspace) < 16) return fail(EMM_ERR_ALIGN, "%s: workspace not on a 16-byte boundary", what);
+  const uint64_t ws = (uint64_t)d_workspace;
   a.pool = token_side(pool);
   a.layer_base = pool->h_layers[layer];
   a.query = (uint64_t)d_query;
@@ -214,29 +338,32 @@ int emm_q4_attend(emm_pool *pool, int32_t head_dim, int32_t dtype, int32_t layer
   a.lens = d_seq_lens;
   a.num_seqs = (uint32_t)num_seqs;
   a.kv_heads = (uint32_t)d.num_kv_heads;
-  a.group = (uint32_t)(num_heads / d.num_kv_heads);
+  a.group = (uint32_t)group;
   a.max_len = (uint32_t)max_len;
   a.scale_log2 = (float)(scale * 1.4426950408889634);
+  a.align = align;
   a.score_base = scores ? scores->h_layers[layer] : 0;
   a.score_block_stride = scores ? (uint64_t)scores->desc.block_stride : 0;
-  a.logits = (float *)d_workspace;
+  a.wait_limit_ns = pool->ctx->wait_limit_ns;
+  a.part_o = (float *)(ws + w.part_o);
+  a.part_ml = (float2 *)(ws + w.part_ml);
+  a.item_span = (int2 *)(ws + w.item_span);
+  a.cta_item = (int *)(ws + w.cta_item);
+  a.lse = (float *)(ws + w.lse);
+  a.logits = (float *)(ws + w.logits);
+  a.logit_stride = w.logit_stride;
   a.status = pool->ctx->d_status;
   DeviceGuard guard(pool->ctx->device);
   if (!guard.ok()) return fail(EMM_ERR_CUDA, "cannot select device %d", pool->ctx->device);
   cudaStream_t st = (cudaStream_t)stream;
-  const unsigned grid = (unsigned)num_seqs * (unsigned)d.num_kv_heads;
   if (dtype == EMM_DTYPE_FP16) {
-    if (head_dim == 64) emm::attend_q4<__half, 64><<<grid, 256, 0, st>>>(a);
-    else if (head_dim == 128) emm::attend_q4<__half, 128><<<grid, 256, 0, st>>>(a);
-    else emm::attend_q4<__half, 256><<<grid, 256, 0, st>>>(a);
-  } else {
-    if (head_dim == 64) emm::attend_q4<__nv_bfloat16, 64><<<grid, 256, 0, st>>>(a);
-    else if (head_dim == 128) emm::attend_q4<__nv_bfloat16, 128><<<grid, 256, 0, st>>>(a);
-    else emm::attend_q4<__nv_bfloat16, 256><<<grid, 256, 0, st>>>(a);
+    if (head_dim == 64) return attend_launch<__half, 64>(pool->ctx, a, smem, st);
+    if (head_dim == 128) return attend_launch<__half, 128>(pool->ctx, a, smem, st);
+    return attend_launch<__half, 256>(pool->ctx, a, smem, st);
   }
-  EMM_CUDA(cudaGetLastError());
-  pool->ctx->launches += 1;
-  return EMM_OK;
+  if (head_dim == 64) return attend_launch<__nv_bfloat16, 64>(pool->ctx, a, smem, st);
+  if (head_dim == 128) return attend_launch<__nv_bfloat16, 128>(pool->ctx, a, smem, st);
+  return attend_launch<__nv_bfloat16, 256>(pool->ctx, a, smem, st);
 }
 
 int emm_select_tokens(emm_pool *scores, const int32_t *d_block_tables, int64_t table_stride, int32_t table_width,

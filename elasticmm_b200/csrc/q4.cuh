@@ -4,7 +4,7 @@
 // offset o, both fp16, and channel x is the code c in 0..15 that stands for o + s * (c - 8):
 //
 //   lo, hi = min, max of the group, clamped to +-65504       s = fp16((hi - lo) / 15)       o = fp16(lo + 8 s)
-//   c = clamp(rint((x - o) / s) + 8, 0, 15), rint to even;  s == 0: c = 8;  a NaN in the group: s = o = NaN, c = 8
+//   c = clamp(rint((x - o) / s) + 8, 0, 15), rint to even;  s == 0: c = 8;  a NaN in the group: o = NaN, s = 0, c = 8
 //
 // The arithmetic is IEEE fp32 (one rounding per operation, no contraction), so a row's bytes do not depend on how the
 // kernel splits the work. s and o are rounded to fp16 because they are read for every group in every decode step
@@ -148,7 +148,10 @@ __global__ void __launch_bounds__(256) q4_append(const __grid_constant__ Q4RowsA
     c = c < 0 ? 0 : (c > 15 ? 15 : c);
     code |= (uint32_t)c << (4 * i);
   }
-  if (nan) s = o = __ushort_as_half((unsigned short)0x7fff);
+  if (nan) {
+    s = __ushort_as_half((unsigned short)0);
+    o = __ushort_as_half((unsigned short)0x7fff);
+  }
   const uint32_t r = unit / 8, u = unit % 8;
   uint8_t *dst = reinterpret_cast<uint8_t *>(row + (uint64_t)h * a.pool.head_stride);
   *reinterpret_cast<uint16_t *>(dst + 2 * (u * G + r)) = (uint16_t)code;

@@ -246,7 +246,8 @@ class KVPoolQ4(KVPool):
         if limit < 0 or limit > cap or limit > 0x7FFFFFFF:
             raise ValueError(f"max_len {limit} outside [0, {cap}], what the tables can hold")
         nbytes = C.c_uint64()
-        _lib.check(self.ctx._lib.emm_q4_attend_workspace(self._h, B, heads, limit, int(scores is not None), C.byref(nbytes)))
+        _lib.check(self.ctx._lib.emm_q4_attend_workspace(self._h, D, B, heads, limit, int(scores is not None),
+                                                             C.byref(nbytes)))
         dense = heads * D * 2
         qs = query.stride(0) * 2 if B > 1 else dense
         os_ = dense if out is None or B <= 1 else out.stride(0) * 2

@@ -342,7 +342,7 @@ int emm_append_unbind(emm_append_binding *binding);
  *   lo, hi = smallest, largest of the group, clamped to +-65504
  *   s = fp16((hi - lo) / 15), o = fp16(lo + 8*s)
  *   c = clamp(rint((x - o) / s) + 8, 0, 15)   (s == 0: c = 8; a NaN in the
- *       group makes s and o NaN, and the whole group reads back as NaN)
+ *       group makes o NaN and s 0, and the whole group reads back as NaN)
  * in fp32, each operation rounded to nearest even. Bytes: D/2 of codes, the
  * D/32 scales, the D/32 offsets, zeros up to a multiple of 16 (48, 80 and 160
  * bytes for the three D). The codes come in units of two bytes, four
@@ -391,8 +391,8 @@ int emm_q4_read(emm_pool *pool, int32_t head_dim, int32_t dtype, int32_t layer_b
  *
  * The workspace (emm_q4_attend_workspace bytes, 16-byte aligned) is scratch of
  * this call: calls that may overlap on the GPU need one each. */
-int emm_q4_attend_workspace(emm_pool *pool, int32_t num_seqs, int32_t num_heads, int32_t max_len, int32_t with_scores,
-                            uint64_t *bytes);
+int emm_q4_attend_workspace(emm_pool *pool, int32_t head_dim, int32_t num_seqs, int32_t num_heads, int32_t max_len,
+                            int32_t with_scores, uint64_t *bytes);
 int emm_q4_attend(emm_pool *pool, int32_t head_dim, int32_t dtype, int32_t layer, const void *d_query,
                   int64_t query_seq_stride, void *d_out, int64_t out_seq_stride, const int32_t *d_block_tables,
                   int64_t table_stride, int32_t table_width, const int32_t *d_seq_lens, int32_t num_seqs,

@@ -31,7 +31,7 @@ def encode_rows(x: np.ndarray) -> np.ndarray:
     c = np.clip(np.where(sf == 0, np.float32(0), q) + 8, 0, 15).astype(np.uint8)
     c[nan] = 8
     bits_s, bits_o = s.view(np.uint16).copy(), o.view(np.uint16).copy()
-    bits_s[nan] = bits_o[nan] = 0x7FFF
+    bits_s[nan], bits_o[nan] = 0, 0x7FFF
     out = np.zeros((N, row_bytes(D)), dtype=np.uint8)
     for d in range(D):
         r, u, i = d // GROUP, d % GROUP // 4, d % 4

@@ -87,7 +87,7 @@ def test_entries_refuse_null_pools():
     n = C.c_uint64()
     assert lib.emm_q4_append(None, 128, 0, 0, 1, None, None, 0, 0, 0, 0, None, 1, None) == _lib.ERR_BAD_ARG
     assert lib.emm_q4_read(None, 128, 0, 0, 1, None, None, 0, 0, 0, 0, None, 1, None) == _lib.ERR_BAD_ARG
-    assert lib.emm_q4_attend_workspace(None, 1, 8, 16, 0, C.byref(n)) == _lib.ERR_BAD_ARG
+    assert lib.emm_q4_attend_workspace(None, 128, 1, 8, 16, 0, C.byref(n)) == _lib.ERR_BAD_ARG
     assert lib.emm_q4_attend(None, 128, 0, 0, None, 0, None, 0, None, 0, 0, None, 1, 8, 16, 1.0, None, None, 0,
                              None) == _lib.ERR_BAD_ARG
     assert lib.emm_select_tokens(None, None, 0, 0, None, 1, 4, 0, 0, None, None, None) == _lib.ERR_BAD_ARG
