@@ -16,25 +16,25 @@
 // two operand elements. The two powers of two are undone in q (keys) or when the result is written (values).
 //
 // Scales and offsets, x = o + s (c - 8), group r of 32 channels:
-//   l[t]   = sum_r s_r[t] (sum_d q_d c_d) + sum_r (o_r[t] - 8 s_r[t]) Q_r,    Q_r = sum of q over the group
-//            the first bracket is two MMAs per group; the last sum is one MMA (two at D = 256) with the offsets and
-//            scales as rows and Q split into two fp16 halves (22 bits).
-//   out[d] = sum_t (p s_r) c_d - 8 sum_t (p s_r) + sum_t p o_r
-//            p s_r is formed per group as the 16-bit operand; the two sums are one MMA each, with rows of ones (the SAME
-//            rounded p s_r, so rounding enters only through s (c - 8), not through s c) and of offsets.
+//   l[t]   = sum_r s_r[t] (sum_d q_d c_d) + sum_r (o_r[t] - 8 s_r[t]) Q_r,      Q_r = sum of q over the group
+//            the first bracket is two MMAs per group; the last sum is one MMA (two at D = 256) with a token's scales and
+//            offsets, which lie side by side in its row, as the row operand and Q in two fp16 halves (22 bits).
+//   out[d] = sum_t (p s_r) c_d + sum_t p (o_r - 8 s_r)
+//            p s_r is formed per group as the 16-bit operand; the last sum is one MMA with scales and offsets as rows.
 // p is held relative to a reference that only follows the running maximum when that outgrows it by 2^6, so the
 // accumulators are rarely rescaled and no maximum is taken across lanes in between. p is scaled by 2^8 (by 2^-4 from
 // the first scale >= 2 on), which keeps p s_r below 2^15 and above fp16's subnormals down to 2^-22 of the largest.
-// With fp16 outputs the rounding of p s_r (2^-12 on average as large as the output's own) is halved again: its
-// remainder, exact by an fma, goes through the same MMAs. bf16 outputs are 8 times coarser and skip that.
+// fp16 outputs: p and p s_r rounded to fp16 (2^-12 each, times up to 15 s) would cost several times the output's own
+// rounding, so their remainders (exact by an fma) go through the same MMAs. bf16 outputs are 8 times coarser: without.
 // Logits, sums and accumulators are 32 bits.
 //
-// Work. A unit is 16 (x token subsets) tokens of one sequence for the KV heads of a CTA. The units of the whole batch,
-// counted on the device, are split evenly over the CTAs, whatever the lengths: a CTA finishes the sequences that
-// lie in its share and leaves a partial result (in the workspace) of the at most two that do not; attend_join adds those.
-// Rows come by cp.async.bulk into a ring of stages: per token (token-major pages: the heads of a CTA are one run) or
-// per run of tokens and head (head-major pages). The warps take turns at issuing a unit's copies; a warp of its own for
-// that would leave 96 instead of 128 registers to each of the others (18 instead of 16 warps on an SM), and spill.
+// Work. A unit is 16 (x token subsets) tokens of one sequence for the KV heads of a CTA, one warp per head, tile of
+// query heads and subset. The units of the whole batch, counted on the device, are split evenly over the CTAs, whatever
+// the lengths: a CTA finishes the sequences that lie in its share and leaves a partial result (in the workspace) of
+// the at most two that do not; attend_join adds those.
+// Every warp fetches its own rows into a ring of its own with 16-byte cp.async, so that warps never wait for one another
+// inside a segment. Bulk copies of a token's heads (640 bytes; 1280 per head of head-major pages) were measured first: an
+// SM completed one in 28 (38) ns whatever was in flight, which held the loads alone to 3.4 (4.7) TB/s.
 #pragma once
 #include <type_traits>
 
@@ -52,11 +52,8 @@ struct AttendShape {
   uint32_t subsets;      // token subsets of a unit, one warp each
   uint32_t tokens;       // tokens per unit: 16 * subsets
   uint32_t warps;        // heads_cta * ntiles * subsets
-  uint32_t run;          // tokens per bulk copy
-  uint32_t copy_heads;   // head copies per token run: 1 (token-major) or heads_cta
-  uint32_t ts, hs;       // shared-memory strides of a token and of a head, bytes
-  uint32_t plane_bytes;  // of one plane of a stage
-  uint32_t stages;
+  uint32_t stages;       // tiles in a warp's ring
+  int32_t block_shift;   // log2 of the block size where it is a power of two >= 16 (a tile lies in one block), else -1
   uint32_t grid;         // CTAs
   uint32_t min_units;    // least units worth a CTA
   uint32_t items;        // num_seqs * head_groups
@@ -80,7 +77,6 @@ struct AttendArgs {
   uint32_t align;             // common alignment of query and out
   uint64_t score_base;        // [NB, H, BS] fp32, or 0
   uint64_t score_block_stride;
-  uint64_t wait_limit_ns;
   AttendShape sh;
   // workspace
   float *part_o;              // [2 * grid][heads_cta * group][D]
@@ -174,35 +170,44 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   }
 }
 
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds16(uint32_t a) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
-  return v;
-}
-// N words from consecutive addresses (8- or 16-byte aligned as the row format guarantees).
-template <int N>
+// N words from shared memory at a + kOff (aligned to N words, as the row format guarantees).
+template <int N, int kOff>
 __device__ __forceinline__ void lds_words(uint32_t (&w)[N], uint32_t a) {
   if constexpr (N == 1) {
-    w[0] = lds32(a);
+    asm volatile("ld.shared.u32 %0, [%1+%2];" : "=r"(w[0]) : "r"(a), "n"(kOff));
   } else if constexpr (N == 2) {
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2+%3];" : "=r"(w[0]), "=r"(w[1]) : "r"(a), "n"(kOff));
   } else {
-#pragma unroll
-    for (int i = 0; i < N; i += 4)
-      asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                   : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3])
-                   : "r"(a + 4 * i));
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4+%5];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(a), "n"(kOff));
+    if constexpr (N == 8)
+      asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4+%5];"
+                   : "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                   : "r"(a), "n"(kOff + 16));
   }
 }
+// Four 8x8 matrices of 16-bit values, lane i giving the address of row i % 8 of matrix i / 8; kTrans: transposed.
+template <bool kTrans, int kOff>
+__device__ __forceinline__ void lds_matrices(uint32_t (&m)[4], uint32_t a) {
+  if constexpr (kTrans)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4+%5];"
+                 : "=r"(m[0]), "=r"(m[1]), "=r"(m[2]), "=r"(m[3])
+                 : "r"(a), "n"(kOff));
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4+%5];"
+                 : "=r"(m[0]), "=r"(m[1]), "=r"(m[2]), "=r"(m[3])
+                 : "r"(a), "n"(kOff));
+}
 
-// Raises the transaction count of the barrier's current phase without arriving.
-__device__ __forceinline__ void mbar_expect_bytes(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+// 16 bytes from global to shared memory, past L1.
+__device__ __forceinline__ void copy16(uint32_t dst, uint64_t src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 constexpr uint32_t kNib0 = 0x000f000fu, kNib1 = 0x00f000f0u;
@@ -218,38 +223,28 @@ struct Share {
   uint64_t first;        // index of the first unit in the batch
 };
 
+// One CTA per SM. At D = 256 a warp's accumulators and queries take over 128 registers, so it has eight warps.
+__host__ __device__ constexpr int attend_max_warps(int D) { return D == 256 ? 8 : 16; }
+// Tiles in a warp's ring: with all warps, about 150 KB of an SM's shared memory.
+__host__ __device__ constexpr int attend_stages(int D) { return D == 64 ? 6 : 4; }
+
 // Decode attention; see the top of the file. kPrecise: carry the remainder of p s_r (fp16 outputs).
 template <typename T, int D>
-__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attend_q4(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const __grid_constant__ AttendArgs a) {
   constexpr int G = q4_groups(D), R = q4_row_bytes(D);
   constexpr int KW = D / 32;  // words of codes per lane and token, keys (two units of every group)
   constexpr int VW = D / 64;  // words of codes per lane and token, values (one unit of every group)
   constexpr int SW = (G + 1) / 2;  // words of a token's scales
-  constexpr bool kPrecise = sizeof(T) == 2 && std::is_same<T, __half>::value;
+  constexpr bool kPrecise = std::is_same<T, __half>::value;
+  constexpr int kTileBytes = 32 * R + 16, kAttendStages = attend_stages(D);
   extern __shared__ __align__(128) unsigned char smem[];
-  constexpr uint32_t kMaxAttendStages = 16;
-  __shared__ __align__(8) uint64_t bar_full[kMaxAttendStages], bar_empty[kMaxAttendStages];
-  __shared__ uint32_t valid[kMaxAttendStages][4];  // which of a stage's tokens count
-  __shared__ uint32_t used[kMaxAttendStages];      // times a stage was filled
   __shared__ Share share;
-  __shared__ uint64_t scan[10];
-  __shared__ int aborted;
+  __shared__ uint64_t scan[16];
 
   const AttendShape &sh = a.sh;
   const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const uint32_t stage_bytes = 2 * sh.plane_bytes;
   grid_launch_dependents();
-
-  if (tid == 0) {
-    for (uint32_t s = 0; s < sh.stages; ++s) {
-      mbar_init(smem_u32(&bar_full[s]), 1);
-      mbar_init(smem_u32(&bar_empty[s]), sh.warps);
-      used[s] = 0;
-    }
-    mbar_init_fence();
-    aborted = 0;
-    a.cta_item[blockIdx.x] = -1;
-  }
+  if (tid == 0) a.cta_item[blockIdx.x] = -1;
   // The batch's units and this CTA's share of them. A thread takes a run of consecutive sequences.
   {
     const uint32_t per = (a.num_seqs + blockDim.x - 1) / blockDim.x;
@@ -298,107 +293,107 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attend_q4(const __grid_
   uint32_t left = share.count;
   if (left == 0) return;
   uint32_t b = share.b, hg = share.hg, unit = share.unit;
-  bool ok = true;
 
-  // ---- loads: this warp's turns are units warp, warp + warps, .. of the share
-  const uint32_t ring = smem_u32(smem);
-  const uint32_t all = left, copies = sh.tokens / sh.run * sh.copy_heads;  // copies per plane
-  uint32_t turn = warp;                                                    // next unit this warp issues
-  uint32_t ib = b, ihg = hg, iunit = unit + warp, in = seq_length(a, b, false), iunits = seq_units(a, in);
-  auto issue = [&]() {
-    while (iunit >= iunits) {
-      iunit -= iunits;
-      if (++ihg == sh.head_groups) {
-        ihg = 0;
-        in = seq_length(a, ++ib, false);
-        iunits = seq_units(a, in);
-      }
-    }
-    const uint32_t use = turn / sh.stages, s = turn - use * sh.stages;
-    const uint32_t h0 = ihg * sh.heads_cta, heads = min(sh.heads_cta, a.kv_heads - h0);
-    const uint32_t full = smem_u32(&bar_full[s]), to = ring + s * stage_bytes;
-    if (use > 0) {
-      ok = mbar_wait_bounded(smem_u32(&bar_empty[s]), (use - 1) & 1, a.wait_limit_ns);
-      ok = __all_sync(0xffffffffu, ok) && !*(volatile int *)&aborted;
-      if (!ok) {
-        if (lane == 0) {
-          report(a.status, kStatusTimeout, (long long)blockIdx.x);
-          *(volatile int *)&aborted = 1;
-        }
-        turn = 0xffffffffu;
-        return;
-      }
-    }
-    uint32_t bits[4] = {0, 0, 0, 0};
+  const uint32_t hl = warp % sh.heads_cta;                 // KV head within the CTA
+  const uint32_t nt = warp / sh.heads_cta % sh.ntiles;     // tile of query heads
+  const uint32_t sub = warp / (sh.heads_cta * sh.ntiles);  // token subset
+  const uint32_t g = lane / 4, q4 = lane % 4, t_sub = sub * 16;
+
+  // ---- loads: a ring of tiles of 16 key rows and 16 value rows, and a word that says which tokens count
+  const uint32_t ring = smem_u32(smem) + warp * kAttendStages * kTileBytes;
+  constexpr int kChunks = R / 16, kCopies = (R + 31) / 32;  // 16-byte chunks of a row; per lane and plane of a tile
+  uint32_t row_off[kCopies];                                // chunk lane + 32 j of a plane: offset from its first row
+#pragma unroll
+  for (int j = 0; j < kCopies; ++j) {
+    const uint32_t c = lane + 32 * j;
+    row_off[j] = c / kChunks * (uint32_t)a.pool.token_stride + c % kChunks * 16;
+  }
+  uint32_t to_load = left, slot_in = ring;
+  uint32_t ib = b, ihg = hg, iunit = unit, in = seq_length(a, b, false), iunits = seq_units(a, in);
+  int32_t id = -1;  // block of the next tile to load, read one tile ahead
+  auto fetch_id = [&]() {
+    const uint32_t t = iunit * sh.tokens + t_sub;
+    if (sh.block_shift >= 0 && t < in) id = a.tables[ib * a.table_stride + (t >> sh.block_shift)];
+  };
+  auto load = [&]() {
+    if (to_load > 0) {
+      --to_load;
+      const uint32_t t = iunit * sh.tokens + t_sub, h = ihg * sh.heads_cta + hl;
+      uint32_t mask = 0;
+      if (t < in && h < a.kv_heads) {
+        const uint32_t count = min(16u, in - t);
+        if (sh.block_shift >= 0) {
+          if ((uint32_t)id < a.pool.num_blocks) {
+            const uint64_t src = a.layer_base + (uint64_t)(uint32_t)id * a.pool.block_stride + h * a.pool.head_stride +
+                                 (t & ((1u << sh.block_shift) - 1u)) * a.pool.token_stride;
+            mask = (1u << count) - 1u;
+#pragma unroll
+            for (int j = 0; j < kCopies; ++j) {
+              const bool inside = (j + 1) * 32 <= R || lane + 32 * j < R;
+              if (inside && (count == 16 || lane + 32 * j < count * kChunks)) {
+                copy16(slot_in + 16 * lane + 512 * j, src + row_off[j]);
+                copy16(slot_in + 16 * R + 16 * lane + 512 * j, src + a.pool.plane_stride + row_off[j]);
+              }
+            }
+          } else if (lane == 0) {
+            report(a.status, kStatusIdRange, id);
+          }
+        } else {
+          // Blocks of any size: every row is looked up.
+          auto row_at = [&](uint32_t row) -> uint64_t {
+            const uint32_t blk = (t + row) / a.pool.block_size;
+            const int32_t i = a.tables[ib * a.table_stride + blk];
+            if ((uint32_t)i >= a.pool.num_blocks) {
+              report(a.status, kStatusIdRange, i);
+              return 0;
+            }
+            return a.layer_base + (uint64_t)i * a.pool.block_stride + h * a.pool.head_stride +
+                   (t + row - blk * a.pool.block_size) * a.pool.token_stride;
+          };
+          mask = __ballot_sync(0xffffffffu, lane < count && row_at(lane) != 0);
 #pragma unroll 1
-    for (uint32_t c = lane; c < copies; c += 32) {
-      const uint32_t run = c / sh.copy_heads, head = c - run * sh.copy_heads;
-      const uint32_t t_rel = run * sh.run, t = iunit * sh.tokens + t_rel;
-      if (t >= in || head >= heads) continue;
-      const uint32_t blk = t / a.pool.block_size;
-      const int32_t id = a.tables[ib * a.table_stride + blk];
-      if ((uint32_t)id >= a.pool.num_blocks) {
-        report(a.status, kStatusIdRange, id);
-        continue;
+          for (uint32_t c = lane; c < count * kChunks; c += 32) {
+            const uint64_t src = row_at(c / kChunks);
+            if (src == 0) continue;
+            copy16(slot_in + 16 * c, src + c % kChunks * 16);
+            copy16(slot_in + 16 * R + 16 * c, src + a.pool.plane_stride + c % kChunks * 16);
+          }
+        }
       }
-      const uint32_t count = min(sh.run, in - t);
-      const uint64_t src = a.layer_base + (uint64_t)id * a.pool.block_stride + (t - blk * a.pool.block_size) * a.pool.token_stride +
-                           (h0 + head) * a.pool.head_stride;
-      const uint32_t dst = to + t_rel * sh.ts + head * sh.hs;
-      const uint32_t len = (sh.copy_heads == 1 ? heads : 1u) * count * R;  // several heads (one token), or several tokens
-      mbar_expect_bytes(full, 2 * len);
-      bulk_load(dst, src, len, full);
-      bulk_load(dst + sh.plane_bytes, src + a.pool.plane_stride, len, full);
-      if (head == 0) {
-        const uint32_t m = ((1u << count) - 1u) << (t_rel % 32);
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          if (t_rel / 32 == w) bits[w] |= m;
+      if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(slot_in + 32 * R), "r"(mask) : "memory");
+      slot_in = slot_in + kTileBytes == ring + kAttendStages * kTileBytes ? ring : slot_in + kTileBytes;
+      if (++iunit == iunits) {
+        iunit = 0;
+        if (++ihg == sh.head_groups) {
+          ihg = 0;
+          if (to_load > 0) {
+            in = seq_length(a, ++ib, false);
+            iunits = seq_units(a, in);
+          }
+        }
       }
+      if (to_load > 0) fetch_id();
     }
-#pragma unroll
-    for (int w = 0; w < 4; ++w)
-      if (w * 32 < (int)sh.tokens) {
-        const uint32_t m = __reduce_or_sync(0xffffffffu, bits[w]);
-        if (lane == 0) valid[s][w] = m;
-      }
-    __syncwarp();
-    if (lane == 0) {
-      used[s] = use + 1;
-      mbar_arrive(full);  // after every lane's expected bytes: the phase ends when they have landed
-    }
-    turn += sh.warps;
-    iunit += sh.warps;
+    copies_commit();  // an empty group at the end keeps the count
   };
-  while (turn < min(all, sh.stages)) issue();
-  uint32_t done = 0;  // units this warp has consumed
+  fetch_id();
+#pragma unroll 1
+  for (int k = 0; k < kAttendStages - 1; ++k) load();
 
-  uint32_t stage = 0, parity = 0;
-  auto advance = [&]() {
-    if (++stage == sh.stages) {
-      stage = 0;
-      parity ^= 1;
-    }
-  };
+  // Tokens are fragment rows in their order. Rows are R apart, an odd multiple of 16 bytes at D = 64 and 128: the value
+  // loads and the matrix loads touch every bank once.
+  const uint32_t tk = g;                             // key rows g and g + 8
+  const uint32_t tv0 = 2 * q4, tv1 = 2 * q4 + 1;     // value rows: tokens tv0, tv1, tv0 + 8, tv1 + 8
+  const uint32_t k_at = tk * R, v_at = (16 + tv0) * R;
+  // Scales and offsets as 8x8 matrices. Keys: rows tokens; the two token halves, at D = 256 scales then offsets, else
+  // the same columns twice (for the high and the low half of Q). Values: columns tokens; likewise by token half.
+  const uint32_t mi = lane / 8, mt = lane % 8;
+  const uint32_t km_at = (mt + 8 * (mi & 1)) * R + (G == 8 && mi >= 2 ? 2 * G : 0);
+  const uint32_t vm_at = (16 + mt + 8 * (mi >> 1)) * R + (G == 8 && (mi & 1) ? 2 * G : 0);
+  const uint32_t scale_bits = G == 8 || g < (uint32_t)G ? 0x40004000u : 0u;  // >= 2, where this lane's rows are scales
+  uint32_t slot_out = ring;
 
-  const uint32_t hl = warp % sh.heads_cta;                       // KV head within the CTA
-  const uint32_t nt = warp / sh.heads_cta % sh.ntiles;           // tile of query heads
-  const uint32_t sub = warp / (sh.heads_cta * sh.ntiles);        // token subset
-  const uint32_t g = lane / 4, q4 = lane % 4;
-  // Tokens of fragment rows: with a token stride of 32 * odd bytes (token-major) rows 2i, 2i + 1 are two tokens apart
-  // and even (odd) rows cover all residues mod 4; with 16 * odd (head-major) even rows are even tokens. Either way the
-  // value loads, and in the first case the key loads too, touch every bank once.
-  auto token_of = [&](uint32_t r) -> uint32_t {
-    if (sh.ts % 32) return r;
-    return r < 4 ? (r >> 1) + 2 * (r & 1) : (r < 6 ? 6 - 2 * (r & 1) : 7 - 2 * (r & 1));
-  };
-  const uint32_t tk = token_of(g);                            // key rows g and g + 8: tokens tk, tk + 8
-  const uint32_t tv0 = token_of(2 * q4), tv1 = token_of(2 * q4 + 1);
-  const uint32_t t_sub = sub * 16;
-  const uint32_t k_off = (t_sub + tk) * sh.ts + hl * sh.hs;
-  const uint32_t v_off0 = sh.plane_bytes + (t_sub + tv0) * sh.ts + hl * sh.hs;
-  const uint32_t v_off1 = sh.plane_bytes + (t_sub + tv1) * sh.ts + hl * sh.hs;
-  float *merge = reinterpret_cast<float *>(smem + sh.stages * stage_bytes);  // [(warps - warps/subsets)][8][D + 2]
+  float *merge = reinterpret_cast<float *>(smem + sh.warps * kAttendStages * kTileBytes);  // [(warps - warps/subsets)][8][D + 2]
 
   while (left > 0) {
     const uint32_t n = seq_length(a, b, false), units = seq_units(a, n);
@@ -409,7 +404,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attend_q4(const __grid_
 
     // ---- the queries of this tile as B fragments
     uint32_t qf[G][4];
-    uint32_t qo[2], qc[2];  // Q_r and -8 Q_r as two halves: B fragments of the offsets' and scales' product
+    uint32_t qo[4];     // Q_r (offsets) and -8 Q_r (scales) as two halves: B fragments
     float c0, c1;       // logit factors of heads 2 q4, 2 q4 + 1
     {
       const bool mine = active && j0 + g < a.group;
@@ -443,9 +438,9 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attend_q4(const __grid_
       int ex = (int)((__float_as_uint(top) >> 23) & 255u) - 127 - 5;
       ex = top == 0.f ? 0 : (ex < -110 ? -110 : (ex > 123 ? 123 : ex));
       const float down = __uint_as_float((uint32_t)(127 - ex) << 23), up = __uint_as_float((uint32_t)(127 + ex) << 23);
-      // k index of the offset product: groups' high halves at 0 .. G-1, low halves at G .. 2G-1
+      // k index of that product: scales of groups 0 .. G-1, then their offsets (G = 8: each 0 .. 7)
       const int r0 = G == 8 ? 2 * (int)q4 : (G == 4 ? 2 * (int)(q4 & 1) : 0);
-      const bool low = G == 4 ? q4 >= 2 : q4 == 1;
+      const bool scales = G == 4 ? q4 < 2 : q4 == 0;
       float pick0 = 0.f, pick1 = 0.f;
 #pragma unroll
       for (int r = 0; r < G; ++r) {
@@ -470,14 +465,15 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attend_q4(const __grid_
       const uint32_t rest = pack_half2(pick0 - rounded.x, pick1 - rounded.y);
       const uint32_t eight = 0xc800c800u;  // -8, -8
       if constexpr (G == 8) {
-        qo[0] = hi;
-        qo[1] = rest;
-        qc[0] = mul_half2(hi, eight);
-        qc[1] = mul_half2(rest, eight);
-      } else {  // one product: offsets in k 0 .. 7, scales in k 8 .. 15
-        qo[0] = G == 4 || q4 < 2 ? (low ? rest : hi) : 0u;
-        qo[1] = mul_half2(qo[0], eight);
-        qc[0] = qc[1] = 0;
+        qo[0] = mul_half2(hi, eight);
+        qo[1] = hi;
+        qo[2] = mul_half2(rest, eight);
+        qo[3] = rest;
+      } else {
+        const bool none = G == 2 && q4 >= 2;  // the row's padding
+        qo[0] = none ? 0u : (scales ? mul_half2(hi, eight) : hi);
+        qo[1] = none ? 0u : (scales ? mul_half2(rest, eight) : rest);
+        qo[2] = qo[3] = 0;
       }
       const float c = up * a.scale_log2;
       c0 = __shfl_sync(0xffffffffu, c, 8 * q4);
@@ -521,104 +517,83 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attend_q4(const __grid_
     };
 
     for (uint32_t k = 0; k < count; ++k) {
-      if (ok) {
-        ok = mbar_wait_bounded(smem_u32(&bar_full[stage]), parity, a.wait_limit_ns);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok && lane == 0) {
-          report(a.status, kStatusTimeout, (long long)blockIdx.x);
-          *(volatile int *)&aborted = 1;
-        }
-      }
-      const uint32_t mask = ok && active ? valid[stage][t_sub / 32] >> (t_sub % 32) & 0xffffu : 0u;
+      copies_wait<kAttendStages - 2>();
+      __syncwarp();  // this tile's rows are there for every lane, and every lane has left the slot of the tile before
+      load();
+      uint32_t mask;
+      asm volatile("ld.shared.u32 %0, [%1+%2];" : "=r"(mask) : "r"(slot_out), "n"(32 * R));
       if (mask) {
-        const uint32_t base = ring + stage * stage_bytes;
+        const uint32_t base = slot_out;
         // ---- logits of 16 tokens
         float l[4];
         {
-          uint32_t w0[KW], w1[KW], s0[SW], s1[SW];
-          const uint32_t ka = base + k_off, kb = ka + 8 * sh.ts;
-          lds_words(w0, ka + q4 * (D / 8));
-          lds_words(w1, kb + q4 * (D / 8));
-          lds_words(s0, ka + D / 2);
-          lds_words(s1, kb + D / 2);
+          uint32_t w0[KW], w1[KW], s0[SW], s1[SW], m[4];
+          const uint32_t ka = base + k_at, kc = ka + q4 * (D / 8);
+          lds_matrices<false, D / 2>(m, base + km_at);
+          lds_words<KW, 0>(w0, kc);
+          lds_words<KW, 8 * R>(w1, kc);
+          lds_words<SW, D / 2>(s0, ka);
+          lds_words<SW, 8 * R + D / 2>(s1, ka);
           float d0[4] = {0.f, 0.f, 0.f, 0.f};
-          {
-            const uint32_t wo = G == 8 ? q4 : (G == 4 ? (q4 & 1) : 0);  // word of two groups
-            const uint32_t o0 = lds32(ka + D / 2 + 2 * G + 4 * wo), o1 = lds32(kb + D / 2 + 2 * G + 4 * wo);
-            if constexpr (G == 8) {
-              const uint32_t e0 = lds32(ka + D / 2 + 4 * wo), e1 = lds32(kb + D / 2 + 4 * wo);
-              mma_k16(d0, o0, o1, o0, o1, qo[0], qo[1], d0);
-              mma_k16(d0, e0, e1, e0, e1, qc[0], qc[1], d0);
-            } else {
-              const uint32_t e0 = G == 4 && (q4 & 1) ? s0[SW - 1] : s0[0], e1 = G == 4 && (q4 & 1) ? s1[SW - 1] : s1[0];
-              mma_k16(d0, o0, o1, e0, e1, qo[0], qo[1], d0);
-            }
-          }
-          float x[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_k16(d0, m[0], m[1], m[2], m[3], qo[0], qo[1], d0);
+          if constexpr (G == 8) mma_k16(d0, m[0], m[1], m[2], m[3], qo[2], qo[3], d0);
+          float x[4];
 #pragma unroll
           for (int r = 0; r < G; ++r) {
             const uint32_t sel = r % 2 ? kHiHalves : kLoHalves;
             const uint32_t u0 = __byte_perm(w0[r / 2], w0[KW / 2 + r / 2], sel), u1 = __byte_perm(w1[r / 2], w1[KW / 2 + r / 2], sel);
             const uint32_t y0 = u0 >> 8, y1 = u1 >> 8;
-            float m[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_k16(m, u0 & kNib0, u1 & kNib0, u0 & kNib1, u1 & kNib1, qf[r][0], qf[r][1], m);
-            mma_k16(m, y0 & kNib0, y1 & kNib0, y0 & kNib1, y1 & kNib1, qf[r][2], qf[r][3], m);
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_k16(d, u0 & kNib0, u1 & kNib0, u0 & kNib1, u1 & kNib1, qf[r][0], qf[r][1], d);
+            mma_k16(d, y0 & kNib0, y1 & kNib0, y0 & kNib1, y1 & kNib1, qf[r][2], qf[r][3], d);
             const float2 f0 = unpack_half2(s0[r / 2]), f1 = unpack_half2(s1[r / 2]);
             const float e0 = r % 2 ? f0.y : f0.x, e1 = r % 2 ? f1.y : f1.x;
-            x[0] = fmaf(e0, m[0], x[0]);
-            x[1] = fmaf(e0, m[1], x[1]);
-            x[2] = fmaf(e1, m[2], x[2]);
-            x[3] = fmaf(e1, m[3], x[3]);
+            x[0] = r ? fmaf(e0, d[0], x[0]) : e0 * d[0];
+            x[1] = r ? fmaf(e0, d[1], x[1]) : e0 * d[1];
+            x[2] = r ? fmaf(e1, d[2], x[2]) : e1 * d[2];
+            x[3] = r ? fmaf(e1, d[3], x[3]) : e1 * d[3];
           }
           l[0] = c0 * fmaf(x[0], 0x1p20f, d0[0]);
           l[1] = c1 * fmaf(x[1], 0x1p20f, d0[1]);
           l[2] = c0 * fmaf(x[2], 0x1p20f, d0[2]);
           l[3] = c1 * fmaf(x[3], 0x1p20f, d0[3]);
         }
+        // ---- scales and offsets of the value rows
+        const uint32_t va = base + v_at;
+        uint32_t sv[4][SW], m[4];  // tokens tv0, tv1, tv0 + 8, tv1 + 8
+        lds_matrices<true, D / 2>(m, base + vm_at);
+        lds_words<SW, D / 2>(sv[0], va);
+        lds_words<SW, R + D / 2>(sv[1], va);
+        lds_words<SW, 8 * R + D / 2>(sv[2], va);
+        lds_words<SW, 9 * R + D / 2>(sv[3], va);
         if (mask != 0xffffu) {
+          // Tokens that do not count: no weight, and no scale or offset that could be anything (0 * NaN).
           if (!(mask >> tk & 1)) l[0] = l[1] = -INFINITY;
           if (!(mask >> (tk + 8) & 1)) l[2] = l[3] = -INFINITY;
-        }
-        if (lg) {
-          const uint32_t t = (unit0 + k) * sh.tokens + t_sub + tk;
-          if (t < n) {
-            if (store0) lg[t] = l[0];
-            if (store1) lg[a.logit_stride + t] = l[1];
-          }
-          if (t + 8 < n) {
-            if (store0) lg[t + 8] = l[2];
-            if (store1) lg[a.logit_stride + t + 8] = l[3];
-          }
-        }
-        // ---- scales of the value rows; from the first one >= 2 (bit 14 of an fp16) p is held smaller
-        uint32_t sv[4][SW];  // tokens tv0, tv1, tv0 + 8, tv1 + 8
-        uint32_t ov[4];      // offsets of group g at the same tokens
-        const uint32_t va = base + v_off0, vb = base + v_off1;
-        lds_words(sv[0], va + D / 2);
-        lds_words(sv[1], vb + D / 2);
-        lds_words(sv[2], va + 8 * sh.ts + D / 2);
-        lds_words(sv[3], vb + 8 * sh.ts + D / 2);
-        const uint32_t oa = D / 2 + 2 * G + 2 * (g & (G - 1));
-        ov[0] = lds16(va + oa);
-        ov[1] = lds16(vb + oa);
-        ov[2] = lds16(va + 8 * sh.ts + oa);
-        ov[3] = lds16(vb + 8 * sh.ts + oa);
-        if (mask != 0xffffu) {
           const uint32_t t[4] = {tv0, tv1, tv0 + 8, tv1 + 8};
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (!(mask >> t[i] & 1)) {
-              ov[i] = 0;
+              const uint32_t stay = i % 2 ? 0x0000ffffu : 0xffff0000u;
+              m[i / 2 * 2] &= stay;
+              m[i / 2 * 2 + 1] &= stay;
 #pragma unroll
               for (int w = 0; w < SW; ++w) sv[i][w] = 0;
             }
         }
-        uint32_t big = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int w = 0; w < SW; ++w) big |= sv[i][w];
-        const bool lower = (big & 0x40004000u) != 0 && lift > 0.f;
+        if (lg) {
+          const uint32_t t = (unit0 + k) * sh.tokens + t_sub + tk;
+          if (mask >> tk & 1) {
+            if (store0) lg[t] = l[0];
+            if (store1) lg[a.logit_stride + t] = l[1];
+          }
+          if (mask >> (tk + 8) & 1) {
+            if (store0) lg[t + 8] = l[2];
+            if (store1) lg[a.logit_stride + t + 8] = l[3];
+          }
+        }
+        // From the first scale >= 2 (bit 14 of an fp16) on p is held smaller.
+        const bool lower = ((m[0] | m[2]) & scale_bits) != 0 && lift > 0.f;
         // ---- weights; the reference follows the maximum only when it is left 2^6 behind
         float p[4] = {l[0] - ref0, l[1] - ref1, l[2] - ref0, l[3] - ref1};
         const float most = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
@@ -651,18 +626,16 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attend_q4(const __grid_
           bl0 = transpose8(pack_half2(p[0] - r01.x, p[1] - r01.y));
           bl1 = transpose8(pack_half2(p[2] - r23.x, p[3] - r23.y));
         }
-        // ---- sum p o_r in rows 8 .. of accx
-        {
-          const uint32_t o01 = ov[0] | ov[1] << 16, o23 = ov[2] | ov[3] << 16;
-          mma_k16(accx, 0u, o01, 0u, o23, b0, b1, accx);
-          if constexpr (kPrecise) mma_k16(accx, 0u, o01, 0u, o23, bl0, bl1, accx);
-        }
+        // ---- sums of p s_r and p o_r: rows r and G + r of accx
+        mma_k16(accx, m[0], m[1], m[2], m[3], b0, b1, accx);
+        if constexpr (kPrecise) mma_k16(accx, m[0], m[1], m[2], m[3], bl0, bl1, accx);
         // ---- values
         uint32_t w[4][VW];
-        lds_words(w[0], va + g * (D / 16));
-        lds_words(w[1], vb + g * (D / 16));
-        lds_words(w[2], va + 8 * sh.ts + g * (D / 16));
-        lds_words(w[3], vb + 8 * sh.ts + g * (D / 16));
+        const uint32_t vc = va + g * (D / 16);
+        lds_words<VW, 0>(w[0], vc);
+        lds_words<VW, R>(w[1], vc);
+        lds_words<VW, 8 * R>(w[2], vc);
+        lds_words<VW, 9 * R>(w[3], vc);
 #pragma unroll
         for (int r = 0; r < G; ++r) {
           const uint32_t sel = r % 2 ? kHiHalves : kLoHalves;
@@ -670,25 +643,17 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attend_q4(const __grid_
           const uint32_t e0 = mul_half2(b0, s01), e1 = mul_half2(b1, s23);
           const uint32_t u01 = __byte_perm(w[0][r / 2], w[1][r / 2], sel), u23 = __byte_perm(w[2][r / 2], w[3][r / 2], sel);
           const uint32_t y01 = u01 >> 8, y23 = u23 >> 8;
-          const uint32_t one = g == (uint32_t)r ? 0x3c003c00u : 0u;
           mma_k16(acc[r][0], u01 & kNib0, u01 & kNib1, u23 & kNib0, u23 & kNib1, e0, e1, acc[r][0]);
           mma_k16(acc[r][1], y01 & kNib0, y01 & kNib1, y23 & kNib0, y23 & kNib1, e0, e1, acc[r][1]);
-          mma_k16(accx, one, 0u, one, 0u, e0, e1, accx);
           if constexpr (kPrecise) {
             const uint32_t f0 = fma_half2(bl0, s01, fma_half2(b0, s01, e0 ^ 0x80008000u));
             const uint32_t f1 = fma_half2(bl1, s23, fma_half2(b1, s23, e1 ^ 0x80008000u));
             mma_k16(acc[r][0], u01 & kNib0, u01 & kNib1, u23 & kNib0, u23 & kNib1, f0, f1, acc[r][0]);
             mma_k16(acc[r][1], y01 & kNib0, y01 & kNib1, y23 & kNib0, y23 & kNib1, f0, f1, acc[r][1]);
-            mma_k16(accx, one, 0u, one, 0u, f0, f1, accx);
           }
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bar_empty[stage]));
-      advance();
-      // Refill the stage of the unit before this one: the other warps have most likely left it.
-      ++done;
-      if (done >= 2 && turn == done + sh.stages - 2 && turn < all) issue();
+      slot_out = slot_out + kTileBytes == ring + kAttendStages * kTileBytes ? ring : slot_out + kTileBytes;
     }
 
     // ---- the segment's result: o[r][i] of channel 32 r + 4 g + i, heads 2 q4 and 2 q4 + 1
@@ -699,8 +664,9 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attend_q4(const __grid_
     }
 #pragma unroll
     for (int r = 0; r < G; ++r) {
-      const float x0 = __shfl_sync(0xffffffffu, accx[2], 4 * r + q4) - 8.f * __shfl_sync(0xffffffffu, accx[0], 4 * r + q4);
-      const float x1 = __shfl_sync(0xffffffffu, accx[3], 4 * r + q4) - 8.f * __shfl_sync(0xffffffffu, accx[1], 4 * r + q4);
+      const int so = G == 8 ? 4 * r : 4 * (G + r);  // lanes that hold the offsets' sums
+      const float x0 = __shfl_sync(0xffffffffu, accx[G == 8 ? 2 : 0], so + q4) - 8.f * __shfl_sync(0xffffffffu, accx[0], 4 * r + q4);
+      const float x1 = __shfl_sync(0xffffffffu, accx[G == 8 ? 3 : 1], so + q4) - 8.f * __shfl_sync(0xffffffffu, accx[1], 4 * r + q4);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         acc[r][i][0] = fmaf(acc[r][i][0], 0x1p24f, x0);
@@ -757,7 +723,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attend_q4(const __grid_
       __syncthreads();  // the buffer is free for the next segment
     }
     const bool whole = count == units;
-    if (sub == 0 && active && ok) {
+    if (sub == 0 && active) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const uint32_t j = j0 + 2 * q4 + c;
@@ -805,26 +771,24 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attend_q4(const __grid_
       ++b;
     }
   }
-  __syncthreads();
-  if (aborted && tid == 0) {
-    // Loads may still be landing in this CTA's shared memory: one more bounded wait for each stage.
-    for (uint32_t s = 0; s < sh.stages; ++s)
-      if (used[s] && !mbar_wait_bounded(smem_u32(&bar_full[s]), (used[s] - 1) & 1, a.wait_limit_ns)) break;
-  }
+  copies_wait<0>();
 }
 
-// Adds the partial results of an item that several CTAs worked on. grid.x: items, or (by_cta) the CTAs that finished
-// one; grid.y: query heads of an item. A warp takes every eighth part, four channels (or two) per lane.
-constexpr int kJoinWarps = 8;
+// Adds the partial results of the items that several CTAs worked on. grid.x: items, or (by_cta) the CTAs that finished
+// one; grid.y x kHeads: the query heads of an item. kJoinWarps / kHeads warps share a head's parts: all of them where
+// few items have many parts, one or two where many items have few.
+constexpr int kJoinWarps = 16;
 
-template <typename T, int D>
+template <typename T, int D, int kHeads>
 __global__ void __launch_bounds__(kJoinWarps * 32) attend_join(const __grid_constant__ AttendArgs a, const uint32_t by_cta) {
-  constexpr int C = D / 32;  // channels per lane
+  constexpr int C = D / 32;                // channels per lane
+  constexpr int W = kJoinWarps / kHeads;   // warps per head
   __shared__ float red[kJoinWarps][2];
   __shared__ float o[kJoinWarps][D];
   grid_launch_dependents();
   grid_dependency_wait();
-  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, y = blockIdx.y;
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, mine = warp % W;
+  const uint32_t rows = a.sh.heads_cta * a.group, y = blockIdx.y * kHeads + warp / W;
   int item = (int)blockIdx.x;
   if (by_cta) item = a.cta_item[blockIdx.x];
   if (item < 0) return;
@@ -832,77 +796,121 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join(const __grid_cons
   if (span.x == span.y) return;
   const uint32_t b = item / a.sh.head_groups, hg = item % a.sh.head_groups;
   const uint32_t h = hg * a.sh.heads_cta + y / a.group;
-  if (h >= a.kv_heads) return;
-  const uint32_t parts = (uint32_t)(span.y - span.x) + 1, rows = a.sh.heads_cta * a.group;
+  const bool real = y < rows && h < a.kv_heads;
+  const uint32_t parts = real ? (uint32_t)(span.y - span.x) + 1 : 0;
   auto row_of = [&](uint32_t i) { return (2ull * (span.x + i) + (i == 0 ? 1 : 0)) * rows + y; };
-  float top = kFirstRef;
-  for (uint32_t i = threadIdx.x; i < parts; i += kJoinWarps * 32) top = fmaxf(top, a.part_ml[row_of(i)].x);
-#pragma unroll
-  for (int m = 16; m; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-  if (lane == 0) red[warp][0] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, red[w][0]);
-  float acc[C], sum = 0.f;
+  // Each warp runs through its parts with a maximum of its own; the warps' results meet in shared memory.
+  float acc[C], sum = 0.f, top = kFirstRef;
 #pragma unroll
   for (int c = 0; c < C; ++c) acc[c] = 0.f;
-#pragma unroll 4
-  for (uint32_t i = warp; i < parts; i += kJoinWarps) {
-    const uint64_t row = row_of(i);
-    const float2 ml = a.part_ml[row];
-    const float f = ex2(ml.x - top);
-    sum = fmaf(ml.y, f, sum);
-    const float *src = a.part_o + row * D + lane * C;
-    float v[C];
-    if constexpr (C == 2) {
-      *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(src);
-    } else {
+  constexpr int kAhead = 8;  // parts whose loads are in flight together
+  for (uint32_t i0 = mine; i0 < parts; i0 += W * kAhead) {
+    float v[kAhead][C];
+    float2 ml[kAhead];
 #pragma unroll
-      for (int c = 0; c < C; c += 4) *reinterpret_cast<float4 *>(v + c) = *reinterpret_cast<const float4 *>(src + c);
+    for (int u = 0; u < kAhead; ++u) {
+      const uint32_t i = i0 + u * W;
+      ml[u] = make_float2(kFirstRef, 0.f);
+#pragma unroll
+      for (int c = 0; c < C; ++c) v[u][c] = 0.f;
+      if (i < parts) {
+        const uint64_t row = row_of(i);
+        ml[u] = a.part_ml[row];
+        const float *src = a.part_o + row * D + lane * C;
+        if constexpr (C == 2) {
+          *reinterpret_cast<float2 *>(v[u]) = *reinterpret_cast<const float2 *>(src);
+        } else {
+#pragma unroll
+          for (int c = 0; c < C; c += 4) *reinterpret_cast<float4 *>(v[u] + c) = *reinterpret_cast<const float4 *>(src + c);
+        }
+      }
     }
+    float to = top;
 #pragma unroll
-    for (int c = 0; c < C; ++c) acc[c] = fmaf(v[c], f, acc[c]);
+    for (int u = 0; u < kAhead; ++u) to = fmaxf(to, ml[u].x);
+    const float f = ex2(top - to);
+    top = to;
+    sum *= f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) acc[c] *= f;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const float e = ex2(ml[u].x - to);
+      sum = fmaf(ml[u].y, e, sum);
+#pragma unroll
+      for (int c = 0; c < C; ++c) acc[c] = fmaf(v[u][c], e, acc[c]);
+    }
   }
+  if constexpr (W > 1) {
 #pragma unroll
-  for (int c = 0; c < C; ++c) o[warp][lane * C + c] = acc[c];
-  if (lane == 0) red[warp][1] = sum;
-  __syncthreads();
-  sum = 0.f;
+    for (int c = 0; c < C; ++c) o[warp][lane * C + c] = acc[c];
+    if (lane == 0) {
+      red[warp][0] = top;
+      red[warp][1] = sum;
+    }
+    __syncthreads();
+    if (mine != 0) return;
+    float to = top;
+    for (int w = 0; w < W; ++w) to = fmaxf(to, red[warp + w][0]);
+    sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) sum += red[w][1];
+    for (int c = 0; c < C; ++c) acc[c] = 0.f;
+    for (int w = 0; w < W; ++w) {
+      const float e = ex2(red[warp + w][0] - to);
+      sum = fmaf(red[warp + w][1], e, sum);
+#pragma unroll
+      for (int c = 0; c < C; ++c) acc[c] = fmaf(o[warp + w][lane * C + c], e, acc[c]);
+    }
+    top = to;
+  }
+  if (!real) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const uint64_t head = (uint64_t)h * a.group + y % a.group;
-  if (threadIdx.x < D) {
-    float v = 0.f;
+  T *out = reinterpret_cast<T *>(a.out + b * a.out_seq_stride) + head * D + lane * C;
+  if (a.align >= 4) {
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) v += o[w][threadIdx.x];
-    reinterpret_cast<T *>(a.out + b * a.out_seq_stride)[head * D + threadIdx.x] = from_f32<T>(v * inv);
+    for (int c = 0; c < C; c += 2) reinterpret_cast<uint32_t *>(out)[c / 2] = pack2<T>(acc[c] * inv, acc[c + 1] * inv);
+  } else {
+#pragma unroll
+    for (int c = 0; c < C; ++c) out[c] = from_f32<T>(acc[c] * inv);
   }
-  if (threadIdx.x == 0 && a.score_base)
+  if (lane == 0 && a.score_base)
     a.lse[(uint64_t)b * a.kv_heads * a.group + head] = sum == 0.f ? INFINITY : top + lg2(sum);
 }
 
-// Adds every token's weight to its score. grid.x: chunks of 256 tokens, grid.y: (sequence, KV head) pairs.
-__global__ void __launch_bounds__(256) attend_scores(const __grid_constant__ AttendArgs a) {
-  __shared__ float lse[64];
+// Adds every token's weight to its score. Persistent: a block takes chunks of 1024 tokens of a (sequence, KV head) pair,
+// four tokens a thread.
+constexpr uint32_t kScoreChunk = 1024;
+
+__global__ void __launch_bounds__(256) attend_scores(const __grid_constant__ AttendArgs a, const uint32_t chunks) {
   grid_launch_dependents();
   grid_dependency_wait();
-  for (uint32_t bh = blockIdx.y; bh < a.num_seqs * a.kv_heads; bh += gridDim.y) {
-    const uint32_t b = bh / a.kv_heads, h = bh % a.kv_heads;
-    const uint32_t n = seq_length(a, b, false), t = blockIdx.x * 256 + threadIdx.x;
-    if (blockIdx.x * 256 >= n) continue;
-    const uint64_t head = ((uint64_t)b * a.kv_heads + h) * a.group;
-    __syncthreads();
-    if (threadIdx.x < a.group) lse[threadIdx.x] = a.lse[head + threadIdx.x];
-    __syncthreads();
+  const uint64_t total = (uint64_t)a.num_seqs * a.kv_heads * chunks;
+  for (uint64_t i = blockIdx.x; i < total; i += gridDim.x) {
+    const uint32_t bh = (uint32_t)(i / chunks), b = bh / a.kv_heads, h = bh % a.kv_heads;
+    const uint32_t n = seq_length(a, b, false), t = (uint32_t)(i % chunks) * kScoreChunk + threadIdx.x * 4;
     if (t >= n) continue;
-    const int32_t id = a.tables[b * a.table_stride + t / a.pool.block_size];
-    if ((uint32_t)id >= a.pool.num_blocks) continue;
-    float w = 0.f;
-    for (uint32_t j = 0; j < a.group; ++j) w += ex2(a.logits[(head + j) * a.logit_stride + t] - lse[j]);
-    float *sc = reinterpret_cast<float *>(a.score_base + (uint64_t)id * a.score_block_stride) +
-                (uint64_t)h * a.pool.block_size + t % a.pool.block_size;
-    *sc += w;
+    const uint64_t head = (uint64_t)bh * a.group;
+    float w[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (uint32_t j = 0; j < a.group; ++j) {
+      const float lse = a.lse[head + j];
+      const float4 l = *reinterpret_cast<const float4 *>(a.logits + (head + j) * a.logit_stride + t);
+      w[0] += ex2(l.x - lse);
+      w[1] += ex2(l.y - lse);
+      w[2] += ex2(l.z - lse);
+      w[3] += ex2(l.w - lse);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (t + k >= n) break;
+      const uint32_t blk = (t + k) / a.pool.block_size;
+      const int32_t id = a.tables[b * a.table_stride + blk];
+      if ((uint32_t)id >= a.pool.num_blocks) continue;
+      float *sc = reinterpret_cast<float *>(a.score_base + (uint64_t)id * a.score_block_stride) +
+                  (uint64_t)h * a.pool.block_size + (t + k - blk * a.pool.block_size);
+      *sc += w[k];
+    }
   }
 }
 

@@ -132,41 +132,29 @@ int attend_shape(const emm_pool *pool, int32_t D, int32_t B, int32_t group, int3
   const uint32_t R = (uint32_t)emm::q4_row_bytes(D), H = (uint32_t)d.num_kv_heads;
   emm::AttendShape s;
   s.ntiles = (uint32_t)(group + 7) / 8;
-  // Eight warps at most: KV heads first (their rows of a token are one copy), equal shares of them, then
-  // the tokens of a unit in as many subsets as are left.
+  // KV heads first (their rows of a token are one copy), in equal shares of at most eight warps, then the tokens of a
+  // unit in as many subsets as there are warps left.
   const uint32_t most = std::max(1u, 8u / s.ntiles);
   s.head_groups = (H + most - 1) / most;
   s.heads_cta = (H + s.head_groups - 1) / s.head_groups;
-  s.subsets = std::max(1u, 8u / (s.heads_cta * s.ntiles));
+  s.items = (uint32_t)B * s.head_groups;
+  s.min_units = 1;
+  const uint64_t sms = (uint64_t)pool->ctx->sm_count;
+  s.subsets = std::max(1u, (uint32_t)emm::attend_max_warps(D) / (s.heads_cta * s.ntiles));
+  auto units = [&]() {
+    return std::max<uint64_t>(1, ((uint64_t)max_len + 16 * s.subsets - 1) / (16 * s.subsets)) * s.items;
+  };
+  // Little work is spread over more, smaller CTAs.
+  while (s.subsets > 1 && units() < sms) s.subsets /= 2;
   s.tokens = 16 * s.subsets;
   s.warps = s.heads_cta * s.ntiles * s.subsets;
-  const bool token_major = d.head_stride == (int64_t)R && !(H == 1 && d.token_stride == (int64_t)R);
-  if (token_major) {
-    s.run = 1;
-    s.copy_heads = 1;
-    const uint32_t lines = (s.heads_cta * R + 31) / 32;
-    s.ts = 32 * (lines | 1u);  // 32 * odd: the fragment rows' loads fall into different banks
-    s.hs = R;
-    s.plane_bytes = s.tokens * s.ts;
-  } else {
-    s.run = 1;
-    if (d.token_stride == (int64_t)R)
-      while (s.run < 16 && d.block_size % (2 * (int)s.run) == 0) s.run *= 2;
-    s.copy_heads = s.heads_cta;
-    s.ts = R;
-    s.hs = s.tokens * R;
-    s.plane_bytes = s.heads_cta * s.hs;
-  }
-  const int per_sm = D == 256 ? 1 : 2;
-  const int budget = std::min(pool->ctx->max_smem_optin, 228 * 1024 / per_sm) - 4096;
+  s.block_shift = -1;
+  for (int k = 4; k < 31; ++k)
+    if (d.block_size == 1 << k && d.token_stride < 1 << 27) s.block_shift = k;  // a tile's offsets take 32 bits
+  s.stages = (uint32_t)emm::attend_stages(D);
   const int merge = (int)((s.subsets - 1) * s.heads_cta * s.ntiles * 8 * (uint32_t)(D + 2) * 4);
-  s.stages = (uint32_t)std::min(16, (budget - merge) / (int)(2 * s.plane_bytes));
-  if (s.stages < 2) return fail(EMM_ERR_TOO_LARGE, "q4_attend: a unit of %u bytes does not fit shared memory", 2 * s.plane_bytes);
-  *smem_out = (int)(s.stages * 2 * s.plane_bytes) + merge;
-  s.items = (uint32_t)B * s.head_groups;
-  s.min_units = 2;
-  const uint64_t units = std::max<uint64_t>(1, ((uint64_t)max_len + s.tokens - 1) / s.tokens) * s.items;
-  s.grid = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(units / s.min_units, (uint64_t)pool->ctx->sm_count * per_sm));
+  *smem_out = (int)(s.warps * s.stages * (32 * R + 16)) + merge;
+  s.grid = (uint32_t)std::min<uint64_t>(units() / s.min_units, sms);
   *out = s;
   return EMM_OK;
 }
@@ -229,16 +217,24 @@ int attend_launch(emm_ctx *ctx, const emm::AttendArgs &a, int smem, cudaStream_t
   cfg.numAttrs = ctx->pdl ? 1 : 0;
   if (a.sh.grid > 1) {  // one CTA splits nothing
     const bool by_cta = a.sh.items > a.sh.grid;
-    cfg.gridDim = dim3(by_cta ? a.sh.grid : a.sh.items, a.sh.heads_cta * a.group);
+    const uint32_t rows = a.sh.heads_cta * a.group, x = by_cta ? a.sh.grid : a.sh.items;
     cfg.blockDim = dim3(emm::kJoinWarps * 32);
-    EMM_CUDA(cudaLaunchKernelEx(&cfg, emm::attend_join<T, D>, a, (uint32_t)by_cta));
+    // Where items are few an item has many parts, and a head needs all warps of a block; else two.
+    if (x * 8 <= a.sh.grid) {
+      cfg.gridDim = dim3(x, rows);
+      EMM_CUDA(cudaLaunchKernelEx(&cfg, emm::attend_join<T, D, 1>, a, (uint32_t)by_cta));
+    } else {
+      cfg.gridDim = dim3(x, (rows + 7) / 8);
+      EMM_CUDA(cudaLaunchKernelEx(&cfg, emm::attend_join<T, D, 8>, a, (uint32_t)by_cta));
+    }
     ctx->launches += 1;
   }
   if (a.score_base && a.max_len > 0) {
-    const uint64_t pairs = (uint64_t)a.num_seqs * a.kv_heads;
-    cfg.gridDim = dim3((a.max_len + 255) / 256, (unsigned)std::min<uint64_t>(pairs, 65535));
+    const uint32_t chunks = (a.max_len + emm::kScoreChunk - 1) / emm::kScoreChunk;
+    const uint64_t total = (uint64_t)a.num_seqs * a.kv_heads * chunks;
+    cfg.gridDim = dim3((unsigned)std::min<uint64_t>(total, (uint64_t)ctx->sm_count * 8));
     cfg.blockDim = dim3(256);
-    EMM_CUDA(cudaLaunchKernelEx(&cfg, emm::attend_scores, a));
+    EMM_CUDA(cudaLaunchKernelEx(&cfg, emm::attend_scores, a, chunks));
     ctx->launches += 1;
   }
   return EMM_OK;
@@ -344,7 +340,6 @@ int emm_q4_attend(emm_pool *pool, int32_t head_dim, int32_t dtype, int32_t layer
   a.align = align;
   a.score_base = scores ? scores->h_layers[layer] : 0;
   a.score_block_stride = scores ? (uint64_t)scores->desc.block_stride : 0;
-  a.wait_limit_ns = pool->ctx->wait_limit_ns;
   a.part_o = (float *)(ws + w.part_o);
   a.part_ml = (float2 *)(ws + w.part_ml);
   a.item_span = (int2 *)(ws + w.item_span);

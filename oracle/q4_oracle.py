@@ -54,6 +54,14 @@ def decode_parts(rows: np.ndarray, D: int):
     return o[..., r], s[..., r] * (code - 8.0)
 
 
+def code_part(rows: np.ndarray, D: int) -> np.ndarray:
+    """scale * code per channel, in 64 bits."""
+    _, v = decode_parts(rows, D)
+    G = D // GROUP
+    s = np.ascontiguousarray(np.ascontiguousarray(rows)[..., D // 2: D // 2 + 2 * G]).view(np.float16).astype(np.float64)
+    return v + 8.0 * s[..., np.arange(D) // GROUP]
+
+
 def decode_rows(rows: np.ndarray, D: int) -> np.ndarray:
     o, v = decode_parts(rows, D)
     return o + v
@@ -70,7 +78,7 @@ def attend(pool: np.ndarray, D: int, q: np.ndarray, tables, lens, scale: float):
     """pool [2, NB, BS, H, row] bytes, q [B, heads, D].
 
     Returns (out [B, heads, D], weights: list of [H, n] per sequence, bound [B, heads, D], spread [B, heads]): `bound` is
-    sum_t p_t (|offset| + |scale (code - 8)|), `spread` the largest scale * sum_d |q| (|offset| + |scale (code - 8)|) of a
+    sum_t p_t (|offset| + |scale (code - 8)| + scale code), `spread` the largest scale * sum_d |q| (|offset| + |scale (code - 8)|) of a
     token, which rounding errors of the weighted sum and of the logits are relative to.
     """
     B, heads, _ = q.shape
@@ -82,7 +90,9 @@ def attend(pool: np.ndarray, D: int, q: np.ndarray, tables, lens, scale: float):
         w = np.zeros((H, n))
         if n:
             ko, kv = decode_parts(sequence(pool[0], tables[b], n), D)
-            vo, vv = decode_parts(sequence(pool[1], tables[b], n), D)
+            values = sequence(pool[1], tables[b], n)
+            vo, vv = decode_parts(values, D)
+            size = np.abs(vo) + np.abs(vv) + code_part(values, D)
             for j in range(heads):
                 h = j // group
                 l = scale * ((ko[:, h] + kv[:, h]) @ q[b, j])
@@ -90,7 +100,7 @@ def attend(pool: np.ndarray, D: int, q: np.ndarray, tables, lens, scale: float):
                 p = np.exp(l - l.max())
                 p /= p.sum()
                 out[b, j] = p @ (vo[:, h] + vv[:, h])
-                bound[b, j] = p @ (np.abs(vo[:, h]) + np.abs(vv[:, h]))
+                bound[b, j] = p @ size[:, h]
                 w[h] += p
         weights.append(w)
     return out, weights, bound, spread

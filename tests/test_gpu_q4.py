@@ -2,8 +2,10 @@
 
 Tolerances, per output value, with h = finfo(dtype).eps / 2 the half step of the output type:
 
-  attention  h |ref| for the final rounding, plus sum_t p_t (|o| + |s (c - 8)|) times
-             2 * 2^-11 for a weight rounded to 16 bits, once before and once after the product with a scale, plus
+  attention  h |ref| for the final rounding, plus bound = sum_t p_t (|o| + |s (c - 8)| + s c) times
+             2^-11: out = sum p s c + sum p (o - 8 s). A weight p rounded to 16 bits, p (1 + d) with |d| <= 2^-11, is the
+             same in both sums and adds at most 2^-11 p |o + s (c - 8)|; the product p s, rounded once more, enters the
+             first sum only and adds at most 2^-11 p s c; plus bound times
              2 * 2^-17 * spread: a logit is a sum of at most 2^7 + 2^1 terms in 32 bits, so it is off by at most 2^-17 of
              the sum of their absolute values (spread), a weight by that share, and its sum by the same once more;
              plus 2^-24, the smallest step of an fp16 result.
@@ -75,7 +77,7 @@ def dev(a):
 
 def check_out(got, ref, bound, spread, dtype, what=""):
     h = torch.finfo(dtype).eps / 2
-    tol = h * np.abs(ref) + bound * (2 * 2.0 ** -11 + 2 * 2.0 ** -17 * spread[..., None]) + 2.0 ** -24
+    tol = h * np.abs(ref) + bound * (2.0 ** -11 + 2 * 2.0 ** -17 * spread[..., None]) + 2.0 ** -24
     err = np.abs(got.double().cpu().numpy() - ref)
     assert (err <= tol).all(), f"{what}: {np.max(err / tol)} of the tolerance at {np.unravel_index(np.argmax(err / tol), err.shape)}"
 
