@@ -55,9 +55,12 @@ struct AttendShape {
   uint32_t stages;       // tiles in a warp's ring
   int32_t block_shift;   // log2 of the block size where it is a power of two >= 16 (a tile lies in one block), else -1
   uint32_t grid;         // CTAs
-  uint32_t min_units;    // least units worth a CTA
   uint32_t items;        // num_seqs * head_groups
 };
+
+// What an item costs besides its units, in units: queries, the subsets' meeting, the result (measured: 3 us against
+// 1.2 us for a unit of 32 tokens and 8 heads). Without it the CTAs with many short sequences finish last.
+constexpr uint32_t kItemCost = 3;
 
 struct AttendArgs {
   TokenSide pool;
@@ -204,6 +207,34 @@ __device__ __forceinline__ void lds_matrices(uint32_t (&m)[4], uint32_t a) {
 __device__ __forceinline__ void copy16(uint32_t dst, uint64_t src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+// Two of them, if `on` is not 0, without a branch.
+template <int kOff0, int kOff1>
+__device__ __forceinline__ void copy16_pair(uint32_t dst, uint64_t src0, uint64_t src1, uint32_t on) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.u32 p, %3, 0;\n"
+      "@p cp.async.cg.shared.global [%0+%4], [%1], 16;\n"
+      "@p cp.async.cg.shared.global [%0+%5], [%2], 16;\n"
+      "}\n" ::"r"(dst), "l"(src0), "l"(src1), "r"(on), "n"(kOff0), "n"(kOff1)
+      : "memory");
+}
+// A lane's share of a tile of 16 key and 16 value rows of R bytes: one chunk of 16 bytes in 32 of each plane.
+template <int R, int J>
+__device__ __forceinline__ void copy_tile(uint32_t dst, uint64_t k, uint64_t v, const uint32_t (&row_off)[(R + 31) / 32], uint32_t tail_lane) {
+  copy16_pair<512 * J, 16 * R + 512 * J>(dst, k + row_off[J], v + row_off[J], (J + 1) * 32 <= R ? 1u : tail_lane);
+  if constexpr (J + 1 < (R + 31) / 32) copy_tile<R, J + 1>(dst, k, v, row_off, tail_lane);
+}
+template <int kOff>
+__device__ __forceinline__ void sts_word(uint32_t a, uint32_t v) {
+  asm volatile("st.shared.u32 [%0+%1], %2;" ::"r"(a), "n"(kOff), "r"(v) : "memory");
+}
+template <int kOff>
+__device__ __forceinline__ uint32_t lds_word(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1+%2];" : "=r"(v) : "r"(a), "n"(kOff));
+  return v;
+}
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copies_wait() {
@@ -211,16 +242,17 @@ __device__ __forceinline__ void copies_wait() {
 }
 
 constexpr uint32_t kNib0 = 0x000f000fu, kNib1 = 0x00f000f0u;
-constexpr uint32_t kLoHalves = 0x5410u, kHiHalves = 0x7632u;  // prmt selectors: low / high halves of two words
+// prmt selectors, from two words: their low (high) halves; those halves shifted down by eight bits, with bits above that
+// the nibble masks drop
+constexpr uint32_t kLoHalves = 0x5410u, kHiHalves = 0x7632u, kLoUpper = 0x5511u, kHiUpper = 0x7733u;
 constexpr float kFirstRef = -1e30f;                            // reference before any token
 
-// Where a CTA's share of the units begins, found by all threads together.
+// A CTA's share. The batch is a line on which every item takes kItemCost and then one place per unit; a CTA has the units
+// whose places lie in its piece of the line.
 struct Share {
-  uint32_t b, hg, unit;  // first unit: sequence, head group, unit within the item
-  uint32_t count;        // units
-  uint32_t grid;         // CTAs that have a share
-  uint64_t total;        // units of the batch
-  uint64_t first;        // index of the first unit in the batch
+  uint32_t b, hg, unit;  // first item and unit
+  uint32_t place, end;   // place of that item's unit 0; end of the share
+  uint32_t each, extra;  // the first `extra` CTAs have each + 1 places, the others each
 };
 
 // One CTA per SM. At D = 256 a warp's accumulators and queries take over 128 registers, so it has eight warps.
@@ -229,7 +261,7 @@ __host__ __device__ constexpr int attend_max_warps(int D) { return D == 256 ? 8 
 __host__ __device__ constexpr int attend_stages(int D) { return D == 64 ? 6 : 4; }
 
 // Decode attention; see the top of the file. kPrecise: carry the remainder of p s_r (fp16 outputs).
-template <typename T, int D>
+template <typename T, int D, bool kScores>
 __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const __grid_constant__ AttendArgs a) {
   constexpr int G = q4_groups(D), R = q4_row_bytes(D);
   constexpr int KW = D / 32;  // words of codes per lane and token, keys (two units of every group)
@@ -239,146 +271,200 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
   constexpr int kTileBytes = 32 * R + 16, kAttendStages = attend_stages(D);
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Share share;
-  __shared__ uint64_t scan[16];
+  __shared__ uint32_t scan[16];
 
   const AttendShape &sh = a.sh;
   const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   grid_launch_dependents();
   if (tid == 0) a.cta_item[blockIdx.x] = -1;
-  // The batch's units and this CTA's share of them. A thread takes a run of consecutive sequences.
+  // The line's length and this CTA's piece. A thread takes a run of consecutive sequences.
   {
     const uint32_t per = (a.num_seqs + blockDim.x - 1) / blockDim.x;
     const uint32_t b0 = min(a.num_seqs, tid * per), b1 = min(a.num_seqs, b0 + per);
-    uint64_t mine = 0;
-    for (uint32_t b = b0; b < b1; ++b) mine += seq_units(a, seq_length(a, b, blockIdx.x == 0)) * (uint64_t)sh.head_groups;
-    uint64_t upto = mine;
+    uint32_t mine = 0, n0 = 0;
+    for (uint32_t b = b0; b < b1; ++b) {
+      const uint32_t n = seq_length(a, b, blockIdx.x == 0);
+      if (b == b0) n0 = n;
+      mine += (seq_units(a, n) + kItemCost) * sh.head_groups;
+    }
+    uint32_t upto = mine;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
-      const uint64_t other = __shfl_up_sync(0xffffffffu, upto, m);
+      const uint32_t other = __shfl_up_sync(0xffffffffu, upto, m);
       if (lane >= m) upto += other;
     }
     if (lane == 31) scan[warp] = upto;
     __syncthreads();
-    uint64_t before = 0, total = 0;
+    uint32_t before = 0, total = 0;
     for (uint32_t w = 0; w < blockDim.x / 32; ++w) {
       if (w < warp) before += scan[w];
       total += scan[w];
     }
     before += upto - mine;
-    const uint64_t worth = max((uint64_t)1, total / sh.min_units);
-    const uint32_t grid = (uint32_t)min((uint64_t)gridDim.x, worth);
-    const uint64_t first = blockIdx.x < grid ? total * blockIdx.x / grid : total;
-    const uint64_t end = blockIdx.x < grid ? total * (blockIdx.x + 1) / grid : total;
-    if (tid == 0) {
-      share.count = (uint32_t)(end - first);
-      share.grid = grid;
-      share.total = total;
-      share.first = first;
-    }
-    if (first < end && before <= first && first < before + mine) {
-      uint64_t at = before;
-      uint32_t b = b0;
-      for (;; ++b) {
-        const uint64_t u = seq_units(a, seq_length(a, b, false)) * (uint64_t)sh.head_groups;
+    const uint32_t each = total / gridDim.x, extra = total - each * gridDim.x;
+    const uint32_t first = each * blockIdx.x + min(blockIdx.x, extra);
+    if (first >= total && tid == 0) share = Share{0, 0, 0, 0, 0, 0, 0};  // more CTAs than places
+    if (before <= first && first < before + mine) {
+      uint32_t at = before, n = n0, b = b0;
+      for (;;) {
+        const uint32_t u = (seq_units(a, n) + kItemCost) * sh.head_groups;
         if (first < at + u) break;
         at += u;
+        n = seq_length(a, ++b, false);
       }
-      const uint32_t units = seq_units(a, seq_length(a, b, false));
+      const uint32_t one = seq_units(a, n) + kItemCost, r = (first - at) / one, rest = first - at - r * one;
       share.b = b;
-      share.hg = (uint32_t)((first - at) / units);
-      share.unit = (uint32_t)((first - at) % units);
+      share.hg = r;
+      share.unit = rest > kItemCost ? rest - kItemCost : 0;
+      share.place = at + r * one + kItemCost;
+      share.end = first + each + (blockIdx.x < extra ? 1 : 0);
+      share.each = each;
+      share.extra = extra;
     }
     __syncthreads();
   }
-  uint32_t left = share.count;
-  if (left == 0) return;
-  uint32_t b = share.b, hg = share.hg, unit = share.unit;
+  const uint32_t end = share.end;
+  uint32_t b = share.b, hg = share.hg, unit = share.unit, place = share.place;
+  if (place + unit >= end) return;  // no unit of its own
 
   const uint32_t hl = warp % sh.heads_cta;                 // KV head within the CTA
   const uint32_t nt = warp / sh.heads_cta % sh.ntiles;     // tile of query heads
   const uint32_t sub = warp / (sh.heads_cta * sh.ntiles);  // token subset
   const uint32_t g = lane / 4, q4 = lane % 4, t_sub = sub * 16;
 
-  // ---- loads: a ring of tiles of 16 key rows and 16 value rows, and a word that says which tokens count
-  const uint32_t ring = smem_u32(smem) + warp * kAttendStages * kTileBytes;
+  // ---- loads: a ring of tiles of 16 key rows and 16 value rows, and a word that says which tokens count: kByLength, or
+  // a mask where a block lies outside the pool (read only once such a block was met)
+  constexpr uint32_t kByLength = 0x10000u;
   constexpr int kChunks = R / 16, kCopies = (R + 31) / 32;  // 16-byte chunks of a row; per lane and plane of a tile
-  uint32_t row_off[kCopies];                                // chunk lane + 32 j of a plane: offset from its first row
+  const uint32_t ring = smem_u32(smem) + warp * kAttendStages * kTileBytes, ring_end = ring + kAttendStages * kTileBytes;
+  uint32_t row_off[kCopies];  // chunk lane + 32 j of a plane: offset from its first row
 #pragma unroll
   for (int j = 0; j < kCopies; ++j) {
     const uint32_t c = lane + 32 * j;
     row_off[j] = c / kChunks * (uint32_t)a.pool.token_stride + c % kChunks * 16;
   }
-  uint32_t to_load = left, slot_in = ring;
-  uint32_t ib = b, ihg = hg, iunit = unit, in = seq_length(a, b, false), iunits = seq_units(a, in);
-  int32_t id = -1;  // block of the next tile to load, read one tile ahead
-  auto fetch_id = [&]() {
-    const uint32_t t = iunit * sh.tokens + t_sub;
-    if (sh.block_shift >= 0 && t < in) id = a.tables[ib * a.table_stride + (t >> sh.block_shift)];
+  const uint32_t tail_lane = R % 32 == 0 || lane < R % 32;  // has a chunk in the last, partial round
+  const uint32_t shift = (uint32_t)sh.block_shift & 31u, block_mask = (1u << shift) - 1u;
+  const bool paged = sh.block_shift >= 0;
+  bool holes = false;              // a block outside the pool was met
+  // Where the next tile to load lies. `run` tiles from here on are 16 tokens of one block each, their blocks at hand in
+  // `ids`; `after` more units of the item follow in the share.
+  uint32_t ib = b, ihg = hg, iplace = place;
+  uint32_t it = unit * sh.tokens + t_sub, in = seq_length(a, b, false), run = 0;
+  uint32_t after = min(seq_units(a, in), end - place) - unit;
+  uint64_t ibase = 0;              // this head's rows of block 0
+  const int32_t *itab = nullptr;   // the sequence's table
+  uint32_t window = 0;             // and its entries window + lane, window + 32 + lane
+  int32_t ids = 0, ids_next = 0;
+  bool ireal = false;              // whether this warp has a head there
+  auto entry = [&](uint32_t i) { return itab[min(i + lane, (in - 1) >> shift)]; };
+  auto enter = [&]() {
+    const uint32_t h = ihg * sh.heads_cta + hl;
+    ireal = h < a.kv_heads;
+    ibase = a.layer_base + h * a.pool.head_stride;
+    itab = a.tables + ib * a.table_stride;
+    window = it >> shift;
+    if (paged && in > 0) {
+      ids = entry(window);
+      ids_next = entry(window + 32);
+    }
   };
-  auto load = [&]() {
-    if (to_load > 0) {
-      --to_load;
-      const uint32_t t = iunit * sh.tokens + t_sub, h = ihg * sh.heads_cta + hl;
-      uint32_t mask = 0;
-      if (t < in && h < a.kv_heads) {
-        const uint32_t count = min(16u, in - t);
-        if (sh.block_shift >= 0) {
-          if ((uint32_t)id < a.pool.num_blocks) {
-            const uint64_t src = a.layer_base + (uint64_t)(uint32_t)id * a.pool.block_stride + h * a.pool.head_stride +
-                                 (t & ((1u << sh.block_shift) - 1u)) * a.pool.token_stride;
-            mask = (1u << count) - 1u;
-#pragma unroll
-            for (int j = 0; j < kCopies; ++j) {
-              const bool inside = (j + 1) * 32 <= R || lane + 32 * j < R;
-              if (inside && (count == 16 || lane + 32 * j < count * kChunks)) {
-                copy16(slot_in + 16 * lane + 512 * j, src + row_off[j]);
-                copy16(slot_in + 16 * R + 16 * lane + 512 * j, src + a.pool.plane_stride + row_off[j]);
-              }
-            }
-          } else if (lane == 0) {
-            report(a.status, kStatusIdRange, id);
-          }
-        } else {
-          // Blocks of any size: every row is looked up.
-          auto row_at = [&](uint32_t row) -> uint64_t {
-            const uint32_t blk = (t + row) / a.pool.block_size;
-            const int32_t i = a.tables[ib * a.table_stride + blk];
-            if ((uint32_t)i >= a.pool.num_blocks) {
-              report(a.status, kStatusIdRange, i);
-              return 0;
-            }
-            return a.layer_base + (uint64_t)i * a.pool.block_stride + h * a.pool.head_stride +
-                   (t + row - blk * a.pool.block_size) * a.pool.token_stride;
-          };
-          mask = __ballot_sync(0xffffffffu, lane < count && row_at(lane) != 0);
+  auto next_item = [&]() {
+    iplace += seq_units(a, in) + kItemCost;
+    if (iplace >= end) return;
+    if (++ihg == sh.head_groups) {
+      ihg = 0;
+      in = seq_length(a, ++ib, false);
+    }
+    after = min(seq_units(a, in), end - iplace);
+    it = t_sub;
+    enter();
+  };
+  auto begin_run = [&]() {
+    if (!paged || !ireal || it + 16 > in) return;
+    if ((it >> shift) - window >= 32) {  // a unit has at most 256 tokens, 16 blocks
+      window += 32;
+      ids = ids_next;
+      ids_next = entry(window + 32);
+    }
+    if (__any_sync(0xffffffffu, (uint32_t)ids >= a.pool.num_blocks)) return;
+    const uint32_t whole = (in - it - 16) / sh.tokens + 1;                                          // tiles of 16 tokens
+    const uint32_t known = (uint32_t)((((uint64_t)window + 32) << shift) - it + sh.tokens - 1) / sh.tokens;  // in the window
+    run = min(min(whole, known), after);
+    after -= run;
+  };
+  // A tile that is not 16 tokens of one block: the end of a sequence, a block outside the pool, other block sizes.
+  auto load_rest = [&](uint32_t slot) {
+    uint32_t word = kByLength;
+    if (it < in && ireal) {
+      const uint32_t count = min(16u, in - it);
+      auto row_at = [&](uint32_t row) -> uint64_t {
+        const uint32_t blk = (it + row) / a.pool.block_size;
+        const int32_t i = itab[blk];
+        if ((uint32_t)i >= a.pool.num_blocks) {
+          report(a.status, kStatusIdRange, i);
+          return 0;
+        }
+        return ibase + (uint64_t)(uint32_t)i * a.pool.block_stride + (it + row - blk * a.pool.block_size) * a.pool.token_stride;
+      };
+      const uint32_t mask = __ballot_sync(0xffffffffu, lane < count && row_at(lane) != 0);
+      if (mask != (1u << count) - 1u) {
+        holes = true;
+        word = mask;
+      }
 #pragma unroll 1
-          for (uint32_t c = lane; c < count * kChunks; c += 32) {
-            const uint64_t src = row_at(c / kChunks);
-            if (src == 0) continue;
-            copy16(slot_in + 16 * c, src + c % kChunks * 16);
-            copy16(slot_in + 16 * R + 16 * c, src + a.pool.plane_stride + c % kChunks * 16);
-          }
-        }
+      for (uint32_t c = lane; c < count * kChunks; c += 32) {
+        const uint64_t src = row_at(c / kChunks);
+        if (src == 0) continue;
+        copy16(slot + 16 * c, src + c % kChunks * 16);
+        copy16(slot + 16 * R + 16 * c, src + a.pool.plane_stride + c % kChunks * 16);
       }
-      if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(slot_in + 32 * R), "r"(mask) : "memory");
-      slot_in = slot_in + kTileBytes == ring + kAttendStages * kTileBytes ? ring : slot_in + kTileBytes;
-      if (++iunit == iunits) {
-        iunit = 0;
-        if (++ihg == sh.head_groups) {
-          ihg = 0;
-          if (to_load > 0) {
-            in = seq_length(a, ++ib, false);
-            iunits = seq_units(a, in);
-          }
-        }
-      }
-      if (to_load > 0) fetch_id();
+    }
+    sts_word<32 * R>(slot, word);
+    it += sh.tokens;
+    if (--after == 0) next_item();
+  };
+  auto load = [&](uint32_t slot) {
+    if (run == 0 && after > 0) {
+      begin_run();
+      if (run == 0) load_rest(slot);
+    } else if (run > 0 && holes) {
+      sts_word<32 * R>(slot, kByLength);
+    }
+    if (run > 0) {
+      const uint32_t id = (uint32_t)__shfl_sync(0xffffffffu, ids, (it >> shift) - window);
+      const uint64_t k = ibase + (uint64_t)id * (uint32_t)a.pool.block_stride +
+                         (uint64_t)(it & block_mask) * (uint32_t)a.pool.token_stride;
+      const uint64_t v = k + a.pool.plane_stride;
+      const uint32_t dst = slot + 16 * lane;
+      copy_tile<R, 0>(dst, k, v, row_off, tail_lane);
+      it += sh.tokens;
+      if (--run == 0 && after == 0) next_item();
     }
     copies_commit();  // an empty group at the end keeps the count
   };
-  fetch_id();
+  enter();
 #pragma unroll 1
-  for (int k = 0; k < kAttendStages - 1; ++k) load();
+  for (uint32_t s = ring; s < ring_end; s += kTileBytes) sts_word<32 * R>(s, kByLength);
+  uint4 q_raw[G];  // eight channels of every group of the query row of this lane
+  auto fetch_query = [&]() {
+    const uint32_t h = hg * sh.heads_cta + hl, j = nt * 8 + g;
+    const bool mine = h < a.kv_heads && j < a.group;
+    const uint64_t src = a.query + b * a.query_seq_stride + ((uint64_t)(h * a.group + j) * D + 8 * q4) * 2;
+#pragma unroll
+    for (int r = 0; r < G; ++r) {
+      q_raw[r] = make_uint4(0, 0, 0, 0);
+      if (mine && a.align >= 16) {
+        q_raw[r] = *reinterpret_cast<const uint4 *>(src + r * 64);
+      } else if (mine) {
+        const uint16_t *e = reinterpret_cast<const uint16_t *>(src + r * 64);
+        q_raw[r] = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
+                              e[6] | (uint32_t)e[7] << 16);
+      }
+    }
+  };
+#pragma unroll 1
+  for (uint32_t s = ring; s < ring_end - kTileBytes; s += kTileBytes) load(s);
 
   // Tokens are fragment rows in their order. Rows are R apart, an odd multiple of 16 bytes at D = 64 and 128: the value
   // loads and the matrix loads touch every bank once.
@@ -391,37 +477,27 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
   const uint32_t km_at = (mt + 8 * (mi & 1)) * R + (G == 8 && mi >= 2 ? 2 * G : 0);
   const uint32_t vm_at = (16 + mt + 8 * (mi >> 1)) * R + (G == 8 && (mi & 1) ? 2 * G : 0);
   const uint32_t scale_bits = G == 8 || g < (uint32_t)G ? 0x40004000u : 0u;  // >= 2, where this lane's rows are scales
-  uint32_t slot_out = ring;
+  uint32_t slot = ring, slot_before = ring_end - kTileBytes;  // of the tile to compute, and of the one before it
 
   float *merge = reinterpret_cast<float *>(smem + sh.warps * kAttendStages * kTileBytes);  // [(warps - warps/subsets)][8][D + 2]
 
-  while (left > 0) {
+  while (place < end) {
     const uint32_t n = seq_length(a, b, false), units = seq_units(a, n);
-    const uint32_t unit0 = unit, count = min(left, units - unit);
+    const uint32_t unit0 = unit, count = min(units, end - place) - unit;
     const uint32_t h = hg * sh.heads_cta + hl;
     const bool active = h < a.kv_heads;
     const uint32_t j0 = nt * 8;  // first query head of the tile, within the group
+    fetch_query();
 
     // ---- the queries of this tile as B fragments
     uint32_t qf[G][4];
     uint32_t qo[4];     // Q_r (offsets) and -8 Q_r (scales) as two halves: B fragments
     float c0, c1;       // logit factors of heads 2 q4, 2 q4 + 1
     {
-      const bool mine = active && j0 + g < a.group;
-      const uint64_t src = a.query + b * a.query_seq_stride + ((uint64_t)(min(h, a.kv_heads - 1) * a.group + j0 + g) * D + 8 * q4) * 2;
       auto load8 = [&](float (&x)[8], int r) {
-        if (!mine) {
+        const uint32_t w[4] = {q_raw[r].x, q_raw[r].y, q_raw[r].z, q_raw[r].w};
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = 0.f;
-        } else if (a.align >= 16) {
-          const uint4 v = *reinterpret_cast<const uint4 *>(src + r * 64);
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) unpack2<T>(w[i], x[2 * i], x[2 * i + 1]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(reinterpret_cast<const T *>(src + r * 64)[i]);
-        }
+        for (int i = 0; i < 4; ++i) unpack2<T>(w[i], x[2 * i], x[2 * i + 1]);
       };
       float top = 0.f;
 #pragma unroll
@@ -445,7 +521,7 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
 #pragma unroll
       for (int r = 0; r < G; ++r) {
         float x[8], sum = 0.f;
-        load8(x, r);  // a second read, from L1, costs less than the registers
+        load8(x, r);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           x[i] = __half2float(__float2half_rn(x[i] * down));
@@ -489,10 +565,10 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
         for (int k = 0; k < 4; ++k) acc[r][i][k] = 0.f;
     float ref0 = kFirstRef, ref1 = kFirstRef, sum0 = 0.f, sum1 = 0.f;
     float lift = 8.f;  // p is held times 2^lift
-    float *lg = a.score_base && active
-                    ? a.logits + ((uint64_t)b * a.kv_heads * a.group + (uint64_t)h * a.group + j0 + 2 * q4) * a.logit_stride
-                    : nullptr;
-    const bool store0 = lg && j0 + 2 * q4 < a.group, store1 = lg && j0 + 2 * q4 + 1 < a.group;
+    float *lg = nullptr;  // logits of head 2 q4; head 2 q4 + 1 lies one row further
+    if constexpr (kScores)
+      lg = a.logits + ((uint64_t)b * a.kv_heads * a.group + (uint64_t)h * a.group + j0 + 2 * q4) * a.logit_stride;
+    const bool store0 = active && j0 + 2 * q4 < a.group, store1 = active && j0 + 2 * q4 + 1 < a.group;
 
     // Moves the references of this lane's two heads and everything held relative to them.
     auto rescale = [&](float to0, float to1) {
@@ -516,14 +592,19 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
       accx[3] *= f1;
     };
 
+    int left = active ? (int)n - (int)(unit0 * sh.tokens + t_sub) : 0;  // tokens from this warp's next tile on
     for (uint32_t k = 0; k < count; ++k) {
       copies_wait<kAttendStages - 2>();
       __syncwarp();  // this tile's rows are there for every lane, and every lane has left the slot of the tile before
-      load();
-      uint32_t mask;
-      asm volatile("ld.shared.u32 %0, [%1+%2];" : "=r"(mask) : "r"(slot_out), "n"(32 * R));
+      load(slot_before);
+      uint32_t mask = left >= 16 ? 0xffffu : (left > 0 ? (1u << left) - 1u : 0u);
+      if (holes) {
+        const uint32_t word = lds_word<32 * R>(slot);
+        if (word != kByLength) mask = word;
+      }
+      left -= (int)sh.tokens;
       if (mask) {
-        const uint32_t base = slot_out;
+        const uint32_t base = slot;
         // ---- logits of 16 tokens
         float l[4];
         {
@@ -540,9 +621,9 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
           float x[4];
 #pragma unroll
           for (int r = 0; r < G; ++r) {
-            const uint32_t sel = r % 2 ? kHiHalves : kLoHalves;
+            const uint32_t sel = r % 2 ? kHiHalves : kLoHalves, up = r % 2 ? kHiUpper : kLoUpper;
             const uint32_t u0 = __byte_perm(w0[r / 2], w0[KW / 2 + r / 2], sel), u1 = __byte_perm(w1[r / 2], w1[KW / 2 + r / 2], sel);
-            const uint32_t y0 = u0 >> 8, y1 = u1 >> 8;
+            const uint32_t y0 = __byte_perm(w0[r / 2], w0[KW / 2 + r / 2], up), y1 = __byte_perm(w1[r / 2], w1[KW / 2 + r / 2], up);
             float d[4] = {0.f, 0.f, 0.f, 0.f};
             mma_k16(d, u0 & kNib0, u1 & kNib0, u0 & kNib1, u1 & kNib1, qf[r][0], qf[r][1], d);
             mma_k16(d, y0 & kNib0, y1 & kNib0, y0 & kNib1, y1 & kNib1, qf[r][2], qf[r][3], d);
@@ -566,6 +647,12 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
         lds_words<SW, R + D / 2>(sv[1], va);
         lds_words<SW, 8 * R + D / 2>(sv[2], va);
         lds_words<SW, 9 * R + D / 2>(sv[3], va);
+        uint32_t w[4][VW];  // their codes
+        const uint32_t vc = va + g * (D / 16);
+        lds_words<VW, 0>(w[0], vc);
+        lds_words<VW, R>(w[1], vc);
+        lds_words<VW, 8 * R>(w[2], vc);
+        lds_words<VW, 9 * R>(w[3], vc);
         if (mask != 0xffffu) {
           // Tokens that do not count: no weight, and no scale or offset that could be anything (0 * NaN).
           if (!(mask >> tk & 1)) l[0] = l[1] = -INFINITY;
@@ -581,7 +668,7 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
               for (int w = 0; w < SW; ++w) sv[i][w] = 0;
             }
         }
-        if (lg) {
+        if constexpr (kScores) {
           const uint32_t t = (unit0 + k) * sh.tokens + t_sub + tk;
           if (mask >> tk & 1) {
             if (store0) lg[t] = l[0];
@@ -630,19 +717,13 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
         mma_k16(accx, m[0], m[1], m[2], m[3], b0, b1, accx);
         if constexpr (kPrecise) mma_k16(accx, m[0], m[1], m[2], m[3], bl0, bl1, accx);
         // ---- values
-        uint32_t w[4][VW];
-        const uint32_t vc = va + g * (D / 16);
-        lds_words<VW, 0>(w[0], vc);
-        lds_words<VW, R>(w[1], vc);
-        lds_words<VW, 8 * R>(w[2], vc);
-        lds_words<VW, 9 * R>(w[3], vc);
 #pragma unroll
         for (int r = 0; r < G; ++r) {
-          const uint32_t sel = r % 2 ? kHiHalves : kLoHalves;
+          const uint32_t sel = r % 2 ? kHiHalves : kLoHalves, up = r % 2 ? kHiUpper : kLoUpper;
           const uint32_t s01 = __byte_perm(sv[0][r / 2], sv[1][r / 2], sel), s23 = __byte_perm(sv[2][r / 2], sv[3][r / 2], sel);
           const uint32_t e0 = mul_half2(b0, s01), e1 = mul_half2(b1, s23);
           const uint32_t u01 = __byte_perm(w[0][r / 2], w[1][r / 2], sel), u23 = __byte_perm(w[2][r / 2], w[3][r / 2], sel);
-          const uint32_t y01 = u01 >> 8, y23 = u23 >> 8;
+          const uint32_t y01 = __byte_perm(w[0][r / 2], w[1][r / 2], up), y23 = __byte_perm(w[2][r / 2], w[3][r / 2], up);
           mma_k16(acc[r][0], u01 & kNib0, u01 & kNib1, u23 & kNib0, u23 & kNib1, e0, e1, acc[r][0]);
           mma_k16(acc[r][1], y01 & kNib0, y01 & kNib1, y23 & kNib0, y23 & kNib1, e0, e1, acc[r][1]);
           if constexpr (kPrecise) {
@@ -653,7 +734,9 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
           }
         }
       }
-      slot_out = slot_out + kTileBytes == ring + kAttendStages * kTileBytes ? ring : slot_out + kTileBytes;
+      slot_before = slot;
+      slot += kTileBytes;
+      if (slot == ring_end) slot = ring;
     }
 
     // ---- the segment's result: o[r][i] of channel 32 r + 4 g + i, heads 2 q4 and 2 q4 + 1
@@ -743,7 +826,7 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
               for (int i = 0; i < 4; ++i) out[32 * r + i] = from_f32<T>(acc[r][i / 2][2 * (i % 2) + c] * inv);
             }
           }
-          if (lg && g == 0) a.lse[(uint64_t)b * a.kv_heads * a.group + head] = sum == 0.f ? INFINITY : ref + lg2(sum);
+          if (kScores && g == 0) a.lse[(uint64_t)b * a.kv_heads * a.group + head] = sum == 0.f ? INFINITY : ref + lg2(sum);
         } else {
           const uint64_t slot = 2ull * blockIdx.x + (unit0 == 0 ? 1 : 0);
           const uint64_t row = slot * sh.heads_cta * a.group + hl * a.group + j;
@@ -756,16 +839,15 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
       }
     }
     if (tid == 0 && unit0 + count == units) {
-      // This CTA ends the item: say where it began.
-      const uint64_t end = share.first + (share.count - left) + count;          // units up to the item's end
-      const uint64_t begin = end - units;
-      const uint32_t from = (uint32_t)(((begin + 1) * share.grid - 1) / share.total);  // the CTA that has unit `begin`
+      // This CTA ends the item: say which CTA has its first unit.
+      const uint32_t long_ones = share.extra * (share.each + 1);
+      const uint32_t from = place < long_ones ? place / (share.each + 1) : share.extra + (place - long_ones) / share.each;
       const uint32_t item = b * sh.head_groups + hg;
       a.item_span[item] = make_int2((int)from, (int)blockIdx.x);
       if (!whole) a.cta_item[blockIdx.x] = (int)item;
     }
-    left -= count;
     unit = 0;
+    place += units + kItemCost;
     if (++hg == sh.head_groups) {
       hg = 0;
       ++b;
@@ -803,7 +885,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join(const __grid_cons
   float acc[C], sum = 0.f, top = kFirstRef;
 #pragma unroll
   for (int c = 0; c < C; ++c) acc[c] = 0.f;
-  constexpr int kAhead = 8;  // parts whose loads are in flight together
+  constexpr int kAhead = D == 256 ? 5 : 10;  // parts whose loads are in flight together: all of 148 CTAs'
   for (uint32_t i0 = mine; i0 < parts; i0 += W * kAhead) {
     float v[kAhead][C];
     float2 ml[kAhead];
@@ -891,7 +973,20 @@ __global__ void __launch_bounds__(256) attend_scores(const __grid_constant__ Att
     const uint32_t n = seq_length(a, b, false), t = (uint32_t)(i % chunks) * kScoreChunk + threadIdx.x * 4;
     if (t >= n) continue;
     const uint64_t head = (uint64_t)bh * a.group;
-    float w[4] = {0.f, 0.f, 0.f, 0.f};
+    float *sc[4];
+    float old[4], w[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {  // the entries' addresses and old values, while the logits come
+      sc[k] = nullptr;
+      old[k] = 0.f;
+      if (t + k >= n) continue;
+      const uint32_t blk = (t + k) / a.pool.block_size;
+      const int32_t id = a.tables[b * a.table_stride + blk];
+      if ((uint32_t)id >= a.pool.num_blocks) continue;
+      sc[k] = reinterpret_cast<float *>(a.score_base + (uint64_t)id * a.score_block_stride) + (uint64_t)h * a.pool.block_size +
+              (t + k - blk * a.pool.block_size);
+      old[k] = *sc[k];
+    }
 #pragma unroll 8
     for (uint32_t j = 0; j < a.group; ++j) {
       const float lse = a.lse[head + j];
@@ -902,15 +997,8 @@ __global__ void __launch_bounds__(256) attend_scores(const __grid_constant__ Att
       w[3] += ex2(l.w - lse);
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (t + k >= n) break;
-      const uint32_t blk = (t + k) / a.pool.block_size;
-      const int32_t id = a.tables[b * a.table_stride + blk];
-      if ((uint32_t)id >= a.pool.num_blocks) continue;
-      float *sc = reinterpret_cast<float *>(a.score_base + (uint64_t)id * a.score_block_stride) +
-                  (uint64_t)h * a.pool.block_size + (t + k - blk * a.pool.block_size);
-      *sc += w[k];
-    }
+    for (int k = 0; k < 4; ++k)
+      if (sc[k]) *sc[k] = old[k] + w[k];
   }
 }
 

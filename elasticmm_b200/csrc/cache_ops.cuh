@@ -138,7 +138,6 @@ int attend_shape(const emm_pool *pool, int32_t D, int32_t B, int32_t group, int3
   s.head_groups = (H + most - 1) / most;
   s.heads_cta = (H + s.head_groups - 1) / s.head_groups;
   s.items = (uint32_t)B * s.head_groups;
-  s.min_units = 1;
   const uint64_t sms = (uint64_t)pool->ctx->sm_count;
   s.subsets = std::max(1u, (uint32_t)emm::attend_max_warps(D) / (s.heads_cta * s.ntiles));
   auto units = [&]() {
@@ -150,11 +149,14 @@ int attend_shape(const emm_pool *pool, int32_t D, int32_t B, int32_t group, int3
   s.warps = s.heads_cta * s.ntiles * s.subsets;
   s.block_shift = -1;
   for (int k = 4; k < 31; ++k)
-    if (d.block_size == 1 << k && d.token_stride < 1 << 27) s.block_shift = k;  // a tile's offsets take 32 bits
+    if (d.block_size == 1 << k && d.token_stride < 1 << 27 && d.block_stride <= 0xffffffffll)  // its offsets take 32 bits
+      s.block_shift = k;
   s.stages = (uint32_t)emm::attend_stages(D);
   const int merge = (int)((s.subsets - 1) * s.heads_cta * s.ntiles * 8 * (uint32_t)(D + 2) * 4);
   *smem_out = (int)(s.warps * s.stages * (32 * R + 16)) + merge;
-  s.grid = (uint32_t)std::min<uint64_t>(units() / s.min_units, sms);
+  if (units() + (uint64_t)emm::kItemCost * s.items > 0x7fffffffull)
+    return fail(EMM_ERR_TOO_LARGE, "q4_attend: %d sequences of up to %d tokens", B, max_len);
+  s.grid = (uint32_t)std::min<uint64_t>(units() + (uint64_t)emm::kItemCost * s.items, sms);
   *out = s;
   return EMM_OK;
 }
@@ -185,7 +187,7 @@ AttendWorkspace attend_workspace(const emm::AttendShape &s, int32_t D, int32_t B
 }
 
 // The kernel's dynamic shared memory is raised to the device's limit once per device.
-template <typename T, int D>
+template <typename T, int D, bool kScores>
 int attend_smem(int device, int smem) {
   static std::atomic<int> limit[kMaxTrackedDevices];
   const bool tracked = device >= 0 && device < kMaxTrackedDevices;
@@ -193,18 +195,23 @@ int attend_smem(int device, int smem) {
   int most = 0;
   EMM_CUDA(cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, device));
   cudaFuncAttributes fa;
-  EMM_CUDA(cudaFuncGetAttributes(&fa, emm::attend_q4<T, D>));
+  EMM_CUDA(cudaFuncGetAttributes(&fa, emm::attend_q4<T, D, kScores>));
   most -= (int)fa.sharedSizeBytes;
   if (smem > most) return fail(EMM_ERR_TOO_LARGE, "q4_attend: %d bytes of shared memory, the device has %d", smem, most);
-  EMM_CUDA(cudaFuncSetAttribute(emm::attend_q4<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+  EMM_CUDA(cudaFuncSetAttribute(emm::attend_q4<T, D, kScores>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
   if (tracked) limit[device].store(most, std::memory_order_release);
   return EMM_OK;
 }
 
 template <typename T, int D>
 int attend_launch(emm_ctx *ctx, const emm::AttendArgs &a, int smem, cudaStream_t st) {
-  if (int rc = attend_smem<T, D>(ctx->device, smem)) return rc;
-  emm::attend_q4<T, D><<<a.sh.grid, a.sh.warps * 32, smem, st>>>(a);
+  if (a.score_base) {
+    if (int rc = attend_smem<T, D, true>(ctx->device, smem)) return rc;
+    emm::attend_q4<T, D, true><<<a.sh.grid, a.sh.warps * 32, smem, st>>>(a);
+  } else {
+    if (int rc = attend_smem<T, D, false>(ctx->device, smem)) return rc;
+    emm::attend_q4<T, D, false><<<a.sh.grid, a.sh.warps * 32, smem, st>>>(a);
+  }
   EMM_CUDA(cudaGetLastError());
   ctx->launches += 1;
   // The two small kernels behind it are placed while it drains.
