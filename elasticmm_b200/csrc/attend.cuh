@@ -36,8 +36,6 @@
 // inside a segment. Bulk copies of a token's heads (640 bytes; 1280 per head of head-major pages) were measured first: an
 // SM completed one in 28 (38) ns whatever was in flight, which held the loads alone to 3.4 (4.7) TB/s.
 #pragma once
-#include <type_traits>
-
 #include "q4.cuh"
 
 namespace emm {
@@ -144,35 +142,6 @@ __device__ __forceinline__ uint32_t fma_half2(uint32_t a, uint32_t b, uint32_t c
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(a), "r"(b), "r"(c));
   return y;
 }
-__device__ __forceinline__ float2 unpack_half2(uint32_t x) {
-  return __half22float2(*reinterpret_cast<const __half2 *>(&x));
-}
-
-// Two 16-bit values of a word.
-template <typename T>
-__device__ __forceinline__ void unpack2(uint32_t w, float &lo, float &hi) {
-  if constexpr (std::is_same<T, __half>::value) {
-    const float2 f = unpack_half2(w);
-    lo = f.x;
-    hi = f.y;
-  } else {
-    lo = __uint_as_float(w << 16);
-    hi = __uint_as_float(w & 0xffff0000u);
-  }
-}
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (std::is_same<T, __half>::value) {
-    uint32_t y;
-    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
-    return y;
-  } else {
-    uint32_t y;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
-    return y;
-  }
-}
-
 // N words from shared memory at a + kOff (aligned to N words, as the row format guarantees).
 template <int N, int kOff>
 __device__ __forceinline__ void lds_words(uint32_t (&w)[N], uint32_t a) {

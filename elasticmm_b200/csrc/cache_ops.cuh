@@ -38,6 +38,9 @@ emm::TokenSide token_side(const emm_pool *p) {
   s.head_stride = (uint64_t)p->desc.head_stride;
   s.num_blocks = (uint32_t)p->desc.num_blocks;
   s.block_size = (uint32_t)p->desc.block_size;
+  s.block_shift = -1;
+  for (int k = 0; k < 31; ++k)
+    if (p->desc.block_size == 1 << k) s.block_shift = k;
   return s;
 }
 
@@ -78,9 +81,12 @@ int q4_rows_impl(emm_pool *pool, bool append, int32_t D, int32_t dtype, int32_t 
                             layer_count > 1 ? (uint64_t)kls : 0, layer_count > 1 ? (uint64_t)vls : 0};
   for (uint64_t v : parts) align = std::min(align, pow2_align(v));
   if (align < 2) return fail(EMM_ERR_ALIGN, "%s: key/value not aligned to their elements", what);
-  const uint64_t units = (uint64_t)T * (uint64_t)pool->desc.num_kv_heads * (uint64_t)(D / 4);
-  const uint64_t blocks = (units + 255) / 256;
-  if ((uint64_t)T * (uint64_t)pool->desc.num_kv_heads > 0xffffffffull || blocks > 0x7fffffffull || layer_count > 32767)
+  // On 32-byte boundaries (where a projection's output lies) a thread takes a group, else four channels.
+  const bool wide = align >= 32;
+  const uint64_t rows = (uint64_t)T * (uint64_t)pool->desc.num_kv_heads;
+  const uint64_t per_block = wide ? (uint64_t)emm::kRowWarps * (32 / emm::q4_groups(D)) : 256 / (uint64_t)(D / 4);
+  const uint64_t blocks = (rows + per_block - 1) / per_block;
+  if (rows > 0xffffffffull || blocks > 0x7fffffffull || layer_count > 32767)
     return fail(EMM_ERR_TOO_LARGE, "%s: %d layers x %d tokens", what, layer_count, T);
 
   emm::Q4RowsArgs a;
@@ -103,11 +109,11 @@ int q4_rows_impl(emm_pool *pool, bool append, int32_t D, int32_t dtype, int32_t 
 #define EMM_Q4_ROWS(T_, D_)                                                                     \
   do {                                                                                          \
     if (append) {                                                                               \
-      if (align >= 8) emm::q4_append<T_, D_, true><<<grid, 256, 0, st>>>(a);                    \
-      else emm::q4_append<T_, D_, false><<<grid, 256, 0, st>>>(a);                              \
+      if (wide) emm::q4_append_rows<T_, D_><<<grid, emm::kRowWarps * 32, 0, st>>>(a);           \
+      else emm::q4_append_units<T_, D_><<<grid, 256, 0, st>>>(a);                               \
     } else {                                                                                    \
-      if (align >= 8) emm::q4_read<T_, D_, true><<<grid, 256, 0, st>>>(a);                      \
-      else emm::q4_read<T_, D_, false><<<grid, 256, 0, st>>>(a);                                \
+      if (wide) emm::q4_read_rows<T_, D_><<<grid, emm::kRowWarps * 32, 0, st>>>(a);             \
+      else emm::q4_read_units<T_, D_><<<grid, 256, 0, st>>>(a);                                 \
     }                                                                                           \
   } while (0)
   if (dtype == EMM_DTYPE_FP16) {

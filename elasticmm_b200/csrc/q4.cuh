@@ -21,6 +21,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "page_copy.cuh"
 
 namespace emm {
@@ -40,6 +42,7 @@ struct TokenSide {
   uint64_t head_stride;
   uint32_t num_blocks;
   uint32_t block_size;
+  int32_t block_shift;  // log2(block_size), or -1
 };
 
 struct Q4RowsArgs {
@@ -74,11 +77,40 @@ __device__ __forceinline__ __half from_f32<__half>(float x) {
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+__device__ __forceinline__ float2 unpack_half2(uint32_t x) {
+  return __half22float2(*reinterpret_cast<const __half2 *>(&x));
+}
+
+// Two 16-bit values of a word.
+template <typename T>
+__device__ __forceinline__ void unpack2(uint32_t w, float &lo, float &hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const float2 f = unpack_half2(w);
+    lo = f.x;
+    hi = f.y;
+  } else {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xffff0000u);
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    uint32_t y;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+    return y;
+  } else {
+    uint32_t y;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+    return y;
+  }
+}
+
 // Address of a token's row of head 0, or 0 when the slot is padding or outside the pool (reported).
 __device__ __forceinline__ uint64_t slot_address(const TokenSide &s, uint32_t layer, uint32_t plane, int64_t slot,
                                                  bool reporter, int *status) {
   if (slot < 0) return 0;
-  const uint64_t blk = (uint64_t)slot / s.block_size;
+  const uint64_t blk = s.block_shift >= 0 ? (uint64_t)slot >> s.block_shift : (uint64_t)slot / s.block_size;
   if (blk >= s.num_blocks) {
     if (reporter) report(status, kStatusIdRange, slot);
     return 0;
@@ -87,14 +119,196 @@ __device__ __forceinline__ uint64_t slot_address(const TokenSide &s, uint32_t la
   return s.layers[layer] + plane * s.plane_stride + blk * s.block_stride + tok * s.token_stride;
 }
 
-struct __align__(8) Quad {
-  uint16_t v[4];
-};
+// ---- one thread per group of 32 channels (64 bytes), where keys and values lie on 32-byte boundaries
+//
+// Append, 32 channels per thread: 64 bytes in, 20 out. At HBM's rate an SM has about 470 issue slots per warp for that, so
+// the bound is how few instructions a channel takes (11 here):
+//   * smallest and largest value on packed 16-bit pairs;
+//   * the quotient (x - o) / s as one fma with 1/s; rounding by adding and taking off 1.5 * 2^23. Where that can differ from
+//     the rounded division (a quotient within the fma's error of a half), or a code would leave 0..15, the thread
+//     repeats its group with divisions, so the bytes are those of the definition;
+//   * four codes make a unit by fma, exactly.
+// Rows are put together in shared memory and leave in 16-byte pieces.
+constexpr int kRowWarps = 8;
 
-// One thread per unit of four channels; the eight threads of a group find its smallest and largest value by shuffles.
-// grid.x * 256 threads cover T * H * D/4 units, grid.y the layers and planes. kWide: 8-byte loads.
-template <typename T, int D, bool kWide>
-__global__ void __launch_bounds__(256) q4_append(const __grid_constant__ Q4RowsArgs a) {
+template <typename T>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  if constexpr (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  if constexpr (std::is_same<T, __half>::value) asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  else asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ void load32(uint32_t (&w)[16], int i, uint64_t src) {
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]), "=r"(w[i + 6]), "=r"(w[i + 7])
+               : "l"(src));
+}
+__device__ __forceinline__ void store32(uint64_t dst, const uint32_t (&w)[16], int i) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]),
+               "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+               : "memory");
+}
+
+// The group by its definition: 16 bits of codes per unit.
+template <typename T>
+__device__ __noinline__ void encode_exact(const uint32_t (&w)[16], float s, float o, uint32_t (&unit)[8]) {
+  for (int u = 0; u < 8; ++u) {
+    float x[4];
+    unpack2<T>(w[2 * u], x[0], x[1]);
+    unpack2<T>(w[2 * u + 1], x[2], x[3]);
+    uint32_t code = 0;
+    for (int i = 0; i < 4; ++i) {
+      const float v = fminf(fmaxf(x[i], -65504.f), 65504.f);
+      const int c = s == 0.f ? 8 : 8 + __float2int_rn(__fdiv_rn(__fsub_rn(v, o), s));
+      code |= (uint32_t)(c < 0 ? 0 : (c > 15 ? 15 : c)) << (4 * i);
+    }
+    unit[u] = code;
+  }
+}
+
+// grid.x * kRowWarps warps cover the T * H rows, 32 / (D/32) of them each; grid.y the layers and planes.
+template <typename T, int D>
+__global__ void __launch_bounds__(kRowWarps * 32) q4_append_rows(const __grid_constant__ Q4RowsArgs a) {
+  constexpr int G = q4_groups(D), R = q4_row_bytes(D), kRows = 32 / G, kPieces = kRows * R / 16;
+  __shared__ __align__(16) uint8_t stage[kRowWarps][kRows * R];
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane % G;
+  const uint64_t rows = (uint64_t)a.num_tokens * a.heads, row = ((uint64_t)blockIdx.x * kRowWarps + warp) * kRows + lane / G;
+  const uint32_t lrel = blockIdx.y >> 1, p = blockIdx.y & 1;
+  const bool mine = row < rows;
+  const uint32_t t = mine ? (uint32_t)row / a.heads : 0u, h = mine ? (uint32_t)row - t * a.heads : 0u;
+  const uint64_t src = (p ? a.value + lrel * a.value_layer_stride + t * a.value_token_stride
+                          : a.key + lrel * a.key_layer_stride + t * a.key_token_stride) +
+                       ((uint64_t)h * D + 32 * r) * 2;
+  uint32_t w[16];
+  load32(w, 0, src);
+  load32(w, 8, src + 32);
+  const int64_t slot = mine ? a.slots[t] : -1;
+
+  uint32_t big = w[0], small = w[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) {
+    big = max2<T>(big, w[i]);
+    small = min2<T>(small, w[i]);
+  }
+  float hi, hi2, lo, lo2;
+  unpack2<T>(big, hi, hi2);
+  unpack2<T>(small, lo, lo2);
+  const bool nan = hi != hi || hi2 != hi2;
+  hi = fmaxf(hi, hi2);
+  lo = fminf(lo, lo2);
+  bool exact = hi > 65504.f || lo < -65504.f;  // infinities too
+  hi = fminf(fmaxf(hi, -65504.f), 65504.f);
+  lo = fminf(fmaxf(lo, -65504.f), 65504.f);
+  __half s = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
+  const float sf = __half2float(s);
+  __half o = __float2half_rn(__fadd_rn(lo, __fmul_rn(8.f, sf)));
+  const float of = __half2float(o);
+
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(sf));
+  const float at = -of * inv;
+  // |error of a quotient| < (|o/s| + 16) 2^-21: of x/s - o/s with 1/s off by 2^-23, and of the definition's own roundings.
+  const float most = 0.5f - (fabsf(at) + 16.f) * 0x1p-21f;
+  exact = exact || !(fmaf(lo, inv, at) > -8.25f && fmaf(hi, inv, at) < 7.25f);  // also for s = 0 and NaN
+  uint32_t unit[8];
+  float off = 0.f;
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    float x[4];
+    unpack2<T>(w[2 * u], x[0], x[1]);
+    unpack2<T>(w[2 * u + 1], x[2], x[3]);
+    float k[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float q = fmaf(x[i], inv, at);
+      k[i] = (q + 12582912.f) - 12582912.f;
+      off = fmaxf(off, fabsf(q - k[i]));
+    }
+    // sum (k + 8) 16^i, an integer below 2^16, in the low bits of 2^23 + it
+    unit[u] = __float_as_uint(fmaf(fmaf(fmaf(k[3], 16.f, k[2]), 16.f, k[1]), 16.f, k[0]) + (8388608.f + 34952.f));
+  }
+  exact = exact || !(off < most);
+  if (exact && !nan) encode_exact<T>(w, sf, of, unit);
+  if (nan) {
+    s = __ushort_as_half((unsigned short)0);
+    o = __ushort_as_half((unsigned short)0x7fff);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) unit[u] = 0x8888u;
+  }
+  uint8_t *mem = stage[warp] + lane / G * R;
+#pragma unroll
+  for (int u = 0; u < 8; ++u) *reinterpret_cast<uint16_t *>(mem + 2 * (u * G + r)) = (uint16_t)unit[u];
+  *reinterpret_cast<__half *>(mem + D / 2 + 2 * r) = s;
+  *reinterpret_cast<__half *>(mem + D / 2 + 2 * G + 2 * r) = o;
+  if (D == 64 && r == 0) *reinterpret_cast<uint2 *>(mem + 40) = make_uint2(0, 0);  // the row's padding
+  uint64_t dst = slot_address(a.pool, a.layer_begin + lrel, p, slot, r == 0 && h == 0, a.status);
+  if (dst) dst += (uint64_t)h * a.pool.head_stride;
+  __syncwarp();
+#pragma unroll
+  for (int c0 = 0; c0 < kPieces; c0 += 32) {
+    const uint32_t c = c0 + lane, from = min(c / (R / 16), (uint32_t)kRows - 1);
+    const uint64_t to = __shfl_sync(0xffffffffu, dst, from * G);
+    if (to && c < kPieces)
+      *reinterpret_cast<uint4 *>(to + c % (R / 16) * 16) = *reinterpret_cast<const uint4 *>(stage[warp] + c * 16);
+  }
+}
+
+// The inverse: o + s * (c - 8), rounded once to T. A padding or reported slot gives a row of zeros.
+template <typename T, int D>
+__global__ void __launch_bounds__(kRowWarps * 32) q4_read_rows(const __grid_constant__ Q4RowsArgs a) {
+  constexpr int G = q4_groups(D), R = q4_row_bytes(D), kRows = 32 / G, kPieces = kRows * R / 16;
+  __shared__ __align__(16) uint8_t stage[kRowWarps][kRows * R];
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane % G;
+  const uint64_t rows = (uint64_t)a.num_tokens * a.heads, row = ((uint64_t)blockIdx.x * kRowWarps + warp) * kRows + lane / G;
+  const uint32_t lrel = blockIdx.y >> 1, p = blockIdx.y & 1;
+  const bool mine = row < rows;
+  const uint32_t t = mine ? (uint32_t)row / a.heads : 0u, h = mine ? (uint32_t)row - t * a.heads : 0u;
+  uint64_t src = slot_address(a.pool, a.layer_begin + lrel, p, mine ? a.slots[t] : -1, r == 0 && h == 0, a.status);
+  if (src) src += (uint64_t)h * a.pool.head_stride;
+#pragma unroll
+  for (int c0 = 0; c0 < kPieces; c0 += 32) {
+    const uint32_t c = c0 + lane, from = min(c / (R / 16), (uint32_t)kRows - 1);
+    const uint64_t at = __shfl_sync(0xffffffffu, src, from * G);
+    if (c < kPieces) {
+      uint4 v = make_uint4(0, 0, 0, 0);  // codes, scale and offset 0 stand for 0
+      if (at) v = *reinterpret_cast<const uint4 *>(at + c % (R / 16) * 16);
+      *reinterpret_cast<uint4 *>(stage[warp] + c * 16) = v;
+    }
+  }
+  __syncwarp();
+  const uint8_t *mem = stage[warp] + lane / G * R;
+  const float s = __half2float(*reinterpret_cast<const __half *>(mem + D / 2 + 2 * r));
+  const float o = __half2float(*reinterpret_cast<const __half *>(mem + D / 2 + 2 * G + 2 * r));
+  uint32_t w[16];
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const uint32_t unit = *reinterpret_cast<const uint16_t *>(mem + 2 * (u * G + r));
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)  // 2^23 + c less 2^23 + 8: exact
+      v[i] = fmaf(s, __uint_as_float(0x4b000000u | (unit >> (4 * i) & 15u)) - 8388616.f, o);
+    w[2 * u] = pack2<T>(v[0], v[1]);
+    w[2 * u + 1] = pack2<T>(v[2], v[3]);
+  }
+  if (!mine) return;
+  const uint64_t dst = (p ? a.value + lrel * a.value_layer_stride + t * a.value_token_stride
+                          : a.key + lrel * a.key_layer_stride + t * a.key_token_stride) +
+                       ((uint64_t)h * D + 32 * r) * 2;
+  store32(dst, w, 0);
+  store32(dst + 32, w, 8);
+}
+
+// ---- keys and values on other boundaries: one thread per unit of four channels, element by element; the eight threads
+// of a group find its smallest and largest value by shuffles. grid.x * 256 threads cover T * H * D/4 units.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) q4_append_units(const __grid_constant__ Q4RowsArgs a) {
   constexpr uint32_t kUnits = D / 4, G = q4_groups(D);
   const uint64_t idx = (uint64_t)blockIdx.x * 256 + threadIdx.x;
   const uint32_t unit = (uint32_t)(idx % kUnits);
@@ -109,15 +323,8 @@ __global__ void __launch_bounds__(256) q4_append(const __grid_constant__ Q4RowsA
     const uint64_t src = (p ? a.value + lrel * a.value_layer_stride + t * a.value_token_stride
                             : a.key + lrel * a.key_layer_stride + t * a.key_token_stride) +
                          ((uint64_t)h * D + unit * 4) * 2;
-    T e[4];
-    if (kWide) {
-      *reinterpret_cast<Quad *>(e) = *reinterpret_cast<const Quad *>(src);
-    } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) e[i] = reinterpret_cast<const T *>(src)[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = to_f32<T>(e[i]);
+    for (int i = 0; i < 4; ++i) x[i] = to_f32<T>(reinterpret_cast<const T *>(src)[i]);
     row = slot_address(a.pool, a.layer_begin + lrel, p, a.slots[t], unit == 0 && h == 0, a.status);
   }
   bool nan = false;
@@ -162,9 +369,8 @@ __global__ void __launch_bounds__(256) q4_append(const __grid_constant__ Q4RowsA
   if (D == 64 && u == 1 && r == 0) *reinterpret_cast<uint2 *>(dst + 40) = make_uint2(0, 0);  // the row's padding
 }
 
-// The inverse: o + s * (c - 8), rounded once to T. A padding or reported slot gives a row of zeros.
-template <typename T, int D, bool kWide>
-__global__ void __launch_bounds__(256) q4_read(const __grid_constant__ Q4RowsArgs a) {
+template <typename T, int D>
+__global__ void __launch_bounds__(256) q4_read_units(const __grid_constant__ Q4RowsArgs a) {
   constexpr uint32_t kUnits = D / 4, G = q4_groups(D);
   const uint64_t idx = (uint64_t)blockIdx.x * 256 + threadIdx.x;
   const uint32_t unit = (uint32_t)(idx % kUnits);
@@ -173,28 +379,20 @@ __global__ void __launch_bounds__(256) q4_read(const __grid_constant__ Q4RowsArg
   const uint32_t lrel = blockIdx.y >> 1, p = blockIdx.y & 1;
   if (t >= a.num_tokens) return;
   const uint64_t row = slot_address(a.pool, a.layer_begin + lrel, p, a.slots[t], unit == 0 && h == 0, a.status);
-  T e[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) e[i] = from_f32<T>(0.f);
+  T *dst = reinterpret_cast<T *>((p ? a.value + lrel * a.value_layer_stride + t * a.value_token_stride
+                                    : a.key + lrel * a.key_layer_stride + t * a.key_token_stride) +
+                                 ((uint64_t)h * D + unit * 4) * 2);
+  float s = 0.f, o = 0.f;
+  uint32_t code = 0;
   if (row) {
     const uint32_t r = unit / 8, u = unit % 8;
     const uint8_t *src = reinterpret_cast<const uint8_t *>(row + (uint64_t)h * a.pool.head_stride);
-    const uint32_t code = *reinterpret_cast<const uint16_t *>(src + 2 * (u * G + r));
-    const float s = __half2float(*reinterpret_cast<const __half *>(src + D / 2 + 2 * r));
-    const float o = __half2float(*reinterpret_cast<const __half *>(src + D / 2 + 2 * G + 2 * r));
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      e[i] = from_f32<T>(__fadd_rn(o, __fmul_rn(s, (float)(int)((code >> (4 * i)) & 15u) - 8.f)));
+    code = *reinterpret_cast<const uint16_t *>(src + 2 * (u * G + r));
+    s = __half2float(*reinterpret_cast<const __half *>(src + D / 2 + 2 * r));
+    o = __half2float(*reinterpret_cast<const __half *>(src + D / 2 + 2 * G + 2 * r));
   }
-  const uint64_t dst = (p ? a.value + lrel * a.value_layer_stride + t * a.value_token_stride
-                          : a.key + lrel * a.key_layer_stride + t * a.key_token_stride) +
-                       ((uint64_t)h * D + unit * 4) * 2;
-  if (kWide) {
-    *reinterpret_cast<Quad *>(dst) = *reinterpret_cast<const Quad *>(e);
-  } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) reinterpret_cast<T *>(dst)[i] = e[i];
-  }
+  for (int i = 0; i < 4; ++i) dst[i] = from_f32<T>(__fadd_rn(o, __fmul_rn(s, (float)(int)((code >> (4 * i)) & 15u) - 8.f)));
 }
 
 }  // namespace emm

@@ -174,6 +174,28 @@ def test_append_extreme_groups(ctx):
     assert_clean(ctx)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_append_quotients_near_a_half_and_out_of_range(ctx, D, dtype):
+    """Groups whose quotients fall on or next to halves, groups far from zero (the offset's rounding shifts the codes out
+    of their range), tiny and subnormal groups, and many random ones: every byte as the definition has it."""
+    H, T = 2, 600
+    g = torch.Generator().manual_seed(D)
+    x = torch.randn(T, H, D, generator=g)
+    x[100:200] = torch.randint(0, 31, (100, H, D), generator=g).float() / 2  # steps of a half
+    x[200:300] = x[200:300] * 0.01 + torch.randn(100, H, 1, generator=g) * 30
+    x[300:350] = x[300:350] * 2.0 ** -22
+    x[350:400] = x[350:400] * 1e4
+    x[400:450, :, ::2] = 1000.0
+    x[450:500] = torch.randint(-8, 8, (50, H, D), generator=g).float() + 0.5 + 2.0 ** -7 * torch.randint(-1, 2, (50, H, D), generator=g)
+    key, value = x.to(dtype), (x * 0.37).to(dtype)
+    pool = KVPoolQ4(new_layers(1, -(-T // 16), 16, H, D, False), D, ctx)
+    pool.append(0, key.cuda(), value.cuda(), torch.arange(T, device="cuda"))
+    got = pool.layers[0].cpu().numpy().reshape(2, -1, H, KVPoolQ4.row_bytes(D))[:, :T]
+    assert (got[0] == rows_of(key)).all() and (got[1] == rows_of(value)).all()
+    assert_clean(ctx)
+
+
 def test_append_strided_rows_and_packed_blocks(ctx):
     """Slices of a fused projection at an odd offset, and the packed blocks of a 16-bit pool."""
     D, H, T, L, BS = 64, 3, 11, 2, 4
