@@ -122,12 +122,16 @@ __device__ __forceinline__ uint64_t slot_address(const TokenSide &s, uint32_t la
 // ---- one thread per group of 32 channels (64 bytes), where keys and values lie on 32-byte boundaries
 //
 // Append, 32 channels per thread: 64 bytes in, 20 out. At HBM's rate an SM has about 470 issue slots per warp for that, so
-// the bound is how few instructions a channel takes (11 here):
+// the bound is how few instructions a channel takes (7 here):
 //   * smallest and largest value on packed 16-bit pairs;
-//   * the quotient (x - o) / s as one fma with 1/s; rounding by adding and taking off 1.5 * 2^23. Where that can differ from
-//     the rounded division (a quotient within the fma's error of a half), or a code would leave 0..15, the thread
-//     repeats its group with divisions, so the bytes are those of the definition;
-//   * four codes make a unit by fma, exactly.
+//   * the quotient d / s, d = x - o, as d times an approximate 1/s and one step of correction with the fma's remainder:
+//     that is within 2^-45 of d / s before its rounding. It rounds to the same integer as the division does: a half-integer
+//     h times s is exact (5 and 11 bits), so d / s is h itself, which the corrected quotient then is too, or d is at least
+//     one unit in its last place away from h s, which is over half a unit of h (by 2^-11 of it or more). Every 50th
+//     group of bf16 values has such an exact half, so a test with divisions behind it would run in half of all warps;
+//   * rounding by adding 1.5 * 2^23 + 8, which leaves the code in the low bits; four make a unit by integer fma;
+//   * a group with a code outside 0..15 before the clamp (an offset much larger than its range), with s = 0, infinities or
+//     NaN goes through the definition step by step.
 // Rows are put together in shared memory and leave in 16-byte pieces.
 constexpr int kRowWarps = 8;
 
@@ -156,20 +160,19 @@ __device__ __forceinline__ void store32(uint64_t dst, const uint32_t (&w)[16], i
                : "memory");
 }
 
-// The group by its definition: 16 bits of codes per unit.
+// The group's codes by the definition, from its channels in memory; `step` is the distance of its units in the row.
 template <typename T>
-__device__ __noinline__ void encode_exact(const uint32_t (&w)[16], float s, float o, uint32_t (&unit)[8]) {
+__device__ __noinline__ void encode_exact(uint64_t src, float s, float o, uint8_t *row, int step) {
+#pragma unroll 1
   for (int u = 0; u < 8; ++u) {
-    float x[4];
-    unpack2<T>(w[2 * u], x[0], x[1]);
-    unpack2<T>(w[2 * u + 1], x[2], x[3]);
     uint32_t code = 0;
+#pragma unroll 1
     for (int i = 0; i < 4; ++i) {
-      const float v = fminf(fmaxf(x[i], -65504.f), 65504.f);
-      const int c = s == 0.f ? 8 : 8 + __float2int_rn(__fdiv_rn(__fsub_rn(v, o), s));
+      const float x = fminf(fmaxf(to_f32<T>(reinterpret_cast<const T *>(src)[4 * u + i]), -65504.f), 65504.f);
+      const int c = s == 0.f ? 8 : 8 + __float2int_rn(__fdiv_rn(__fsub_rn(x, o), s));
       code |= (uint32_t)(c < 0 ? 0 : (c > 15 ? 15 : c)) << (4 * i);
     }
-    unit[u] = code;
+    *reinterpret_cast<uint16_t *>(row + u * step) = (uint16_t)code;
   }
 }
 
@@ -213,29 +216,21 @@ __global__ void __launch_bounds__(kRowWarps * 32) q4_append_rows(const __grid_co
 
   float inv;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(sf));
-  const float at = -of * inv;
-  // |error of a quotient| < (|o/s| + 16) 2^-21: of x/s - o/s with 1/s off by 2^-23, and of the definition's own roundings.
-  const float most = 0.5f - (fabsf(at) + 16.f) * 0x1p-21f;
-  exact = exact || !(fmaf(lo, inv, at) > -8.25f && fmaf(hi, inv, at) < 7.25f);  // also for s = 0 and NaN
+  exact = exact || !((lo - of) * inv > -8.25f && (hi - of) * inv < 7.25f);  // also for s = 0 and NaN
   uint32_t unit[8];
-  float off = 0.f;
 #pragma unroll
   for (int u = 0; u < 8; ++u) {
     float x[4];
     unpack2<T>(w[2 * u], x[0], x[1]);
     unpack2<T>(w[2 * u + 1], x[2], x[3]);
-    float k[4];
+    uint32_t k[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float q = fmaf(x[i], inv, at);
-      k[i] = (q + 12582912.f) - 12582912.f;
-      off = fmaxf(off, fabsf(q - k[i]));
+      const float d = __fsub_rn(x[i], of), q = __fmul_rn(d, inv);
+      k[i] = __float_as_uint(__fadd_rn(__fmaf_rn(__fmaf_rn(-q, sf, d), inv, q), 12582920.f));
     }
-    // sum (k + 8) 16^i, an integer below 2^16, in the low bits of 2^23 + it
-    unit[u] = __float_as_uint(fmaf(fmaf(fmaf(k[3], 16.f, k[2]), 16.f, k[1]), 16.f, k[0]) + (8388608.f + 34952.f));
+    unit[u] = ((k[3] * 16u + k[2]) * 16u + k[1]) * 16u + k[0];  // its low 16 bits: the constant's are zero but for the 8
   }
-  exact = exact || !(off < most);
-  if (exact && !nan) encode_exact<T>(w, sf, of, unit);
   if (nan) {
     s = __ushort_as_half((unsigned short)0);
     o = __ushort_as_half((unsigned short)0x7fff);
@@ -245,6 +240,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) q4_append_rows(const __grid_co
   uint8_t *mem = stage[warp] + lane / G * R;
 #pragma unroll
   for (int u = 0; u < 8; ++u) *reinterpret_cast<uint16_t *>(mem + 2 * (u * G + r)) = (uint16_t)unit[u];
+  if (exact && !nan) encode_exact<T>(src, sf, of, mem + 2 * r, 2 * G);
   *reinterpret_cast<__half *>(mem + D / 2 + 2 * r) = s;
   *reinterpret_cast<__half *>(mem + D / 2 + 2 * G + 2 * r) = o;
   if (D == 64 && r == 0) *reinterpret_cast<uint2 *>(mem + 40) = make_uint2(0, 0);  // the row's padding
