@@ -29,6 +29,13 @@ int check_dtype(int32_t dtype, const char *what) {
   return EMM_OK;
 }
 
+// log2 of a power of two, else -1.
+int32_t shift_of(int32_t v) {
+  for (int k = 0; k < 31; ++k)
+    if (v == 1 << k) return k;
+  return -1;
+}
+
 emm::TokenSide token_side(const emm_pool *p) {
   emm::TokenSide s;
   s.layers = p->d_layers;
@@ -38,9 +45,7 @@ emm::TokenSide token_side(const emm_pool *p) {
   s.head_stride = (uint64_t)p->desc.head_stride;
   s.num_blocks = (uint32_t)p->desc.num_blocks;
   s.block_size = (uint32_t)p->desc.block_size;
-  s.block_shift = -1;
-  for (int k = 0; k < 31; ++k)
-    if (p->desc.block_size == 1 << k) s.block_shift = k;
+  s.block_shift = shift_of(p->desc.block_size);
   return s;
 }
 
@@ -153,10 +158,9 @@ int attend_shape(const emm_pool *pool, int32_t D, int32_t B, int32_t group, int3
   while (s.subsets > 1 && units() < sms) s.subsets /= 2;
   s.tokens = 16 * s.subsets;
   s.warps = s.heads_cta * s.ntiles * s.subsets;
-  s.block_shift = -1;
-  for (int k = 4; k < 31; ++k)
-    if (d.block_size == 1 << k && d.token_stride < 1 << 27 && d.block_stride <= 0xffffffffll)  // its offsets take 32 bits
-      s.block_shift = k;
+  // A tile's offsets within a block take 32 bits.
+  s.block_shift = d.token_stride < 1 << 27 && d.block_stride <= 0xffffffffll ? shift_of(d.block_size) : -1;
+  if (s.block_shift < 4) s.block_shift = -1;
   s.stages = (uint32_t)emm::attend_stages(D);
   const int merge = (int)((s.subsets - 1) * s.heads_cta * s.ntiles * 8 * (uint32_t)(D + 2) * 4);
   *smem_out = (int)(s.warps * s.stages * (32 * R + 16)) + merge;
@@ -393,6 +397,7 @@ int emm_select_tokens(emm_pool *scores, const int32_t *d_block_tables, int64_t t
   a.block_stride = (uint64_t)d.block_stride;
   a.num_blocks = (uint32_t)d.num_blocks;
   a.block_size = (uint32_t)d.head_size;
+  a.block_shift = shift_of(d.head_size);
   a.tables = d_block_tables;
   a.table_stride = (uint64_t)table_stride;
   a.table_width = (uint32_t)table_width;
@@ -408,7 +413,12 @@ int emm_select_tokens(emm_pool *scores, const int32_t *d_block_tables, int64_t t
   DeviceGuard guard(scores->ctx->device);
   if (!guard.ok()) return fail(EMM_ERR_CUDA, "cannot select device %d", scores->ctx->device);
   const dim3 grid((unsigned)num_seqs * (unsigned)d.block_size, (unsigned)d.num_layers);
-  emm::select_tokens<<<grid, emm::kSelectThreads, 0, (cudaStream_t)stream>>>(a);
+  // As few threads as have the longest sequence in registers.
+  const int64_t most = (int64_t)table_width * d.head_size;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (most <= 256 * emm::kSelectKeys) emm::select_tokens<256><<<grid, 256, 0, st>>>(a);
+  else if (most <= 512 * emm::kSelectKeys) emm::select_tokens<512><<<grid, 512, 0, st>>>(a);
+  else emm::select_tokens<1024><<<grid, 1024, 0, st>>>(a);
   EMM_CUDA(cudaGetLastError());
   scores->ctx->launches += 1;
   return EMM_OK;
@@ -431,6 +441,7 @@ int emm_keep_tokens(emm_pool *pool, const int32_t *d_index, int32_t index_heads,
     a.heads = (uint32_t)d.block_size;
     a.row_bytes = (uint32_t)d.elem_size;
     a.pool.block_size = (uint32_t)d.head_size;
+    a.pool.block_shift = shift_of(d.head_size);
     a.pool.token_stride = (uint64_t)d.elem_size;
     a.pool.head_stride = (uint64_t)d.token_stride;
   } else {
@@ -461,11 +472,21 @@ int emm_keep_tokens(emm_pool *pool, const int32_t *d_index, int32_t index_heads,
   if (!guard.ok()) return fail(EMM_ERR_CUDA, "cannot select device %d", pool->ctx->device);
   const dim3 grid((unsigned)num_seqs * a.heads * a.planes, (unsigned)d.num_layers);
   cudaStream_t st = (cudaStream_t)stream;
-  if (align >= 16) emm::keep_rows<uint4><<<grid, emm::kKeepThreads, 0, st>>>(a);
-  else if (align >= 8) emm::keep_rows<uint2><<<grid, emm::kKeepThreads, 0, st>>>(a);
-  else if (align >= 4) emm::keep_rows<uint32_t><<<grid, emm::kKeepThreads, 0, st>>>(a);
-  else if (align >= 2) emm::keep_rows<uint16_t><<<grid, emm::kKeepThreads, 0, st>>>(a);
-  else emm::keep_rows<uint8_t><<<grid, emm::kKeepThreads, 0, st>>>(a);
+  const uint32_t vec = std::min(align, 16u);
+  const bool plain = a.row_bytes / vec <= (uint32_t)emm::kKeepThreads && a.pool.block_shift >= 0 &&
+                     std::max(a.pool.block_stride, a.pool.token_stride) <= 0xffffffffull &&
+                     (uint64_t)keep < (1ull << 31) - 64 * emm::kKeepThreads;
+#define EMM_KEEP(V_)                                                                  \
+  do {                                                                                \
+    if (plain) emm::keep_rows<V_, true><<<grid, emm::kKeepThreads, 0, st>>>(a);       \
+    else emm::keep_rows<V_, false><<<grid, emm::kKeepThreads, 0, st>>>(a);            \
+  } while (0)
+  if (vec >= 16) EMM_KEEP(uint4);
+  else if (vec >= 8) EMM_KEEP(uint2);
+  else if (vec >= 4) EMM_KEEP(uint32_t);
+  else if (vec >= 2) EMM_KEEP(uint16_t);
+  else EMM_KEEP(uint8_t);
+#undef EMM_KEEP
   EMM_CUDA(cudaGetLastError());
   pool->ctx->launches += 1;
   return EMM_OK;
