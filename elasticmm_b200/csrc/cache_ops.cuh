@@ -29,6 +29,8 @@ int check_dtype(int32_t dtype, const char *what) {
   return EMM_OK;
 }
 
+constexpr int kSelectSharedMax = 200 * 1024;  // bytes of keys a CTA holds
+
 // log2 of a power of two, else -1.
 int32_t shift_of(int32_t v) {
   for (int k = 0; k < 31; ++k)
@@ -413,12 +415,20 @@ int emm_select_tokens(emm_pool *scores, const int32_t *d_block_tables, int64_t t
   DeviceGuard guard(scores->ctx->device);
   if (!guard.ok()) return fail(EMM_ERR_CUDA, "cannot select device %d", scores->ctx->device);
   const dim3 grid((unsigned)num_seqs * (unsigned)d.block_size, (unsigned)d.num_layers);
-  // As few threads as have the longest sequence in registers.
   const int64_t most = (int64_t)table_width * d.head_size;
   cudaStream_t st = (cudaStream_t)stream;
-  if (most <= 256 * emm::kSelectKeys) emm::select_tokens<256><<<grid, 256, 0, st>>>(a);
-  else if (most <= 512 * emm::kSelectKeys) emm::select_tokens<512><<<grid, 512, 0, st>>>(a);
-  else emm::select_tokens<1024><<<grid, 1024, 0, st>>>(a);
+  if (most * 4 <= kSelectSharedMax) {
+    if (most <= 4096) {
+      emm::select_tokens<256, true><<<grid, 256, (size_t)most * 4, st>>>(a);
+    } else if (most <= 11264) {  // 44 KB: fits the default limit
+      emm::select_tokens<512, true><<<grid, 512, (size_t)most * 4, st>>>(a);
+    } else {
+      EMM_CUDA(cudaFuncSetAttribute(emm::select_tokens<1024, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectSharedMax));
+      emm::select_tokens<1024, true><<<grid, 1024, (size_t)most * 4, st>>>(a);
+    }
+  } else {
+    emm::select_tokens<1024, false><<<grid, 1024, 0, st>>>(a);
+  }
   EMM_CUDA(cudaGetLastError());
   scores->ctx->launches += 1;
   return EMM_OK;
@@ -452,7 +462,7 @@ int emm_keep_tokens(emm_pool *pool, const int32_t *d_index, int32_t index_heads,
     return fail(EMM_ERR_LENGTH, "%s: index of %d heads, the pool has %u", what, index_heads, a.heads);
   if (num_seqs == 0) return EMM_OK;
   if (!d_index) return fail(EMM_ERR_BAD_ARG, "%s: null pointer", what);
-  if ((uint64_t)num_seqs * a.heads * pool->planes > 0x7fffffffull || d.num_layers > 65535 ||
+  if ((uint64_t)num_seqs * a.heads * pool->planes > 0x1fffffffull || d.num_layers > 65535 ||
       (int64_t)table_width * a.pool.block_size > 0x7fffffffll)
     return fail(EMM_ERR_TOO_LARGE, "%s: %d layers x %d sequences of %d blocks", what, d.num_layers, num_seqs, table_width);
   a.planes = (uint32_t)pool->planes;
@@ -470,7 +480,16 @@ int emm_keep_tokens(emm_pool *pool, const int32_t *d_index, int32_t index_heads,
   for (uint64_t v : strides) align = std::min(align, pow2_align(v));
   DeviceGuard guard(pool->ctx->device);
   if (!guard.ok()) return fail(EMM_ERR_CUDA, "cannot select device %d", pool->ctx->device);
-  const dim3 grid((unsigned)num_seqs * a.heads * a.planes, (unsigned)d.num_layers);
+  // Where an SM would have fewer than four CTAs, two or four share a row, down to 64 bytes each: a CTA's rows come one
+  // chunk after the other, so few CTAs cannot keep HBM busy.
+  a.splits = 1;
+  const uint64_t ctas = (uint64_t)num_seqs * a.heads * a.planes * (uint64_t)d.num_layers;
+  while (a.splits < 4 && ctas * a.splits < 4ull * pool->ctx->sm_count && a.row_bytes % 32 == 0 && a.row_bytes / 2 >= 64) {
+    a.splits *= 2;
+    a.row_bytes /= 2;
+    align = std::min(align, pow2_align(a.row_bytes));
+  }
+  const dim3 grid((unsigned)num_seqs * a.heads * a.planes * a.splits, (unsigned)d.num_layers);
   cudaStream_t st = (cudaStream_t)stream;
   const uint32_t vec = std::min(align, 16u);
   const bool plain = a.row_bytes / vec <= (uint32_t)emm::kKeepThreads && a.pool.block_shift >= 0 &&

@@ -36,19 +36,17 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// One CTA per (layer, sequence, head). Warp w of a tile of 16 * kThreads positions has positions w * 512 .. + 511, 16 keys
-// in each lane's registers; the want-th largest key is found by three radix passes of 11, 11 and 10 bits over
-// histograms in shared memory. A sequence of one tile reads its weights once; a longer one reads them again in every
-// pass, which L2 serves. What bounds it is latency (table, weight, three passes), so the host takes as few
-// threads as hold the longest sequence, and as many CTAs share an SM.
-constexpr int kSelectKeys = 16, kSelectBins = 2048;
-
-template <int kThreads>
-__global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : 1536 / kThreads) select_tokens(const __grid_constant__ SelectArgs a) {
-  constexpr int kWarps = kThreads / 32, kBins = kSelectBins / kThreads, kTile = kThreads * kSelectKeys;
-  __shared__ uint32_t hist[kSelectBins];
-  __shared__ uint32_t part[2][kWarps];
-  __shared__ uint32_t pick[2];
+// One CTA per (layer, sequence, head). The keys are read once into shared memory (kShared; a sequence that does not fit
+// there reads its weights again in every pass, which L2 serves). The want-th largest is found by at most four radix passes
+// of eight bits, fewer where a digit's bin is taken whole. What bounds it is latency: the table, the weights, the passes'
+// barriers. So a digit is found by one warp, bins are cleared a pass ahead, and the index leaves after one more barrier.
+template <int kThreads, bool kShared>
+__global__ void __launch_bounds__(kThreads) select_tokens(const __grid_constant__ SelectArgs a) {
+  constexpr int kWarps = kThreads / 32, kAhead = 8;
+  extern __shared__ uint32_t keys[];  // kShared: one per position
+  __shared__ uint32_t hist[2][256];
+  __shared__ uint32_t part[2][32];
+  __shared__ uint32_t pick[3];
   const uint32_t h = blockIdx.x % a.heads, b = blockIdx.x / a.heads, l = blockIdx.y;
   const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   int32_t len = a.lens[b];
@@ -67,117 +65,119 @@ __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : 1536 / kThrea
   const int32_t *table = a.tables + b * a.table_stride;
   const uint32_t first = a.sink, last = n - a.recent;  // candidates [first, last)
   uint32_t want = a.keep - a.sink - a.recent;           // of them
-  const bool none = want == 0;
 
-  uint32_t keys[kSelectKeys];
-  auto load = [&](uint32_t tile) {
-    int32_t id[kSelectKeys];
-#pragma unroll
-    for (int u = 0; u < kSelectKeys; ++u) {
-      const uint32_t t = tile + warp * (32 * kSelectKeys) + u * 32 + lane;
-      id[u] = -1;
-      if (t < n) id[u] = table[a.block_shift >= 0 ? t >> a.block_shift : t / a.block_size];
+  auto block_at = [&](uint32_t t) -> int32_t { return table[a.block_shift >= 0 ? t >> a.block_shift : t / a.block_size]; };
+  auto key_in = [&](uint32_t t, int32_t id) -> uint32_t {
+    if ((uint32_t)id >= a.num_blocks) {
+      report(a.status, kStatusIdRange, id);
+      return 0;
     }
-#pragma unroll
-    for (int u = 0; u < kSelectKeys; ++u) {
-      const uint32_t t = tile + warp * (32 * kSelectKeys) + u * 32 + lane;
-      keys[u] = 0;
-      if (t >= n) continue;
-      if ((uint32_t)id[u] >= a.num_blocks) {
-        report(a.status, kStatusIdRange, id[u]);
-        continue;
-      }
-      const uint32_t place = a.block_shift >= 0 ? t & ((1u << a.block_shift) - 1u) : t % a.block_size;
-      keys[u] = order_key(reinterpret_cast<const float *>(base + (uint64_t)(uint32_t)id[u] * a.block_stride)[place]);
-    }
+    const uint32_t place = a.block_shift >= 0 ? t & ((1u << a.block_shift) - 1u) : t % a.block_size;
+    return order_key(reinterpret_cast<const float *>(base + (uint64_t)(uint32_t)id * a.block_stride)[place]);
   };
-  const bool one_tile = n <= kTile;
-  load(0);
+  auto key_at = [&](uint32_t t) -> uint32_t {
+    if constexpr (kShared) return keys[t];
+    return key_in(t, block_at(t));
+  };
+  if (tid < 256) hist[0][tid] = 0;
+  if constexpr (kShared) {
+    for (uint32_t t0 = tid; t0 < n; t0 += kThreads * kAhead) {
+      int32_t id[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) id[u] = t0 + u * kThreads < n ? block_at(t0 + u * kThreads) : 0;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (t0 + u * kThreads < n) keys[t0 + u * kThreads] = key_in(t0 + u * kThreads, id[u]);
+    }
+  }
+  __syncthreads();
   uint32_t prefix = 0, mask = 0;  // the digits found, and where they stand
-  for (int pass = 0; pass < 3 && !none; ++pass) {
-    const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
-#pragma unroll
-    for (int i = 0; i < kBins; ++i) hist[i * kThreads + tid] = 0;
+  const bool none = want == 0;
+  for (int pass = 0; pass < 4 && !none; ++pass) {
+    const int shift = 24 - 8 * pass;
+    uint32_t *bins = hist[pass & 1];
+    if (tid < 256) hist[~pass & 1][tid] = 0;
+#pragma unroll 4
+    for (uint32_t t = first + tid; t < last; t += kThreads) {
+      const uint32_t k = key_at(t);
+      if ((k & mask) == prefix) atomicAdd(&bins[k >> shift & 255u], 1u);
+    }
     __syncthreads();
-    for (uint32_t tile = 0; tile < n; tile += kTile) {
-      if (!one_tile) load(tile);
+    if (warp == 0) {  // lane i has bins 255 - 8 i and the seven below: a scan from the largest digit down
+      uint32_t c[8], mine = 0;
 #pragma unroll
-      for (int u = 0; u < kSelectKeys; ++u) {
-        const uint32_t t = tile + warp * (32 * kSelectKeys) + u * 32 + lane;
-        if (t >= first && t < last && (keys[u] & mask) == prefix) atomicAdd(&hist[keys[u] >> shift & ((1u << bits) - 1u)], 1u);
+      for (int i = 0; i < 8; ++i) mine += c[i] = bins[255 - 8 * lane - i];
+      uint32_t upto = mine;
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) {
+        const uint32_t other = __shfl_up_sync(0xffffffffu, upto, m);
+        if (lane >= m) upto += other;
       }
-    }
-    __syncthreads();
-    // Thread t has bins 2047 - kBins t and the ones below it: a scan from the largest digit down.
-    uint32_t mine = 0;
+      uint32_t above = upto - mine;
+      if (above < want && want <= upto) {
+        int i = 0;
 #pragma unroll
-    for (int i = 0; i < kBins; ++i) mine += hist[kSelectBins - 1 - (tid * kBins + i)];
-    uint32_t upto = mine;
+        for (int k = 0; k < 7; ++k)
+          if (i == k && above + c[k] < want) {
+            above += c[k];
+            i = k + 1;
+          }
+        uint32_t in_bin = c[0];
 #pragma unroll
-    for (int m = 1; m < 32; m <<= 1) {
-      const uint32_t other = __shfl_up_sync(0xffffffffu, upto, m);
-      if (lane >= m) upto += other;
-    }
-    if (lane == 31) part[0][warp] = upto;
-    __syncthreads();
-    uint32_t above = upto - mine;
-    for (uint32_t w = 0; w < warp; ++w) above += part[0][w];
-    if (above < want && want <= above + mine) {
-      uint32_t d = kSelectBins - 1 - tid * kBins;
-      while (above + hist[d] < want) above += hist[d--];
-      pick[0] = d;
-      pick[1] = want - above;
+        for (int k = 1; k < 8; ++k)
+          if (i == k) in_bin = c[k];
+        pick[0] = 255 - 8 * lane - i;
+        pick[1] = want - above;
+        pick[2] = in_bin;
+      }
     }
     __syncthreads();
     prefix |= pick[0] << shift;
-    mask |= ((1u << bits) - 1u) << shift;
+    mask |= 255u << shift;
     want = pick[1];
+    if (pick[2] == want) break;  // the whole bin is taken
   }
-  // Taken: the ends, keys above the one found, and the `want` earliest equal to it.
-  uint32_t done = 0, ties = 0;  // in the tiles before
-  for (uint32_t tile = 0; tile < n; tile += kTile) {
-    if (!one_tile) load(tile);
-    uint32_t sure = 0, tie = 0;  // bit u: this lane's key u
-    uint32_t n_sure = 0, n_tie = 0;
-#pragma unroll
-    for (int u = 0; u < kSelectKeys; ++u) {
-      const uint32_t t = tile + warp * (32 * kSelectKeys) + u * 32 + lane;
-      const bool in = t < n, end = in && (t < first || t >= last), mid = in && !end && !none;
-      if (end || (mid && keys[u] > prefix)) sure |= 1u << u;
-      if (mid && keys[u] == prefix) tie |= 1u << u;
-      n_sure += __popc(__ballot_sync(0xffffffffu, sure >> u & 1));
-      n_tie += __popc(__ballot_sync(0xffffffffu, tie >> u & 1));
+  // Taken: the ends, keys above the one found (as far as its digits go), and the `want` earliest equal to it. Warp w has a
+  // run of positions, counts both kinds, and after a barrier knows where its part of the index begins.
+  const uint32_t run = (n + kWarps * 32 - 1) / (kWarps * 32) * 32, begin = min(n, warp * run), end = min(n, begin + run);
+  auto kinds = [&](uint32_t t, bool &sure, bool &tie) {
+    sure = tie = false;
+    if (t >= end) return;
+    if (t < first || t >= last) {
+      sure = true;
+    } else if (!none) {
+      const uint32_t k = key_at(t) & mask;
+      sure = k > prefix;
+      tie = k == prefix;
     }
-    __syncthreads();
-    if (lane == 0) {
-      part[0][warp] = n_sure;
-      part[1][warp] = n_tie;
-    }
-    __syncthreads();
-    uint32_t s_before = 0, t_before = ties, s_all = 0, t_all = 0;
-    for (uint32_t w = 0; w < kWarps; ++w) {
-      if (w < warp) {
-        s_before += part[0][w];
-        t_before += part[1][w];
-      }
-      s_all += part[0][w];
-      t_all += part[1][w];
-    }
-    // Of the ties before this warp, the first `want` are taken; done counts what earlier tiles took.
-    uint32_t at = done + s_before + min(t_before, want) - min(ties, want);
-#pragma unroll
-    for (int u = 0; u < kSelectKeys; ++u) {
-      const uint32_t below = (1u << lane) - 1u;
-      const uint32_t tb = __ballot_sync(0xffffffffu, tie >> u & 1);
-      const bool take = (sure >> u & 1) || ((tie >> u & 1) && t_before + __popc(tb & below) < want);
-      const uint32_t kb = __ballot_sync(0xffffffffu, take);
-      const uint32_t j = at + __popc(kb & below);
-      if (take && j < a.keep) out[j] = (int32_t)(tile + warp * (32 * kSelectKeys) + u * 32 + lane);
-      at += __popc(kb);
-      t_before += __popc(tb);
-    }
-    done += s_all + min(ties + t_all, want) - min(ties, want);
-    ties += t_all;
+  };
+  uint32_t n_sure = 0, n_tie = 0;
+  for (uint32_t t0 = begin; t0 < end; t0 += 32) {
+    bool sure, tie;
+    kinds(t0 + lane, sure, tie);
+    n_sure += __popc(__ballot_sync(0xffffffffu, sure));
+    n_tie += __popc(__ballot_sync(0xffffffffu, tie));
+  }
+  if (lane == 0) {
+    part[0][warp] = n_sure;
+    part[1][warp] = n_tie;
+  }
+  __syncthreads();
+  uint32_t s_before = lane < warp ? part[0][lane] : 0, t_before = lane < warp ? part[1][lane] : 0;
+  s_before = __reduce_add_sync(0xffffffffu, s_before);
+  t_before = __reduce_add_sync(0xffffffffu, t_before);
+  uint32_t at = s_before + min(t_before, want);
+  for (uint32_t t0 = begin; t0 < end; t0 += 32) {
+    const uint32_t below = (1u << lane) - 1u;
+    bool sure, tie;
+    kinds(t0 + lane, sure, tie);
+    const uint32_t tb = __ballot_sync(0xffffffffu, tie);
+    const bool take = sure || (tie && t_before + __popc(tb & below) < want);
+    const uint32_t kb = __ballot_sync(0xffffffffu, take);
+    const uint32_t j = at + __popc(kb & below);
+    if (take && j < a.keep) out[j] = (int32_t)(t0 + lane);
+    at += __popc(kb);
+    t_before += __popc(tb);
   }
 }
 
@@ -185,7 +185,8 @@ struct KeepArgs {
   TokenSide pool;
   uint32_t planes;
   uint32_t heads;
-  uint32_t row_bytes;
+  uint32_t splits;     // CTAs that share a row's bytes
+  uint32_t row_bytes;  // of one of them
   const int32_t *tables;
   uint64_t table_stride;
   uint32_t table_width;
@@ -196,7 +197,7 @@ struct KeepArgs {
   int *status;
 };
 
-// One CTA per (layer, sequence, head, plane); every kept row is read and written once, so HBM bounds it, and what counts is
+// One CTA per (layer, sequence, head, plane), several where those are few; every kept row is read and written once, so HBM bounds it, and what counts is
 // how many rows are in flight and how few instructions a row takes (300 for two vectors, with 64-bit positions and
 // divisions, held the kernel to 3.6 TB/s). A ring of chunks in shared memory is filled by asynchronous copies. A thread has
 // one vector of type V at a fixed place of a row and kKeepAhead rows of a chunk, and stores what it loaded itself.
@@ -210,7 +211,8 @@ template <typename V, bool kPlain>
 __global__ void __launch_bounds__(kKeepThreads) keep_rows(const __grid_constant__ KeepArgs a) {
   using Pos = typename std::conditional<kPlain, uint32_t, uint64_t>::type;
   __shared__ __align__(16) V ring[kKeepStages][kKeepAhead][kKeepThreads];
-  const uint32_t p = blockIdx.x % a.planes, bh = blockIdx.x / a.planes;
+  const uint32_t piece = blockIdx.x % a.splits, pbh = blockIdx.x / a.splits;
+  const uint32_t p = pbh % a.planes, bh = pbh / a.planes;
   const uint32_t h = bh % a.heads, b = bh / a.heads, l = blockIdx.y;
   const int32_t len = a.lens[b];
   if (len < 0 || (uint64_t)len > (uint64_t)a.table_width * a.pool.block_size) {
@@ -224,7 +226,7 @@ __global__ void __launch_bounds__(kKeepThreads) keep_rows(const __grid_constant_
   const uint32_t segments = kPlain ? 1u : (vecs + kKeepThreads - 1) / kKeepThreads, wide = min(vecs, (uint32_t)kKeepThreads);
   const uint32_t rows = kKeepThreads / wide;  // rows (or segments) side by side
   const uint32_t mine = threadIdx.x / wide, part = threadIdx.x % wide;
-  const uint64_t base = a.pool.layers[l] + p * a.pool.plane_stride + h * a.pool.head_stride + part * sizeof(V);
+  const uint64_t base = a.pool.layers[l] + p * a.pool.plane_stride + h * a.pool.head_stride + piece * a.row_bytes + part * sizeof(V);
   // Row segments in order; a thread that has none counts from behind the end.
   const Pos total = (Pos)a.keep * segments, step = (Pos)rows * kKeepAhead, own = mine < rows ? (Pos)mine : total;
   auto row_at = [&](uint32_t t) -> uint64_t {
