@@ -16,7 +16,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from .kv_pool import Context, KVPool, check_block_tables
+from .kv_pool import Context, KVPool, _stream_ptr, check_block_tables
 
 _DTYPES = {torch.float16: _lib.DTYPE_FP16, torch.bfloat16: _lib.DTYPE_BF16}
 _MAX_SIGNATURES = 64
@@ -51,7 +51,7 @@ class ScorePool(KVPool):
                 or not slot_mapping.is_contiguous()):
             raise ValueError("slot_mapping must be a contiguous 1-D int64 tensor on the pool's device")
         _lib.check(self.ctx._lib.emm_reset_scores(self._h, slot_mapping.data_ptr(), slot_mapping.numel(),
-                                                  torch.cuda.current_stream(self.ctx.device).cuda_stream))
+                                                  _stream_ptr(self.ctx.device)))
 
     def select_tokens(self, block_tables: torch.Tensor, seq_lens: torch.Tensor, keep: int, recent: int = 0,
                       sink: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -71,7 +71,7 @@ class ScorePool(KVPool):
         new_lens = torch.empty(B, dtype=torch.int32, device=self.device)
         rc = self.ctx._lib.emm_select_tokens(
             self._h, block_tables.data_ptr(), block_tables.stride(0), width, seq_lens.data_ptr(), B, keep, recent, sink,
-            index.data_ptr(), new_lens.data_ptr(), torch.cuda.current_stream(self.ctx.device).cuda_stream)
+            index.data_ptr(), new_lens.data_ptr(), _stream_ptr(self.ctx.device))
         if rc:
             _lib.check(rc)
         return index, new_lens
@@ -161,7 +161,7 @@ class KVPoolQ4(KVPool):
         """Quantises one layer's new rows [T, H, D] (fp16 or bf16) into their slots; slot < 0 is skipped."""
         T, dt, (_, kts, _, vts) = self._rows_sig(key, value, slot_mapping, 0)
         rc = self._emm_q4_append(self._h, self.head_dim, dt, layer, 1, key.data_ptr(), value.data_ptr(), 0, kts, 0, vts,
-                                 slot_mapping.data_ptr(), T, torch.cuda.current_stream(self.ctx.device).cuda_stream)
+                                 slot_mapping.data_ptr(), T, _stream_ptr(self.ctx.device))
         if rc:
             _lib.check(rc)
 
@@ -170,7 +170,7 @@ class KVPoolQ4(KVPool):
         T, dt, (kls, kts, vls, vts) = self._rows_sig(key, value, slot_mapping, 1)
         rc = self._emm_q4_append(self._h, self.head_dim, dt, 0, self.num_layers, key.data_ptr(), value.data_ptr(), kls, kts,
                                  vls, vts, slot_mapping.data_ptr(), T,
-                                 torch.cuda.current_stream(self.ctx.device).cuda_stream)
+                                 _stream_ptr(self.ctx.device))
         if rc:
             _lib.check(rc)
 
@@ -191,7 +191,7 @@ class KVPoolQ4(KVPool):
         def append(layer: int, stream: Optional[int] = None) -> None:
             if not 0 <= layer < L:
                 raise _lib.EmmError(_lib.ERR_BAD_ARG, f"layer {layer} outside [0, {L})")
-            rc = raw(layer, torch.cuda.current_stream(device).cuda_stream if stream is None else stream)
+            rc = raw(layer, _stream_ptr(device) if stream is None else stream)
             if rc:
                 _lib.check(rc)
 
@@ -211,15 +211,15 @@ class KVPoolQ4(KVPool):
         lc = self.num_layers - layer_begin if layer_count is None else layer_count
         if layer_begin < 0 or lc < 0 or layer_begin + lc > self.num_layers:
             raise ValueError(f"layer range [{layer_begin}, {layer_begin + lc}) outside [0, {self.num_layers})")
-        T, H, D = slot_mapping.numel(), self.num_kv_heads, self.head_dim
-        both = torch.empty((2, lc, T, H, D), dtype=dtype, device=self.device)
+        T, H, D = slot_mapping.shape[0], self.num_kv_heads, self.head_dim
+        both = torch.empty((2, lc, T, H, D), dtype=dtype, device=self.ctx.device)
         ts = H * D * 2
         ls, base = T * ts, both.data_ptr()
         rc = self._emm_q4_read(self._h, D, dt, layer_begin, lc, base, base + lc * ls, ls, ts, ls, ts,
-                               slot_mapping.data_ptr(), T, torch.cuda.current_stream(self.ctx.device).cuda_stream)
+                               slot_mapping.data_ptr(), T, _stream_ptr(self.ctx.device))
         if rc:
             _lib.check(rc)
-        return both[0], both[1]
+        return both.unbind(0)
 
     # -- attention --------------------------------------------------------------
     def _check_attend(self, query, block_tables, seq_lens, out, scores, max_len) -> tuple:
@@ -285,7 +285,7 @@ class KVPoolQ4(KVPool):
             self._h, self.head_dim, dt, layer, query.data_ptr(), qs, out.data_ptr(), os_, block_tables.data_ptr(),
             block_tables.stride(0), width, seq_lens.data_ptr(), B, heads, limit, default_scale if scale is None else scale,
             None if scores is None else scores._h, None if ws is None else ws.data_ptr(), nbytes,
-            torch.cuda.current_stream(device).cuda_stream)
+            _stream_ptr(device))
         if rc:
             _lib.check(rc)
         return out
