@@ -562,147 +562,152 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
     };
 
     int left = active ? (int)n - (int)(unit0 * sh.tokens + t_sub) : 0;  // tokens from this warp's next tile on
+    // One tile. kWhole: all 16 tokens count (mask is not read).
+    auto tile = [&](auto whole_tag, const uint32_t base, const uint32_t mask) {
+      constexpr bool kWhole = decltype(whole_tag)::value;
+        // ---- logits of 16 tokens
+      float l[4];
+      {
+        uint32_t w0[KW], w1[KW], s0[SW], s1[SW], m[4];
+        const uint32_t ka = base + k_at, kc = ka + q4 * (D / 8);
+        lds_matrices<false, D / 2>(m, base + km_at);
+        lds_words<KW, 0>(w0, kc);
+        lds_words<KW, 8 * R>(w1, kc);
+        lds_words<SW, D / 2>(s0, ka);
+        lds_words<SW, 8 * R + D / 2>(s1, ka);
+        float d0[4] = {0.f, 0.f, 0.f, 0.f};
+        mma_k16(d0, m[0], m[1], m[2], m[3], qo[0], qo[1], d0);
+        if constexpr (G == 8) mma_k16(d0, m[0], m[1], m[2], m[3], qo[2], qo[3], d0);
+        float x[4];
+#pragma unroll
+        for (int r = 0; r < G; ++r) {
+          const uint32_t sel = r % 2 ? kHiHalves : kLoHalves, up = r % 2 ? kHiUpper : kLoUpper;
+          const uint32_t u0 = __byte_perm(w0[r / 2], w0[KW / 2 + r / 2], sel), u1 = __byte_perm(w1[r / 2], w1[KW / 2 + r / 2], sel);
+          const uint32_t y0 = __byte_perm(w0[r / 2], w0[KW / 2 + r / 2], up), y1 = __byte_perm(w1[r / 2], w1[KW / 2 + r / 2], up);
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_k16(d, u0 & kNib0, u1 & kNib0, u0 & kNib1, u1 & kNib1, qf[r][0], qf[r][1], d);
+          mma_k16(d, y0 & kNib0, y1 & kNib0, y0 & kNib1, y1 & kNib1, qf[r][2], qf[r][3], d);
+          const float2 f0 = unpack_half2(s0[r / 2]), f1 = unpack_half2(s1[r / 2]);
+          const float e0 = r % 2 ? f0.y : f0.x, e1 = r % 2 ? f1.y : f1.x;
+          x[0] = r ? fmaf(e0, d[0], x[0]) : e0 * d[0];
+          x[1] = r ? fmaf(e0, d[1], x[1]) : e0 * d[1];
+          x[2] = r ? fmaf(e1, d[2], x[2]) : e1 * d[2];
+          x[3] = r ? fmaf(e1, d[3], x[3]) : e1 * d[3];
+        }
+        l[0] = c0 * fmaf(x[0], 0x1p20f, d0[0]);
+        l[1] = c1 * fmaf(x[1], 0x1p20f, d0[1]);
+        l[2] = c0 * fmaf(x[2], 0x1p20f, d0[2]);
+        l[3] = c1 * fmaf(x[3], 0x1p20f, d0[3]);
+      }
+      // ---- scales and offsets of the value rows
+      const uint32_t va = base + v_at;
+      uint32_t sv[4][SW], m[4];  // tokens tv0, tv1, tv0 + 8, tv1 + 8
+      lds_matrices<true, D / 2>(m, base + vm_at);
+      lds_words<SW, D / 2>(sv[0], va);
+      lds_words<SW, R + D / 2>(sv[1], va);
+      lds_words<SW, 8 * R + D / 2>(sv[2], va);
+      lds_words<SW, 9 * R + D / 2>(sv[3], va);
+      uint32_t w[4][VW];  // their codes
+      const uint32_t vc = va + g * (D / 16);
+      lds_words<VW, 0>(w[0], vc);
+      lds_words<VW, R>(w[1], vc);
+      lds_words<VW, 8 * R>(w[2], vc);
+      lds_words<VW, 9 * R>(w[3], vc);
+      if constexpr (!kWhole) {
+        // Tokens that do not count: no weight, and no scale or offset that could be anything (0 * NaN).
+        if (!(mask >> tk & 1)) l[0] = l[1] = -INFINITY;
+        if (!(mask >> (tk + 8) & 1)) l[2] = l[3] = -INFINITY;
+        const uint32_t t[4] = {tv0, tv1, tv0 + 8, tv1 + 8};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!(mask >> t[i] & 1)) {
+            const uint32_t stay = i % 2 ? 0x0000ffffu : 0xffff0000u;
+            m[i / 2 * 2] &= stay;
+            m[i / 2 * 2 + 1] &= stay;
+#pragma unroll
+            for (int w = 0; w < SW; ++w) sv[i][w] = 0;
+          }
+      }
+      if constexpr (kScores) {
+        const uint32_t t = n - (uint32_t)left + tk;
+        if (kWhole || (mask >> tk & 1)) {
+          if (store0) lg[t] = l[0];
+          if (store1) lg[a.logit_stride + t] = l[1];
+        }
+        if (kWhole || (mask >> (tk + 8) & 1)) {
+          if (store0) lg[t + 8] = l[2];
+          if (store1) lg[a.logit_stride + t + 8] = l[3];
+        }
+      }
+      // From the first scale >= 2 (bit 14 of an fp16) on p is held smaller.
+      const bool lower = ((m[0] | m[2]) & scale_bits) != 0 && lift > 0.f;
+      // ---- weights; the reference follows the maximum only when it is left 2^6 behind
+      float p[4] = {l[0] - ref0, l[1] - ref1, l[2] - ref0, l[3] - ref1};
+      const float most = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
+      if (__any_sync(0xffffffffu, most > lift + 6.f || lower)) {
+        if (__any_sync(0xffffffffu, lower)) {
+          rescale(ref0 == kFirstRef ? ref0 : ref0 + lift + 4.f, ref1 == kFirstRef ? ref1 : ref1 + lift + 4.f);
+          lift = -4.f;
+        }
+        float m0 = fmaxf(l[0], l[2]), m1 = fmaxf(l[1], l[3]);
+#pragma unroll
+        for (int s = 4; s < 32; s <<= 1) {
+          m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, s));
+          m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, s));
+        }
+        rescale(fmaxf(ref0, m0 - lift), fmaxf(ref1, m1 - lift));
+        p[0] = l[0] - ref0;
+        p[1] = l[1] - ref1;
+        p[2] = l[2] - ref0;
+        p[3] = l[3] - ref1;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = ex2(p[i]);
+      sum0 += p[0] + p[2];
+      sum1 += p[1] + p[3];
+      const uint32_t h01 = pack_half2(p[0], p[1]), h23 = pack_half2(p[2], p[3]);
+      const uint32_t b0 = transpose8(h01), b1 = transpose8(h23);
+      uint32_t bl0 = 0, bl1 = 0;
+      if constexpr (kPrecise) {
+        const float2 r01 = unpack_half2(h01), r23 = unpack_half2(h23);
+        bl0 = transpose8(pack_half2(p[0] - r01.x, p[1] - r01.y));
+        bl1 = transpose8(pack_half2(p[2] - r23.x, p[3] - r23.y));
+      }
+      // ---- sums of p s_r and p o_r: rows r and G + r of accx
+      mma_k16(accx, m[0], m[1], m[2], m[3], b0, b1, accx);
+      if constexpr (kPrecise) mma_k16(accx, m[0], m[1], m[2], m[3], bl0, bl1, accx);
+      // ---- values
+#pragma unroll
+      for (int r = 0; r < G; ++r) {
+        const uint32_t sel = r % 2 ? kHiHalves : kLoHalves, up = r % 2 ? kHiUpper : kLoUpper;
+        const uint32_t s01 = __byte_perm(sv[0][r / 2], sv[1][r / 2], sel), s23 = __byte_perm(sv[2][r / 2], sv[3][r / 2], sel);
+        const uint32_t e0 = mul_half2(b0, s01), e1 = mul_half2(b1, s23);
+        const uint32_t u01 = __byte_perm(w[0][r / 2], w[1][r / 2], sel), u23 = __byte_perm(w[2][r / 2], w[3][r / 2], sel);
+        const uint32_t y01 = __byte_perm(w[0][r / 2], w[1][r / 2], up), y23 = __byte_perm(w[2][r / 2], w[3][r / 2], up);
+        mma_k16(acc[r][0], u01 & kNib0, u01 & kNib1, u23 & kNib0, u23 & kNib1, e0, e1, acc[r][0]);
+        mma_k16(acc[r][1], y01 & kNib0, y01 & kNib1, y23 & kNib0, y23 & kNib1, e0, e1, acc[r][1]);
+        if constexpr (kPrecise) {
+          const uint32_t f0 = fma_half2(bl0, s01, fma_half2(b0, s01, e0 ^ 0x80008000u));
+          const uint32_t f1 = fma_half2(bl1, s23, fma_half2(b1, s23, e1 ^ 0x80008000u));
+          mma_k16(acc[r][0], u01 & kNib0, u01 & kNib1, u23 & kNib0, u23 & kNib1, f0, f1, acc[r][0]);
+          mma_k16(acc[r][1], y01 & kNib0, y01 & kNib1, y23 & kNib0, y23 & kNib1, f0, f1, acc[r][1]);
+        }
+      }
+    };
+
     for (uint32_t k = 0; k < count; ++k) {
       copies_wait<kAttendStages - 2>();
       __syncwarp();  // this tile's rows are there for every lane, and every lane has left the slot of the tile before
       load(slot_before);
-      uint32_t mask = left >= 16 ? 0xffffu : (left > 0 ? (1u << left) - 1u : 0u);
-      if (holes) {
+      if (left >= 16 && !holes) {
+        tile(std::true_type{}, slot, 0xffffu);
+      } else if (left > 0) {
+        uint32_t mask = left >= 16 ? 0xffffu : (1u << left) - 1u;
         const uint32_t word = lds_word<32 * R>(slot);
         if (word != kByLength) mask = word;
+        if (mask) tile(std::false_type{}, slot, mask);
       }
       left -= (int)sh.tokens;
-      if (mask) {
-        const uint32_t base = slot;
-        // ---- logits of 16 tokens
-        float l[4];
-        {
-          uint32_t w0[KW], w1[KW], s0[SW], s1[SW], m[4];
-          const uint32_t ka = base + k_at, kc = ka + q4 * (D / 8);
-          lds_matrices<false, D / 2>(m, base + km_at);
-          lds_words<KW, 0>(w0, kc);
-          lds_words<KW, 8 * R>(w1, kc);
-          lds_words<SW, D / 2>(s0, ka);
-          lds_words<SW, 8 * R + D / 2>(s1, ka);
-          float d0[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_k16(d0, m[0], m[1], m[2], m[3], qo[0], qo[1], d0);
-          if constexpr (G == 8) mma_k16(d0, m[0], m[1], m[2], m[3], qo[2], qo[3], d0);
-          float x[4];
-#pragma unroll
-          for (int r = 0; r < G; ++r) {
-            const uint32_t sel = r % 2 ? kHiHalves : kLoHalves, up = r % 2 ? kHiUpper : kLoUpper;
-            const uint32_t u0 = __byte_perm(w0[r / 2], w0[KW / 2 + r / 2], sel), u1 = __byte_perm(w1[r / 2], w1[KW / 2 + r / 2], sel);
-            const uint32_t y0 = __byte_perm(w0[r / 2], w0[KW / 2 + r / 2], up), y1 = __byte_perm(w1[r / 2], w1[KW / 2 + r / 2], up);
-            float d[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_k16(d, u0 & kNib0, u1 & kNib0, u0 & kNib1, u1 & kNib1, qf[r][0], qf[r][1], d);
-            mma_k16(d, y0 & kNib0, y1 & kNib0, y0 & kNib1, y1 & kNib1, qf[r][2], qf[r][3], d);
-            const float2 f0 = unpack_half2(s0[r / 2]), f1 = unpack_half2(s1[r / 2]);
-            const float e0 = r % 2 ? f0.y : f0.x, e1 = r % 2 ? f1.y : f1.x;
-            x[0] = r ? fmaf(e0, d[0], x[0]) : e0 * d[0];
-            x[1] = r ? fmaf(e0, d[1], x[1]) : e0 * d[1];
-            x[2] = r ? fmaf(e1, d[2], x[2]) : e1 * d[2];
-            x[3] = r ? fmaf(e1, d[3], x[3]) : e1 * d[3];
-          }
-          l[0] = c0 * fmaf(x[0], 0x1p20f, d0[0]);
-          l[1] = c1 * fmaf(x[1], 0x1p20f, d0[1]);
-          l[2] = c0 * fmaf(x[2], 0x1p20f, d0[2]);
-          l[3] = c1 * fmaf(x[3], 0x1p20f, d0[3]);
-        }
-        // ---- scales and offsets of the value rows
-        const uint32_t va = base + v_at;
-        uint32_t sv[4][SW], m[4];  // tokens tv0, tv1, tv0 + 8, tv1 + 8
-        lds_matrices<true, D / 2>(m, base + vm_at);
-        lds_words<SW, D / 2>(sv[0], va);
-        lds_words<SW, R + D / 2>(sv[1], va);
-        lds_words<SW, 8 * R + D / 2>(sv[2], va);
-        lds_words<SW, 9 * R + D / 2>(sv[3], va);
-        uint32_t w[4][VW];  // their codes
-        const uint32_t vc = va + g * (D / 16);
-        lds_words<VW, 0>(w[0], vc);
-        lds_words<VW, R>(w[1], vc);
-        lds_words<VW, 8 * R>(w[2], vc);
-        lds_words<VW, 9 * R>(w[3], vc);
-        if (mask != 0xffffu) {
-          // Tokens that do not count: no weight, and no scale or offset that could be anything (0 * NaN).
-          if (!(mask >> tk & 1)) l[0] = l[1] = -INFINITY;
-          if (!(mask >> (tk + 8) & 1)) l[2] = l[3] = -INFINITY;
-          const uint32_t t[4] = {tv0, tv1, tv0 + 8, tv1 + 8};
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (!(mask >> t[i] & 1)) {
-              const uint32_t stay = i % 2 ? 0x0000ffffu : 0xffff0000u;
-              m[i / 2 * 2] &= stay;
-              m[i / 2 * 2 + 1] &= stay;
-#pragma unroll
-              for (int w = 0; w < SW; ++w) sv[i][w] = 0;
-            }
-        }
-        if constexpr (kScores) {
-          const uint32_t t = (unit0 + k) * sh.tokens + t_sub + tk;
-          if (mask >> tk & 1) {
-            if (store0) lg[t] = l[0];
-            if (store1) lg[a.logit_stride + t] = l[1];
-          }
-          if (mask >> (tk + 8) & 1) {
-            if (store0) lg[t + 8] = l[2];
-            if (store1) lg[a.logit_stride + t + 8] = l[3];
-          }
-        }
-        // From the first scale >= 2 (bit 14 of an fp16) on p is held smaller.
-        const bool lower = ((m[0] | m[2]) & scale_bits) != 0 && lift > 0.f;
-        // ---- weights; the reference follows the maximum only when it is left 2^6 behind
-        float p[4] = {l[0] - ref0, l[1] - ref1, l[2] - ref0, l[3] - ref1};
-        const float most = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
-        if (__any_sync(0xffffffffu, most > lift + 6.f || lower)) {
-          if (__any_sync(0xffffffffu, lower)) {
-            rescale(ref0 == kFirstRef ? ref0 : ref0 + lift + 4.f, ref1 == kFirstRef ? ref1 : ref1 + lift + 4.f);
-            lift = -4.f;
-          }
-          float m0 = fmaxf(l[0], l[2]), m1 = fmaxf(l[1], l[3]);
-#pragma unroll
-          for (int s = 4; s < 32; s <<= 1) {
-            m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, s));
-            m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, s));
-          }
-          rescale(fmaxf(ref0, m0 - lift), fmaxf(ref1, m1 - lift));
-          p[0] = l[0] - ref0;
-          p[1] = l[1] - ref1;
-          p[2] = l[2] - ref0;
-          p[3] = l[3] - ref1;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = ex2(p[i]);
-        sum0 += p[0] + p[2];
-        sum1 += p[1] + p[3];
-        const uint32_t h01 = pack_half2(p[0], p[1]), h23 = pack_half2(p[2], p[3]);
-        const uint32_t b0 = transpose8(h01), b1 = transpose8(h23);
-        uint32_t bl0 = 0, bl1 = 0;
-        if constexpr (kPrecise) {
-          const float2 r01 = unpack_half2(h01), r23 = unpack_half2(h23);
-          bl0 = transpose8(pack_half2(p[0] - r01.x, p[1] - r01.y));
-          bl1 = transpose8(pack_half2(p[2] - r23.x, p[3] - r23.y));
-        }
-        // ---- sums of p s_r and p o_r: rows r and G + r of accx
-        mma_k16(accx, m[0], m[1], m[2], m[3], b0, b1, accx);
-        if constexpr (kPrecise) mma_k16(accx, m[0], m[1], m[2], m[3], bl0, bl1, accx);
-        // ---- values
-#pragma unroll
-        for (int r = 0; r < G; ++r) {
-          const uint32_t sel = r % 2 ? kHiHalves : kLoHalves, up = r % 2 ? kHiUpper : kLoUpper;
-          const uint32_t s01 = __byte_perm(sv[0][r / 2], sv[1][r / 2], sel), s23 = __byte_perm(sv[2][r / 2], sv[3][r / 2], sel);
-          const uint32_t e0 = mul_half2(b0, s01), e1 = mul_half2(b1, s23);
-          const uint32_t u01 = __byte_perm(w[0][r / 2], w[1][r / 2], sel), u23 = __byte_perm(w[2][r / 2], w[3][r / 2], sel);
-          const uint32_t y01 = __byte_perm(w[0][r / 2], w[1][r / 2], up), y23 = __byte_perm(w[2][r / 2], w[3][r / 2], up);
-          mma_k16(acc[r][0], u01 & kNib0, u01 & kNib1, u23 & kNib0, u23 & kNib1, e0, e1, acc[r][0]);
-          mma_k16(acc[r][1], y01 & kNib0, y01 & kNib1, y23 & kNib0, y23 & kNib1, e0, e1, acc[r][1]);
-          if constexpr (kPrecise) {
-            const uint32_t f0 = fma_half2(bl0, s01, fma_half2(b0, s01, e0 ^ 0x80008000u));
-            const uint32_t f1 = fma_half2(bl1, s23, fma_half2(b1, s23, e1 ^ 0x80008000u));
-            mma_k16(acc[r][0], u01 & kNib0, u01 & kNib1, u23 & kNib0, u23 & kNib1, f0, f1, acc[r][0]);
-            mma_k16(acc[r][1], y01 & kNib0, y01 & kNib1, y23 & kNib0, y23 & kNib1, f0, f1, acc[r][1]);
-          }
-        }
-      }
       slot_before = slot;
       slot += kTileBytes;
       if (slot == ring_end) slot = ring;
