@@ -48,7 +48,7 @@ struct AttendShape {
   uint32_t head_groups;  // CTAs' worth of heads: ceil(H / heads_cta)
   uint32_t ntiles;       // tiles of eight query heads per KV head
   uint32_t subsets;      // token subsets of a unit, one warp each
-  uint32_t tokens;       // tokens per unit: 16 * subsets
+  uint32_t tokens;       // tokens per unit: 16 * attend_tiles(D) * subsets
   uint32_t warps;        // heads_cta * ntiles * subsets
   uint32_t stages;       // tiles in a warp's ring
   int32_t block_shift;   // log2 of the block size where it is a power of two >= 16 (a tile lies in one block), else -1
@@ -224,23 +224,28 @@ struct Share {
   uint32_t each, extra;  // the first `extra` CTAs have each + 1 places, the others each
 };
 
-// One CTA per SM. At D = 256 a warp's accumulators and queries take over 128 registers, so it has eight warps.
-__host__ __device__ constexpr int attend_max_warps(int D) { return D == 256 ? 8 : 16; }
-// Tiles in a warp's ring: with all warps, about 150 KB of an SM's shared memory.
+// One CTA of eight warps per SM. A warp takes two tiles of 16 tokens at a time (one at D = 256, where its accumulators and
+// queries fill the registers): their products, which depend on nothing of one another's, hide each other's latency
+// better than twice the warps with half the registers did, and the loop around them is paid once.
+constexpr int kAttendWarps = 8;
+__host__ __device__ constexpr int attend_tiles(int D) { return D == 256 ? 1 : 2; }
+// Slots of attend_tiles() tiles in a warp's ring: about 150 KB of an SM's shared memory.
 __host__ __device__ constexpr int attend_stages(int D) { return D == 64 ? 6 : 4; }
+__host__ __device__ constexpr int attend_slot_bytes(int D) { return attend_tiles(D) * 32 * q4_row_bytes(D) + 16; }
 
 // Decode attention; see the top of the file. kPrecise: carry the remainder of p s_r (fp16 outputs).
 template <typename T, int D, bool kScores>
-__global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_constant__ AttendArgs a) {
   constexpr int G = q4_groups(D), R = q4_row_bytes(D);
   constexpr int KW = D / 32;  // words of codes per lane and token, keys (two units of every group)
   constexpr int VW = D / 64;  // words of codes per lane and token, values (one unit of every group)
   constexpr int SW = (G + 1) / 2;  // words of a token's scales
   constexpr bool kPrecise = std::is_same<T, __half>::value;
-  constexpr int kTileBytes = 32 * R + 16, kAttendStages = attend_stages(D);
+  constexpr int kT = attend_tiles(D), kSlotBytes = attend_slot_bytes(D), kAttendStages = attend_stages(D);
+  constexpr int kTile = 32 * R, kWords = kT * kTile;  // bytes of a tile; where a slot's words begin
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Share share;
-  __shared__ uint32_t scan[16];
+  __shared__ uint32_t scan[kAttendWarps];
 
   const AttendShape &sh = a.sh;
   const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -299,13 +304,13 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
   const uint32_t hl = warp % sh.heads_cta;                 // KV head within the CTA
   const uint32_t nt = warp / sh.heads_cta % sh.ntiles;     // tile of query heads
   const uint32_t sub = warp / (sh.heads_cta * sh.ntiles);  // token subset
-  const uint32_t g = lane / 4, q4 = lane % 4, t_sub = sub * 16;
+  const uint32_t g = lane / 4, q4 = lane % 4, t_sub = sub * 16 * kT;
 
-  // ---- loads: a ring of tiles of 16 key rows and 16 value rows, and a word that says which tokens count: kByLength, or
-  // a mask where a block lies outside the pool (read only once such a block was met)
+  // ---- loads: a ring of slots of kT tiles, 16 key rows and 16 value rows each, and a word per tile that says which tokens
+  // count: kByLength, or a mask where a block lies outside the pool (read only once such a block was met)
   constexpr uint32_t kByLength = 0x10000u;
   constexpr int kChunks = R / 16, kCopies = (R + 31) / 32;  // 16-byte chunks of a row; per lane and plane of a tile
-  const uint32_t ring = smem_u32(smem) + warp * kAttendStages * kTileBytes, ring_end = ring + kAttendStages * kTileBytes;
+  const uint32_t ring = smem_u32(smem) + warp * kAttendStages * kSlotBytes, ring_end = ring + kAttendStages * kSlotBytes;
   uint32_t row_off[kCopies];  // chunk lane + 32 j of a plane: offset from its first row
 #pragma unroll
   for (int j = 0; j < kCopies; ++j) {
@@ -316,8 +321,8 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
   const uint32_t shift = (uint32_t)sh.block_shift & 31u, block_mask = (1u << shift) - 1u;
   const bool paged = sh.block_shift >= 0;
   bool holes = false;              // a block outside the pool was met
-  // Where the next tile to load lies. `run` tiles from here on are 16 tokens of one block each, their blocks at hand in
-  // `ids`; `after` more units of the item follow in the share.
+  // Where the next slot's tokens lie. `run` slots from here on hold whole tiles of one block each, their blocks at hand
+  // in `ids`; `after` more units of the item follow in the share.
   uint32_t ib = b, ihg = hg, iplace = place;
   uint32_t it = unit * sh.tokens + t_sub, in = seq_length(a, b, false), run = 0;
   uint32_t after = min(seq_units(a, in), end - place) - unit;
@@ -350,63 +355,74 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
     enter();
   };
   auto begin_run = [&]() {
-    if (!paged || !ireal || it + 16 > in) return;
+    if (!paged || !ireal || it + 16 * kT > in) return;
     if ((it >> shift) - window >= 32) {  // a unit has at most 256 tokens, 16 blocks
       window += 32;
       ids = ids_next;
       ids_next = entry(window + 32);
     }
     if (__any_sync(0xffffffffu, (uint32_t)ids >= a.pool.num_blocks)) return;
-    const uint32_t whole = (in - it - 16) / sh.tokens + 1;                                          // tiles of 16 tokens
-    const uint32_t known = (uint32_t)((((uint64_t)window + 32) << shift) - it + sh.tokens - 1) / sh.tokens;  // in the window
+    // `it` is a multiple of 16 kT and so is a block, or a pair of blocks: a slot's tiles lie in the same window
+    const uint32_t whole = (in - it - 16 * kT) / sh.tokens + 1;
+    const uint32_t known = (uint32_t)((((uint64_t)window + 32) << shift) - it + sh.tokens - 1) / sh.tokens;
     run = min(min(whole, known), after);
     after -= run;
   };
-  // A tile that is not 16 tokens of one block: the end of a sequence, a block outside the pool, other block sizes.
+  // Tiles that are not 16 tokens of one block: the end of a sequence, a block outside the pool, other block sizes.
   auto load_rest = [&](uint32_t slot) {
-    uint32_t word = kByLength;
-    if (it < in && ireal) {
-      const uint32_t count = min(16u, in - it);
-      auto row_at = [&](uint32_t row) -> uint64_t {
-        const uint32_t blk = (it + row) / a.pool.block_size;
-        const int32_t i = itab[blk];
-        if ((uint32_t)i >= a.pool.num_blocks) {
-          report(a.status, kStatusIdRange, i);
-          return 0;
-        }
-        return ibase + (uint64_t)(uint32_t)i * a.pool.block_stride + (it + row - blk * a.pool.block_size) * a.pool.token_stride;
-      };
-      const uint32_t mask = __ballot_sync(0xffffffffu, lane < count && row_at(lane) != 0);
-      if (mask != (1u << count) - 1u) {
-        holes = true;
-        word = mask;
-      }
 #pragma unroll 1
-      for (uint32_t c = lane; c < count * kChunks; c += 32) {
-        const uint64_t src = row_at(c / kChunks);
-        if (src == 0) continue;
-        copy16(slot + 16 * c, src + c % kChunks * 16);
-        copy16(slot + 16 * R + 16 * c, src + a.pool.plane_stride + c % kChunks * 16);
+    for (uint32_t i = 0; i < kT; ++i) {
+      const uint32_t t = it + 16 * i, to = slot + i * kTile;
+      uint32_t word = kByLength;
+      if (t < in && ireal) {
+        const uint32_t count = min(16u, in - t);
+        auto row_at = [&](uint32_t row) -> uint64_t {
+          const uint32_t blk = (t + row) / a.pool.block_size;
+          const int32_t id = itab[blk];
+          if ((uint32_t)id >= a.pool.num_blocks) {
+            report(a.status, kStatusIdRange, id);
+            return 0;
+          }
+          return ibase + (uint64_t)(uint32_t)id * a.pool.block_stride + (t + row - blk * a.pool.block_size) * a.pool.token_stride;
+        };
+        const uint32_t mask = __ballot_sync(0xffffffffu, lane < count && row_at(lane) != 0);
+        if (mask != (1u << count) - 1u) {
+          holes = true;
+          word = mask;
+        }
+#pragma unroll 1
+        for (uint32_t c = lane; c < count * kChunks; c += 32) {
+          const uint64_t src = row_at(c / kChunks);
+          if (src == 0) continue;
+          copy16(to + 16 * c, src + c % kChunks * 16);
+          copy16(to + 16 * R + 16 * c, src + a.pool.plane_stride + c % kChunks * 16);
+        }
       }
+      sts_word<kWords>(slot + 4 * i, word);
     }
-    sts_word<32 * R>(slot, word);
     it += sh.tokens;
     if (--after == 0) next_item();
+  };
+  auto by_length = [&](uint32_t slot) {
+#pragma unroll
+    for (int i = 0; i < kT; ++i) sts_word<kWords>(slot + 4 * i, kByLength);
   };
   auto load = [&](uint32_t slot) {
     if (run == 0 && after > 0) {
       begin_run();
       if (run == 0) load_rest(slot);
     } else if (run > 0 && holes) {
-      sts_word<32 * R>(slot, kByLength);
+      by_length(slot);
     }
     if (run > 0) {
-      const uint32_t id = (uint32_t)__shfl_sync(0xffffffffu, ids, (it >> shift) - window);
-      const uint64_t k = ibase + (uint64_t)id * (uint32_t)a.pool.block_stride +
-                         (uint64_t)(it & block_mask) * (uint32_t)a.pool.token_stride;
-      const uint64_t v = k + a.pool.plane_stride;
-      const uint32_t dst = slot + 16 * lane;
-      copy_tile<R, 0>(dst, k, v, row_off, tail_lane);
+#pragma unroll
+      for (int i = 0; i < kT; ++i) {
+        const uint32_t t = it + 16 * i;
+        const uint32_t id = (uint32_t)__shfl_sync(0xffffffffu, ids, (t >> shift) - window);
+        const uint64_t k = ibase + (uint64_t)id * (uint32_t)a.pool.block_stride +
+                           (uint64_t)(t & block_mask) * (uint32_t)a.pool.token_stride;
+        copy_tile<R, 0>(slot + i * kTile + 16 * lane, k, k + a.pool.plane_stride, row_off, tail_lane);
+      }
       it += sh.tokens;
       if (--run == 0 && after == 0) next_item();
     }
@@ -414,7 +430,7 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
   };
   enter();
 #pragma unroll 1
-  for (uint32_t s = ring; s < ring_end; s += kTileBytes) sts_word<32 * R>(s, kByLength);
+  for (uint32_t s = ring; s < ring_end; s += kSlotBytes) by_length(s);
   uint4 q_raw[G];  // eight channels of every group of the query row of this lane
   auto fetch_query = [&]() {
     const uint32_t h = hg * sh.heads_cta + hl, j = nt * 8 + g;
@@ -433,7 +449,7 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
     }
   };
 #pragma unroll 1
-  for (uint32_t s = ring; s < ring_end - kTileBytes; s += kTileBytes) load(s);
+  for (uint32_t s = ring; s < ring_end - kSlotBytes; s += kSlotBytes) load(s);
 
   // Tokens are fragment rows in their order. Rows are R apart, an odd multiple of 16 bytes at D = 64 and 128: the value
   // loads and the matrix loads touch every bank once.
@@ -446,9 +462,9 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
   const uint32_t km_at = (mt + 8 * (mi & 1)) * R + (G == 8 && mi >= 2 ? 2 * G : 0);
   const uint32_t vm_at = (16 + mt + 8 * (mi >> 1)) * R + (G == 8 && (mi & 1) ? 2 * G : 0);
   const uint32_t scale_bits = G == 8 || g < (uint32_t)G ? 0x40004000u : 0u;  // >= 2, where this lane's rows are scales
-  uint32_t slot = ring, slot_before = ring_end - kTileBytes;  // of the tile to compute, and of the one before it
+  uint32_t slot = ring, slot_before = ring_end - kSlotBytes;  // the slot to compute on, and the one before it
 
-  float *merge = reinterpret_cast<float *>(smem + sh.warps * kAttendStages * kTileBytes);  // [(warps - warps/subsets)][8][D + 2]
+  float *merge = reinterpret_cast<float *>(smem + sh.warps * kAttendStages * kSlotBytes);  // [(warps - warps/subsets)][8][D + 2]
 
   while (place < end) {
     const uint32_t n = seq_length(a, b, false), units = seq_units(a, n);
@@ -562,15 +578,17 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
     };
 
     int left = active ? (int)n - (int)(unit0 * sh.tokens + t_sub) : 0;  // tokens from this warp's next tile on
-    // One tile. kWhole: all 16 tokens count (mask is not read).
-    auto tile = [&](auto whole_tag, const uint32_t base, const uint32_t mask) {
+    // N tiles, the first at position n - left. kWhole: all their tokens count (mask is not read; else N = 1).
+    auto tiles = [&](auto whole_tag, auto count_tag, const uint32_t base, const uint32_t mask) {
       constexpr bool kWhole = decltype(whole_tag)::value;
-        // ---- logits of 16 tokens
-      float l[4];
-      {
+      constexpr int N = decltype(count_tag)::value;
+      // ---- logits of 16 tokens each
+      float l[N][4];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
         uint32_t w0[KW], w1[KW], s0[SW], s1[SW], m[4];
-        const uint32_t ka = base + k_at, kc = ka + q4 * (D / 8);
-        lds_matrices<false, D / 2>(m, base + km_at);
+        const uint32_t ka = base + i * kTile + k_at, kc = ka + q4 * (D / 8);
+        lds_matrices<false, D / 2>(m, base + i * kTile + km_at);
         lds_words<KW, 0>(w0, kc);
         lds_words<KW, 8 * R>(w1, kc);
         lds_words<SW, D / 2>(s0, ka);
@@ -594,122 +612,152 @@ __global__ void __launch_bounds__(attend_max_warps(D) * 32, 1) attend_q4(const _
           x[2] = r ? fmaf(e1, d[2], x[2]) : e1 * d[2];
           x[3] = r ? fmaf(e1, d[3], x[3]) : e1 * d[3];
         }
-        l[0] = c0 * fmaf(x[0], 0x1p20f, d0[0]);
-        l[1] = c1 * fmaf(x[1], 0x1p20f, d0[1]);
-        l[2] = c0 * fmaf(x[2], 0x1p20f, d0[2]);
-        l[3] = c1 * fmaf(x[3], 0x1p20f, d0[3]);
+        l[i][0] = c0 * fmaf(x[0], 0x1p20f, d0[0]);
+        l[i][1] = c1 * fmaf(x[1], 0x1p20f, d0[1]);
+        l[i][2] = c0 * fmaf(x[2], 0x1p20f, d0[2]);
+        l[i][3] = c1 * fmaf(x[3], 0x1p20f, d0[3]);
       }
-      // ---- scales and offsets of the value rows
-      const uint32_t va = base + v_at;
-      uint32_t sv[4][SW], m[4];  // tokens tv0, tv1, tv0 + 8, tv1 + 8
-      lds_matrices<true, D / 2>(m, base + vm_at);
-      lds_words<SW, D / 2>(sv[0], va);
-      lds_words<SW, R + D / 2>(sv[1], va);
-      lds_words<SW, 8 * R + D / 2>(sv[2], va);
-      lds_words<SW, 9 * R + D / 2>(sv[3], va);
-      uint32_t w[4][VW];  // their codes
-      const uint32_t vc = va + g * (D / 16);
-      lds_words<VW, 0>(w[0], vc);
-      lds_words<VW, R>(w[1], vc);
-      lds_words<VW, 8 * R>(w[2], vc);
-      lds_words<VW, 9 * R>(w[3], vc);
+      // ---- scales, offsets and codes of the value rows: tokens tv0, tv1, tv0 + 8, tv1 + 8
+      uint32_t sv[N][4][SW], m[N][4], w[N][4][VW];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t va = base + i * kTile + v_at, vc = va + g * (D / 16);
+        lds_matrices<true, D / 2>(m[i], base + i * kTile + vm_at);
+        lds_words<SW, D / 2>(sv[i][0], va);
+        lds_words<SW, R + D / 2>(sv[i][1], va);
+        lds_words<SW, 8 * R + D / 2>(sv[i][2], va);
+        lds_words<SW, 9 * R + D / 2>(sv[i][3], va);
+        lds_words<VW, 0>(w[i][0], vc);
+        lds_words<VW, R>(w[i][1], vc);
+        lds_words<VW, 8 * R>(w[i][2], vc);
+        lds_words<VW, 9 * R>(w[i][3], vc);
+      }
       if constexpr (!kWhole) {
         // Tokens that do not count: no weight, and no scale or offset that could be anything (0 * NaN).
-        if (!(mask >> tk & 1)) l[0] = l[1] = -INFINITY;
-        if (!(mask >> (tk + 8) & 1)) l[2] = l[3] = -INFINITY;
+        if (!(mask >> tk & 1)) l[0][0] = l[0][1] = -INFINITY;
+        if (!(mask >> (tk + 8) & 1)) l[0][2] = l[0][3] = -INFINITY;
         const uint32_t t[4] = {tv0, tv1, tv0 + 8, tv1 + 8};
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (!(mask >> t[i] & 1)) {
             const uint32_t stay = i % 2 ? 0x0000ffffu : 0xffff0000u;
-            m[i / 2 * 2] &= stay;
-            m[i / 2 * 2 + 1] &= stay;
+            m[0][i / 2 * 2] &= stay;
+            m[0][i / 2 * 2 + 1] &= stay;
 #pragma unroll
-            for (int w = 0; w < SW; ++w) sv[i][w] = 0;
+            for (int k = 0; k < SW; ++k) sv[0][i][k] = 0;
           }
       }
       if constexpr (kScores) {
-        const uint32_t t = n - (uint32_t)left + tk;
-        if (kWhole || (mask >> tk & 1)) {
-          if (store0) lg[t] = l[0];
-          if (store1) lg[a.logit_stride + t] = l[1];
-        }
-        if (kWhole || (mask >> (tk + 8) & 1)) {
-          if (store0) lg[t + 8] = l[2];
-          if (store1) lg[a.logit_stride + t + 8] = l[3];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const uint32_t t = n - (uint32_t)left + 16 * i + tk;
+          if (kWhole || (mask >> tk & 1)) {
+            if (store0) lg[t] = l[i][0];
+            if (store1) lg[a.logit_stride + t] = l[i][1];
+          }
+          if (kWhole || (mask >> (tk + 8) & 1)) {
+            if (store0) lg[t + 8] = l[i][2];
+            if (store1) lg[a.logit_stride + t + 8] = l[i][3];
+          }
         }
       }
-      // From the first scale >= 2 (bit 14 of an fp16) on p is held smaller.
-      const bool lower = ((m[0] | m[2]) & scale_bits) != 0 && lift > 0.f;
-      // ---- weights; the reference follows the maximum only when it is left 2^6 behind
-      float p[4] = {l[0] - ref0, l[1] - ref1, l[2] - ref0, l[3] - ref1};
-      const float most = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
+      // ---- weights; the reference follows the maximum only when it is left 2^6 behind. From the first scale >= 2 (bit 14
+      // of an fp16) on p is held smaller.
+      float p[N][4], most = kFirstRef;
+      uint32_t big = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        big |= m[i][0] | m[i][2];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          p[i][k] = l[i][k] - (k % 2 ? ref1 : ref0);
+          most = fmaxf(most, p[i][k]);
+        }
+      }
+      const bool lower = (big & scale_bits) != 0 && lift > 0.f;
       if (__any_sync(0xffffffffu, most > lift + 6.f || lower)) {
         if (__any_sync(0xffffffffu, lower)) {
           rescale(ref0 == kFirstRef ? ref0 : ref0 + lift + 4.f, ref1 == kFirstRef ? ref1 : ref1 + lift + 4.f);
           lift = -4.f;
         }
-        float m0 = fmaxf(l[0], l[2]), m1 = fmaxf(l[1], l[3]);
+        float m0 = l[0][0], m1 = l[0][1];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          m0 = fmaxf(m0, fmaxf(l[i][0], l[i][2]));
+          m1 = fmaxf(m1, fmaxf(l[i][1], l[i][3]));
+        }
 #pragma unroll
         for (int s = 4; s < 32; s <<= 1) {
           m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, s));
           m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, s));
         }
         rescale(fmaxf(ref0, m0 - lift), fmaxf(ref1, m1 - lift));
-        p[0] = l[0] - ref0;
-        p[1] = l[1] - ref1;
-        p[2] = l[2] - ref0;
-        p[3] = l[3] - ref1;
-      }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = ex2(p[i]);
-      sum0 += p[0] + p[2];
-      sum1 += p[1] + p[3];
-      const uint32_t h01 = pack_half2(p[0], p[1]), h23 = pack_half2(p[2], p[3]);
-      const uint32_t b0 = transpose8(h01), b1 = transpose8(h23);
-      uint32_t bl0 = 0, bl1 = 0;
-      if constexpr (kPrecise) {
-        const float2 r01 = unpack_half2(h01), r23 = unpack_half2(h23);
-        bl0 = transpose8(pack_half2(p[0] - r01.x, p[1] - r01.y));
-        bl1 = transpose8(pack_half2(p[2] - r23.x, p[3] - r23.y));
-      }
-      // ---- sums of p s_r and p o_r: rows r and G + r of accx
-      mma_k16(accx, m[0], m[1], m[2], m[3], b0, b1, accx);
-      if constexpr (kPrecise) mma_k16(accx, m[0], m[1], m[2], m[3], bl0, bl1, accx);
-      // ---- values
+        for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int r = 0; r < G; ++r) {
-        const uint32_t sel = r % 2 ? kHiHalves : kLoHalves, up = r % 2 ? kHiUpper : kLoUpper;
-        const uint32_t s01 = __byte_perm(sv[0][r / 2], sv[1][r / 2], sel), s23 = __byte_perm(sv[2][r / 2], sv[3][r / 2], sel);
-        const uint32_t e0 = mul_half2(b0, s01), e1 = mul_half2(b1, s23);
-        const uint32_t u01 = __byte_perm(w[0][r / 2], w[1][r / 2], sel), u23 = __byte_perm(w[2][r / 2], w[3][r / 2], sel);
-        const uint32_t y01 = __byte_perm(w[0][r / 2], w[1][r / 2], up), y23 = __byte_perm(w[2][r / 2], w[3][r / 2], up);
-        mma_k16(acc[r][0], u01 & kNib0, u01 & kNib1, u23 & kNib0, u23 & kNib1, e0, e1, acc[r][0]);
-        mma_k16(acc[r][1], y01 & kNib0, y01 & kNib1, y23 & kNib0, y23 & kNib1, e0, e1, acc[r][1]);
+          for (int k = 0; k < 4; ++k) p[i][k] = l[i][k] - (k % 2 ? ref1 : ref0);
+      }
+      uint32_t b0[N], b1[N], bl0[N], bl1[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) p[i][k] = ex2(p[i][k]);
+        sum0 += p[i][0] + p[i][2];
+        sum1 += p[i][1] + p[i][3];
+        const uint32_t h01 = pack_half2(p[i][0], p[i][1]), h23 = pack_half2(p[i][2], p[i][3]);
+        b0[i] = transpose8(h01);
+        b1[i] = transpose8(h23);
         if constexpr (kPrecise) {
-          const uint32_t f0 = fma_half2(bl0, s01, fma_half2(b0, s01, e0 ^ 0x80008000u));
-          const uint32_t f1 = fma_half2(bl1, s23, fma_half2(b1, s23, e1 ^ 0x80008000u));
-          mma_k16(acc[r][0], u01 & kNib0, u01 & kNib1, u23 & kNib0, u23 & kNib1, f0, f1, acc[r][0]);
-          mma_k16(acc[r][1], y01 & kNib0, y01 & kNib1, y23 & kNib0, y23 & kNib1, f0, f1, acc[r][1]);
+          const float2 r01 = unpack_half2(h01), r23 = unpack_half2(h23);
+          bl0[i] = transpose8(pack_half2(p[i][0] - r01.x, p[i][1] - r01.y));
+          bl1[i] = transpose8(pack_half2(p[i][2] - r23.x, p[i][3] - r23.y));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        // ---- sums of p s_r and p o_r: rows r and G + r of accx
+        mma_k16(accx, m[i][0], m[i][1], m[i][2], m[i][3], b0[i], b1[i], accx);
+        if constexpr (kPrecise) mma_k16(accx, m[i][0], m[i][1], m[i][2], m[i][3], bl0[i], bl1[i], accx);
+        // ---- values
+#pragma unroll
+        for (int r = 0; r < G; ++r) {
+          const uint32_t sel = r % 2 ? kHiHalves : kLoHalves, up = r % 2 ? kHiUpper : kLoUpper;
+          const uint32_t s01 = __byte_perm(sv[i][0][r / 2], sv[i][1][r / 2], sel), s23 = __byte_perm(sv[i][2][r / 2], sv[i][3][r / 2], sel);
+          const uint32_t e0 = mul_half2(b0[i], s01), e1 = mul_half2(b1[i], s23);
+          const uint32_t u01 = __byte_perm(w[i][0][r / 2], w[i][1][r / 2], sel), u23 = __byte_perm(w[i][2][r / 2], w[i][3][r / 2], sel);
+          const uint32_t y01 = __byte_perm(w[i][0][r / 2], w[i][1][r / 2], up), y23 = __byte_perm(w[i][2][r / 2], w[i][3][r / 2], up);
+          mma_k16(acc[r][0], u01 & kNib0, u01 & kNib1, u23 & kNib0, u23 & kNib1, e0, e1, acc[r][0]);
+          mma_k16(acc[r][1], y01 & kNib0, y01 & kNib1, y23 & kNib0, y23 & kNib1, e0, e1, acc[r][1]);
+          if constexpr (kPrecise) {
+            const uint32_t f0 = fma_half2(bl0[i], s01, fma_half2(b0[i], s01, e0 ^ 0x80008000u));
+            const uint32_t f1 = fma_half2(bl1[i], s23, fma_half2(b1[i], s23, e1 ^ 0x80008000u));
+            mma_k16(acc[r][0], u01 & kNib0, u01 & kNib1, u23 & kNib0, u23 & kNib1, f0, f1, acc[r][0]);
+            mma_k16(acc[r][1], y01 & kNib0, y01 & kNib1, y23 & kNib0, y23 & kNib1, f0, f1, acc[r][1]);
+          }
         }
       }
     };
 
     for (uint32_t k = 0; k < count; ++k) {
       copies_wait<kAttendStages - 2>();
-      __syncwarp();  // this tile's rows are there for every lane, and every lane has left the slot of the tile before
+      __syncwarp();  // this slot's rows are there for every lane, and every lane has left the slot before
       load(slot_before);
-      if (left >= 16 && !holes) {
-        tile(std::true_type{}, slot, 0xffffu);
-      } else if (left > 0) {
-        uint32_t mask = left >= 16 ? 0xffffu : (1u << left) - 1u;
-        const uint32_t word = lds_word<32 * R>(slot);
-        if (word != kByLength) mask = word;
-        if (mask) tile(std::false_type{}, slot, mask);
+      if (left >= 16 * kT && !holes) {
+        tiles(std::true_type{}, std::integral_constant<int, kT>{}, slot, 0xffffu);
+        left -= (int)sh.tokens;
+      } else {
+        const int next = left - (int)sh.tokens;
+#pragma unroll 1
+        for (uint32_t i = 0; i < kT && left > 0; ++i, left -= 16) {
+          uint32_t mask = left >= 16 ? 0xffffu : (1u << left) - 1u;
+          const uint32_t word = lds_word<kWords>(slot + 4 * i);
+          if (word != kByLength) mask = word;
+          if (mask) tiles(std::false_type{}, std::integral_constant<int, 1>{}, slot + i * kTile, mask);
+        }
+        left = next;
       }
-      left -= (int)sh.tokens;
       slot_before = slot;
-      slot += kTileBytes;
+      slot += kSlotBytes;
       if (slot == ring_end) slot = ring;
     }
 

@@ -142,7 +142,7 @@ int q4_rows_impl(emm_pool *pool, bool append, int32_t D, int32_t dtype, int32_t 
 int attend_shape(const emm_pool *pool, int32_t D, int32_t B, int32_t group, int32_t max_len, emm::AttendShape *out,
                  int *smem_out) {
   const emm_pool_desc &d = pool->desc;
-  const uint32_t R = (uint32_t)emm::q4_row_bytes(D), H = (uint32_t)d.num_kv_heads;
+  const uint32_t H = (uint32_t)d.num_kv_heads;
   emm::AttendShape s;
   s.ntiles = (uint32_t)(group + 7) / 8;
   // KV heads first (their rows of a token are one copy), in equal shares of at most eight warps, then the tokens of a
@@ -152,20 +152,21 @@ int attend_shape(const emm_pool *pool, int32_t D, int32_t B, int32_t group, int3
   s.heads_cta = (H + s.head_groups - 1) / s.head_groups;
   s.items = (uint32_t)B * s.head_groups;
   const uint64_t sms = (uint64_t)pool->ctx->sm_count;
-  s.subsets = std::max(1u, (uint32_t)emm::attend_max_warps(D) / (s.heads_cta * s.ntiles));
+  s.subsets = std::max(1u, (uint32_t)emm::kAttendWarps / (s.heads_cta * s.ntiles));
   auto units = [&]() {
-    return std::max<uint64_t>(1, ((uint64_t)max_len + 16 * s.subsets - 1) / (16 * s.subsets)) * s.items;
+    const uint32_t tokens = 16 * (uint32_t)emm::attend_tiles(D) * s.subsets;
+    return std::max<uint64_t>(1, ((uint64_t)max_len + tokens - 1) / tokens) * s.items;
   };
   // Little work is spread over more, smaller CTAs.
   while (s.subsets > 1 && units() < sms) s.subsets /= 2;
-  s.tokens = 16 * s.subsets;
+  s.tokens = 16 * (uint32_t)emm::attend_tiles(D) * s.subsets;
   s.warps = s.heads_cta * s.ntiles * s.subsets;
   // A tile's offsets within a block take 32 bits.
   s.block_shift = d.token_stride < 1 << 27 && d.block_stride <= 0xffffffffll ? shift_of(d.block_size) : -1;
   if (s.block_shift < 4) s.block_shift = -1;
   s.stages = (uint32_t)emm::attend_stages(D);
   const int merge = (int)((s.subsets - 1) * s.heads_cta * s.ntiles * 8 * (uint32_t)(D + 2) * 4);
-  *smem_out = (int)(s.warps * s.stages * (32 * R + 16)) + merge;
+  *smem_out = (int)(s.warps * s.stages * (uint32_t)emm::attend_slot_bytes(D)) + merge;
   if (units() + (uint64_t)emm::kItemCost * s.items > 0x7fffffffull)
     return fail(EMM_ERR_TOO_LARGE, "q4_attend: %d sequences of up to %d tokens", B, max_len);
   s.grid = (uint32_t)std::min<uint64_t>(units() + (uint64_t)emm::kItemCost * s.items, sms);
