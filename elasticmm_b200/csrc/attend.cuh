@@ -982,17 +982,19 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join(const __grid_cons
     a.lse[(uint64_t)b * a.kv_heads * a.group + head] = sum == 0.f ? INFINITY : top + lg2(sum);
 }
 
-// Adds every token's weight to its score. Persistent: a block takes chunks of 1024 tokens of a (sequence, KV head) pair,
-// four tokens a thread.
-constexpr uint32_t kScoreChunk = 1024;
+// Adds every token's weight to its score. A warp's turn is 128 tokens of a (sequence, KV head) pair, four a lane; turns go
+// chunk by chunk over all pairs, so that long and short sequences are spread over all warps. Nothing here needs the
+// latency hidden better than by many warps with few registers.
+constexpr uint32_t kScoreTokens = 128;
 
-__global__ void __launch_bounds__(256) attend_scores(const __grid_constant__ AttendArgs a, const uint32_t chunks) {
+__global__ void __launch_bounds__(256, 6) attend_scores(const __grid_constant__ AttendArgs a, const uint32_t chunks) {
   grid_launch_dependents();
   grid_dependency_wait();
-  const uint64_t total = (uint64_t)a.num_seqs * a.kv_heads * chunks;
-  for (uint64_t i = blockIdx.x; i < total; i += gridDim.x) {
-    const uint32_t bh = (uint32_t)(i / chunks), b = bh / a.kv_heads, h = bh % a.kv_heads;
-    const uint32_t n = seq_length(a, b, false), t = (uint32_t)(i % chunks) * kScoreChunk + threadIdx.x * 4;
+  const uint32_t lane = threadIdx.x % 32, pairs = a.num_seqs * a.kv_heads;
+  const uint64_t total = (uint64_t)pairs * chunks, step = (uint64_t)gridDim.x * 8;
+  for (uint64_t i = (uint64_t)blockIdx.x * 8 + threadIdx.x / 32; i < total; i += step) {
+    const uint32_t c = (uint32_t)(i / pairs), bh = (uint32_t)(i - (uint64_t)c * pairs), b = bh / a.kv_heads, h = bh - b * a.kv_heads;
+    const uint32_t n = seq_length(a, b, false), t = c * kScoreTokens + lane * 4;
     if (t >= n) continue;
     const uint64_t head = (uint64_t)bh * a.group;
     float *sc[4];
@@ -1002,14 +1004,14 @@ __global__ void __launch_bounds__(256) attend_scores(const __grid_constant__ Att
       sc[k] = nullptr;
       old[k] = 0.f;
       if (t + k >= n) continue;
-      const uint32_t blk = (t + k) / a.pool.block_size;
+      const uint32_t blk = a.pool.block_shift >= 0 ? (t + k) >> a.pool.block_shift : (t + k) / a.pool.block_size;
       const int32_t id = a.tables[b * a.table_stride + blk];
       if ((uint32_t)id >= a.pool.num_blocks) continue;
       sc[k] = reinterpret_cast<float *>(a.score_base + (uint64_t)id * a.score_block_stride) + (uint64_t)h * a.pool.block_size +
               (t + k - blk * a.pool.block_size);
       old[k] = *sc[k];
     }
-#pragma unroll 8
+#pragma unroll 4
     for (uint32_t j = 0; j < a.group; ++j) {
       const float lse = a.lse[head + j];
       const float4 l = *reinterpret_cast<const float4 *>(a.logits + (head + j) * a.logit_stride + t);

@@ -250,9 +250,9 @@ int attend_launch(emm_ctx *ctx, const emm::AttendArgs &a, int smem, cudaStream_t
     ctx->launches += 1;
   }
   if (a.score_base && a.max_len > 0) {
-    const uint32_t chunks = (a.max_len + emm::kScoreChunk - 1) / emm::kScoreChunk;
-    const uint64_t total = (uint64_t)a.num_seqs * a.kv_heads * chunks;
-    cfg.gridDim = dim3((unsigned)std::min<uint64_t>(total, (uint64_t)ctx->sm_count * 8));
+    const uint32_t chunks = (a.max_len + emm::kScoreTokens - 1) / emm::kScoreTokens;
+    const uint64_t turns = (uint64_t)a.num_seqs * a.kv_heads * chunks;
+    cfg.gridDim = dim3((unsigned)std::min<uint64_t>((turns + 7) / 8, (uint64_t)ctx->sm_count * 6));
     cfg.blockDim = dim3(256);
     EMM_CUDA(cudaLaunchKernelEx(&cfg, emm::attend_scores, a, chunks));
     ctx->launches += 1;
