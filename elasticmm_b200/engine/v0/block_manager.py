@@ -8,7 +8,8 @@ location and parks the old ids on a "swapping" list that is folded back into
 the free list once the copies are known to be done (:118-123,305-377).
 
 Added here, with no counterpart in the reference: `compact` (defragmentation
-plan + table rewrite, planned by the C library's emm_compact_plan) and
+plan + table rewrite, planned by the C library's emm_compact_plan),
+`truncate_blocks` (the blocks behind a request's kept tokens) and
 `get_slot_mapping` (the table-to-slot arithmetic that the model runner
 applies before reshape_and_cache, elasticmm/engine/v0/worker_steps.py:219,411).
 """
@@ -228,6 +229,21 @@ class V0BlockManager:
         table = self.block_table[request_id]
         bs = self.block_size
         return [table[p // bs] * bs + p % bs for p in positions]
+
+    def truncate_blocks(self, request_id: str, num_tokens: int) -> List[int]:
+        """Frees the blocks behind a request's first `num_tokens` tokens, as an eviction leaves them
+        (V0Worker.evict_tokens); returns their ids. The caller's launches that read those blocks must come before the
+        next owner's writes on the stream."""
+        if request_id not in self.block_table:
+            raise ValueError(f"Request {request_id} not allocated")
+        if num_tokens < 0:
+            raise ValueError(f"num_tokens must not be negative, got {num_tokens}")
+        table = self.block_table[request_id]
+        need = -(-num_tokens // self.block_size)
+        freed = table[need:]
+        del table[need:]
+        self._free[self.request_location[request_id]].extend(freed)
+        return freed
 
     def compact(self) -> Tuple[List[int], List[int]]:
         """Plans a defragmentation of the GPU pool and rewrites the tables.

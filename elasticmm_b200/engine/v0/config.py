@@ -39,6 +39,7 @@ class V0KVCacheConfig:
     num_kv_heads: int = 32
     head_size: int = 128
     layout: str = "nhd"          # "nhd": [2, NB, BS, H, D] (reference), "hnd": [2, NB, H, BS, D]
+    kv_bits: int = 16            # 4: a 4-bit cache (KVPoolQ4), `dtype` is then that of keys, values and queries
     # B200_PEER only: which end runs the copy kernel
     peer_direction: str = "pull"
 
@@ -65,6 +66,10 @@ class V0KVCacheConfig:
         assert self.layout in ("nhd", "hnd"), f"Unknown pool layout: {self.layout}"
         assert self.peer_direction in ("pull", "push"), f"Unknown peer direction: {self.peer_direction}"
         assert min(self.num_layers, self.num_kv_heads, self.head_size) > 0, "Pool geometry must be positive"
+        assert self.kv_bits in (4, 16), f"kv_bits must be 16 (a pool of `dtype`) or 4: {self.kv_bits}"
+        if self.kv_bits == 4:
+            assert self.head_size in (64, 128, 256), f"A 4-bit cache has 64, 128 or 256 channels: {self.head_size}"
+            assert self.dtype in ("float16", "half", "bfloat16"), f"A 4-bit cache takes 16-bit keys and values: {self.dtype}"
 
     # -- derived quantities ---------------------------------------------------
 
@@ -79,7 +84,10 @@ class V0KVCacheConfig:
     @property
     def page_bytes(self) -> int:
         """One block of one plane (K or V) of one layer."""
-        return self.block_size * self.num_kv_heads * self.head_size * self.elem_size
+        row = self.head_size * self.elem_size
+        if self.kv_bits == 4:  # codes, then a 16-bit scale and offset per 32 channels, to a multiple of 16
+            row = -(-(self.head_size // 2 + self.head_size // 8) // 16) * 16
+        return self.block_size * self.num_kv_heads * row
 
     @property
     def block_bytes(self) -> int:

@@ -24,6 +24,7 @@ import torch.distributed as dist
 
 from ... import _lib
 from ...kv_pool import Context, KVPool, _as_host_ids, get_context
+from ...kv_pool_q4 import KVPoolQ4, ScorePool, alloc_q4_layers
 from .transport import (MigrationPlan, plan_chunks, max_chunk_layers, pipelined_recv,
                         pipelined_send, run_waves, PIPELINE_DEPTH)
 from .utils import EngineStage
@@ -63,9 +64,14 @@ class V0Worker:
         world_size: Optional[int] = None,
         nccl_init_method: Optional[str] = None,
         kv_cache: Optional[Sequence[torch.Tensor]] = None,
+        kv_bits: int = 16,
     ):
         if not torch.cuda.is_available():
             raise RuntimeError("V0Worker needs a CUDA device; the KV data plane has no CPU path")
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 16 (a pool of dtype) or 4, got {kv_bits}")
+        self.kv_bits = kv_bits
+        self.scores: Optional[ScorePool] = None  # accumulated attention weights (init_scores)
         self.worker_id = worker_id
         self.stage = stage
         self.original_role = stage
@@ -115,6 +121,14 @@ class V0Worker:
         """
         if layout not in ("nhd", "hnd"):
             raise ValueError(f"unknown pool layout {layout!r}")
+        if self.kv_bits == 4:
+            self.bind_kv_cache(alloc_q4_layers(num_layers, num_gpu_blocks, self.block_size, num_kv_heads, head_size,
+                                               self.device, layout))
+            if num_cpu_blocks > 0:
+                self.bind_kv_swap([t.pin_memory() if layout == "nhd" else t.permute(0, 1, 3, 2, 4).pin_memory().permute(0, 1, 3, 2, 4)
+                                   for t in alloc_q4_layers(num_layers, num_cpu_blocks, self.block_size, num_kv_heads,
+                                                            head_size, "cpu", layout)])
+            return
         dt = _DTYPES[self.dtype]
 
         def alloc(nb: int, pinned: bool) -> torch.Tensor:
@@ -139,7 +153,7 @@ class V0Worker:
         counts default to the configuration's maxima)."""
         config.validate()
         w = cls(worker_id=worker_id, stage=stage, block_size=config.block_size, dtype=config.dtype,
-                device=device, global_rank=global_rank, world_size=world_size)
+                device=device, global_rank=global_rank, world_size=world_size, kv_bits=config.kv_bits)
         w.init_kvcache(config.max_num_gpu_blocks if num_gpu_blocks is None else num_gpu_blocks,
                        config.num_layers, config.num_kv_heads, config.head_size,
                        num_cpu_blocks=config.max_num_cpu_blocks if num_cpu_blocks is None else num_cpu_blocks,
@@ -147,9 +161,15 @@ class V0Worker:
         return w
 
     def bind_kv_cache(self, kv_cache: Sequence[torch.Tensor]) -> None:
-        """Adopts an existing list of per-layer pool tensors (not copied)."""
+        """Adopts an existing list of per-layer pool tensors (not copied); with kv_bits 4 uint8 tensors of 4-bit rows."""
         self.kv_cache = list(kv_cache)
-        self.pool = KVPool(self.kv_cache, self.ctx)
+        if self.kv_bits == 4:
+            row = self.kv_cache[0].shape[-1] if self.kv_cache else 0
+            head = next((d for d in (64, 128, 256) if KVPoolQ4.row_bytes(d) == row), 128)
+            self.pool = KVPoolQ4(self.kv_cache, head, self.ctx)
+        else:
+            self.pool = KVPool(self.kv_cache, self.ctx)
+        self.scores = None
 
     def bind_kv_swap(self, kv_swap: Sequence[torch.Tensor]) -> None:
         """Adopts a pinned host pool with the GPU pool's page geometry."""
@@ -185,7 +205,38 @@ class V0Worker:
         assert kv_data.shape[2] == len(block_indices), (
             f"Block count mismatch: {kv_data.shape[2]} vs {len(block_indices)}")
         with _range("emm.write_kv_blocks"):
-            pool.scatter(block_indices, kv_data)
+            if self.kv_bits == 4 and kv_data.dtype != torch.uint8:
+                self._quantize_kv_blocks(block_indices, kv_data)
+            else:
+                pool.scatter(block_indices, kv_data)
+
+    def _quantize_kv_blocks(self, block_indices: List[int], kv_data: torch.Tensor) -> None:
+        """write_kv_blocks of a 16-bit worker's blocks into a 4-bit pool: [L, 2, n, BS, H, D] fp16 or bf16."""
+        pool = self._require_pool()
+        n, bs = len(block_indices), pool.block_size
+        want = (pool.num_layers, 2, n, bs, pool.num_kv_heads, pool.head_dim)
+        if tuple(kv_data.shape) != want:
+            raise ValueError(f"packed tensor has shape {tuple(kv_data.shape)}, expected {want}")
+        host = pool._validated(_as_host_ids(block_indices), unique=True)
+        first = pool.upload_ids(host).long() * bs
+        slots = (first[:, None] + torch.arange(bs, device=self.device)).flatten()
+        # a head-major worker's blocks are a permuted view: made token-major first
+        rows = kv_data if kv_data.is_contiguous() else kv_data.contiguous()
+        pool.append_all_layers(rows[:, 0].flatten(1, 2), rows[:, 1].flatten(1, 2), slots)
+
+    def read_kv_blocks(self, block_indices: List[int]) -> torch.Tensor:
+        """The blocks of a 4-bit pool as [L, 2, n, BS, H, D] of the worker's dtype, for a 16-bit consumer
+        (extract_kv_blocks gives the rows' bytes, which move between 4-bit workers)."""
+        pool = self._require_pool()
+        if self.kv_bits != 4:
+            raise RuntimeError("read_kv_blocks is for a 4-bit pool; use extract_kv_blocks")
+        n, bs = len(block_indices), pool.block_size
+        host = pool._validated(_as_host_ids(block_indices))
+        first = pool.upload_ids(host).long() * bs
+        slots = (first[:, None] + torch.arange(bs, device=self.device)).flatten()
+        key, value = pool.read(slots, _DTYPES[self.dtype])
+        shape = (pool.num_layers, n, bs, pool.num_kv_heads, pool.head_dim)
+        return torch.stack([key.view(shape), value.view(shape)], dim=1)
 
     def extract_kv_blocks_many(self, block_index_lists: Sequence[List[int]]) -> List[torch.Tensor]:
         """extract_kv_blocks for several requests with one kernel launch; one tensor per request."""
@@ -204,13 +255,16 @@ class V0Worker:
         if not self.kv_cache:
             return {}
         pool = self._require_pool()
-        return {
+        layout = {
             "num_layers": pool.num_layers,
             "block_size": pool.block_size,
             "num_heads": pool.num_kv_heads,
             "head_size": pool.head_size,
             "dtype": str(pool.dtype).split(".")[-1],
         }
+        if self.kv_bits == 4:  # head_size above is a row's bytes
+            layout.update(kv_bits=4, head_dim=pool.head_dim)
+        return layout
 
     # -- vision embeddings (elasticmm/engine/v0/worker.py:1007-1060) --------------
     def init_ve_cache(self) -> None:
@@ -270,6 +324,47 @@ class V0Worker:
                                      slot_mapping: torch.Tensor) -> None:
         """Same for all layers at once; key/value are [L, T, H, D]."""
         self._require_pool().append_all_layers(key, value, slot_mapping)
+
+    # -- decode attention and token eviction (no counterpart in the reference) ----
+    def attend(self, layer: int, query: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+               scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+               max_len: Optional[int] = None) -> torch.Tensor:
+        """One decode step's attention of one layer over a 4-bit pool (KVPoolQ4.attend); after init_scores the tokens'
+        weights are gathered for evict_tokens."""
+        pool = self._require_pool()
+        if self.kv_bits != 4:
+            raise RuntimeError("attention is over a 4-bit pool (kv_bits=4); a 16-bit pool is read by the engine's own")
+        return pool.attend(layer, query, block_tables, seq_lens, scale=scale, out=out, scores=self.scores, max_len=max_len)
+
+    def init_scores(self) -> ScorePool:
+        """Starts to gather every cached token's attention weight, from zero. On a 16-bit pool the engine that computes
+        the attention adds to `scores.layers` itself."""
+        self.scores = ScorePool.like(self._require_pool())
+        return self.scores
+
+    def reset_scores(self, slot_mapping: torch.Tensor) -> None:
+        """Zeroes the weights of newly appended tokens, whose slots may have held others (all layers; once per step)."""
+        if self.scores is None:
+            raise RuntimeError("Scores not initialized (init_scores)")
+        self.scores.reset(slot_mapping)
+
+    def evict_tokens(self, block_tables: torch.Tensor, seq_lens: torch.Tensor, keep: int, recent: int = 0,
+                     sink: int = 0) -> Dict[str, Any]:
+        """Cuts every sequence to its `keep` tokens with the most weight, the first `sink` and the last `recent` among
+        them, per layer and KV head; rows and weights move to the front of the sequence's blocks. Returns
+        {"seq_lens": the new lengths (int32, on the device), "index": the kept positions}. The blocks behind
+        ceil(keep / block size) can then be freed (V0BlockManager.truncate_blocks)."""
+        pool = self._require_pool()
+        if self.scores is None:
+            raise RuntimeError("Scores not initialized (init_scores)")
+        with _range("emm.evict_tokens"):
+            try:
+                index, lens = self.scores.select_tokens(block_tables, seq_lens, keep, recent=recent, sink=sink)
+                pool.keep_tokens(index, block_tables, seq_lens)
+                self.scores.keep_tokens(index, block_tables, seq_lens)
+            except _lib.EmmError as e:
+                return {"error": str(e), "bytes": 0, "blocks": 0}
+        return {"seq_lens": lens, "index": index}
 
     def compact_blocks(self, move_src: Sequence[int], move_dst: Sequence[int]) -> Dict[str, Any]:
         """Executes a compaction plan (V0BlockManager.compact) inside the pool."""

@@ -107,3 +107,31 @@ def test_selection_by_the_restatement():
     assert got[0, 0, 0].tolist() == [0, 1, 2, 4, 5, 6]
     got = q4_oracle.select_tokens(scores, [[1, 0]], [3], 5, 2, 0)
     assert got[0, 0, 0].tolist() == [0, 1, 2, -1, -1]
+
+
+def test_configuration_of_a_4_bit_cache():
+    from elasticmm_b200.engine.v0 import V0KVCacheConfig
+    c = V0KVCacheConfig(kv_bits=4, num_kv_heads=8, dtype="bfloat16")
+    c.validate()
+    for D, row in ((64, 48), (128, 80), (256, 160)):
+        d = V0KVCacheConfig(kv_bits=4, num_kv_heads=8, head_size=D)
+        d.validate()
+        assert d.page_bytes == 16 * 8 * row == 16 * 8 * KVPoolQ4.row_bytes(D)
+    assert V0KVCacheConfig.from_dict(c.to_dict()) == c
+    for bad in (dict(kv_bits=8), dict(kv_bits=4, head_size=96), dict(kv_bits=4, dtype="float32")):
+        with pytest.raises(AssertionError):
+            V0KVCacheConfig(**bad).validate()
+
+
+def test_truncated_tables_give_their_blocks_back():
+    from elasticmm_b200.engine.v0 import Request, V0BlockManager
+    bm = V0BlockManager("decoding", 10, 0, 16)
+    bm.allocate_blocks(Request.of_length("a", 70))  # five blocks
+    assert bm.truncate_blocks("a", 33) == [3, 4] and bm.get_block_table("a") == [0, 1, 2]
+    assert bm.get_num_avail_gpu_blocks() == 7 and bm.free_gpu_blocks_list[-2:] == [3, 4]
+    assert bm.truncate_blocks("a", 48) == [] and bm.truncate_blocks("a", 1000) == []
+    assert bm.truncate_blocks("a", 0) == [0, 1, 2] and bm.get_block_table("a") == []
+    with pytest.raises(ValueError):
+        bm.truncate_blocks("b", 3)
+    with pytest.raises(ValueError):
+        bm.truncate_blocks("a", -1)
