@@ -577,6 +577,27 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
       accx[3] *= f1;
     };
 
+    // Takes the -8 s of x = o + s (c - 8) out of the value sums so far. The tensor cores cut each sum of theirs short
+    // rather than round it, by a share of its size, and sum p s c alone is much larger than what is left of it when the
+    // values have no common sign: with a fixed number of tiles between two calls the loss stays below 2^-20 of sum p s c
+    // however long the sequence (24 sequences of 2 048-4 096 tokens, fp16: the result's error 2.1e-4, that of its own
+    // rounding, instead of 3.4e-4).
+    auto recentre = [&]() {
+#pragma unroll
+      for (int r = 0; r < G; ++r) {
+        const float x0 = -8.f * __shfl_sync(0xffffffffu, accx[0], 4 * r + q4), x1 = -8.f * __shfl_sync(0xffffffffu, accx[1], 4 * r + q4);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          acc[r][i][0] = fmaf(x0, 0x1p-24f, acc[r][i][0]);
+          acc[r][i][1] = fmaf(x1, 0x1p-24f, acc[r][i][1]);
+          acc[r][i][2] = fmaf(x0, 0x1p-20f, acc[r][i][2]);
+          acc[r][i][3] = fmaf(x1, 0x1p-20f, acc[r][i][3]);
+        }
+      }
+      if (g < (uint32_t)G) accx[0] = accx[1] = 0.f;  // the scales' rows
+    };
+    constexpr uint32_t kRecentre = 16 / kT;  // slots between two calls
+
     int left = active ? (int)n - (int)(unit0 * sh.tokens + t_sub) : 0;  // tokens from this warp's next tile on
     // N tiles, the first at position n - left. kWhole: all their tokens count (mask is not read; else N = 1).
     auto tiles = [&](auto whole_tag, auto count_tag, const uint32_t base, const uint32_t mask) {
@@ -756,6 +777,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
         }
         left = next;
       }
+      if (k % kRecentre == kRecentre - 1) recentre();
       slot_before = slot;
       slot += kSlotBytes;
       if (slot == ring_end) slot = ring;
