@@ -51,7 +51,7 @@ struct AttendShape {
   uint32_t tokens;       // tokens per unit: 16 * attend_tiles(D) * subsets
   uint32_t warps;        // heads_cta * ntiles * subsets
   uint32_t stages;       // tiles in a warp's ring
-  int32_t block_shift;   // log2 of the block size where it is a power of two >= 16 (a tile lies in one block), else -1
+  int32_t block_shift;   // log2 of the block size where it is a power of two, else -1
   uint32_t grid;         // CTAs
   uint32_t items;        // num_seqs * head_groups
 };
@@ -234,7 +234,8 @@ __host__ __device__ constexpr int attend_stages(int D) { return D == 64 ? 6 : 4;
 __host__ __device__ constexpr int attend_slot_bytes(int D) { return attend_tiles(D) * 32 * q4_row_bytes(D) + 16; }
 
 // Decode attention; see the top of the file. kPrecise: carry the remainder of p s_r (fp16 outputs).
-template <typename T, int D, bool kScores>
+// kPages: blocks of 2^k >= 16 tokens (sh.block_shift >= 4), so that a tile lies in one.
+template <typename T, int D, bool kScores, bool kPages>
 __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_constant__ AttendArgs a) {
   constexpr int G = q4_groups(D), R = q4_row_bytes(D);
   constexpr int KW = D / 32;  // words of codes per lane and token, keys (two units of every group)
@@ -319,7 +320,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
   }
   const uint32_t tail_lane = R % 32 == 0 || lane < R % 32;  // has a chunk in the last, partial round
   const uint32_t shift = (uint32_t)sh.block_shift & 31u, block_mask = (1u << shift) - 1u;
-  const bool paged = sh.block_shift >= 0;
+  const bool paged = kPages || sh.block_shift >= 0;
   bool holes = false;              // a block outside the pool was met
   // Where the next slot's tokens lie. `run` slots from here on hold whole tiles of one block each, their blocks at hand
   // in `ids`; `after` more units of the item follow in the share.
@@ -354,30 +355,54 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
     it = t_sub;
     enter();
   };
+  bool small = false;              // the next slot's tiles are whole, of blocks of less than 16 tokens in `ids`
   auto begin_run = [&]() {
+    small = false;
     if (!paged || !ireal || it + 16 * kT > in) return;
-    if ((it >> shift) - window >= 32) {  // a unit has at most 256 tokens, 16 blocks
-      window += 32;
-      ids = ids_next;
+    const uint32_t far = (it >> shift) - window;
+    if (far >= 32) {
+      if (kPages || far < 64) {  // a unit has at most 256 tokens: 32 blocks of 8
+        window += 32;
+        ids = ids_next;
+      } else {
+        window = it >> shift;
+        ids = entry(window);
+      }
       ids_next = entry(window + 32);
     }
     if (__any_sync(0xffffffffu, (uint32_t)ids >= a.pool.num_blocks)) return;
-    // `it` is a multiple of 16 kT and so is a block, or a pair of blocks: a slot's tiles lie in the same window
+    // slots begin at multiples of 16 kT tokens, so a slot's blocks (32 at most) lie in one window
+    if (!kPages && shift < 4) {
+      small = true;
+      return;
+    }
     const uint32_t whole = (in - it - 16 * kT) / sh.tokens + 1;
     const uint32_t known = (uint32_t)((((uint64_t)window + 32) << shift) - it + sh.tokens - 1) / sh.tokens;
     run = min(min(whole, known), after);
     after -= run;
   };
-  // Tiles that are not 16 tokens of one block: the end of a sequence, a block outside the pool, other block sizes.
+  // Tiles of smaller blocks, and those that are not 16 tokens, not all inside the pool or of blocks of no 2^k tokens.
   auto load_rest = [&](uint32_t slot) {
 #pragma unroll 1
     for (uint32_t i = 0; i < kT; ++i) {
       const uint32_t t = it + 16 * i, to = slot + i * kTile;
       uint32_t word = kByLength;
-      if (t < in && ireal) {
+      if (!kPages && small) {
+#pragma unroll
+        for (int j = 0; j < kCopies; ++j) {
+          const uint32_t c = min(lane + 32 * j, (uint32_t)(16 * kChunks - 1)), at = t + c / kChunks;
+          const uint32_t id = (uint32_t)__shfl_sync(0xffffffffu, ids, (at >> shift) - window);
+          const uint64_t k = ibase + (uint64_t)id * (uint32_t)a.pool.block_stride +
+                             (uint64_t)(at & block_mask) * (uint32_t)a.pool.token_stride + c % kChunks * 16;
+          if (lane + 32 * j < 16 * kChunks) {
+            copy16(to + 16 * c, k);
+            copy16(to + 16 * R + 16 * c, k + a.pool.plane_stride);
+          }
+        }
+      } else if (t < in && ireal) {
         const uint32_t count = min(16u, in - t);
         auto row_at = [&](uint32_t row) -> uint64_t {
-          const uint32_t blk = (t + row) / a.pool.block_size;
+          const uint32_t blk = kPages ? (t + row) >> shift : (t + row) / a.pool.block_size;
           const int32_t id = itab[blk];
           if ((uint32_t)id >= a.pool.num_blocks) {
             report(a.status, kStatusIdRange, id);
@@ -408,10 +433,10 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
     for (int i = 0; i < kT; ++i) sts_word<kWords>(slot + 4 * i, kByLength);
   };
   auto load = [&](uint32_t slot) {
-    if (run == 0 && after > 0) {
+    if (__builtin_expect(run == 0 && after > 0, 0)) {
       begin_run();
       if (run == 0) load_rest(slot);
-    } else if (run > 0 && holes) {
+    } else if (__builtin_expect(run > 0 && holes, 0)) {
       by_length(slot);
     }
     if (run > 0) {
@@ -424,7 +449,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
         copy_tile<R, 0>(slot + i * kTile + 16 * lane, k, k + a.pool.plane_stride, row_off, tail_lane);
       }
       it += sh.tokens;
-      if (--run == 0 && after == 0) next_item();
+      if (__builtin_expect(--run == 0, 0) && after == 0) next_item();
     }
     copies_commit();  // an empty group at the end keeps the count
   };
@@ -696,7 +721,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
         }
       }
       const bool lower = (big & scale_bits) != 0 && lift > 0.f;
-      if (__any_sync(0xffffffffu, most > lift + 6.f || lower)) {
+      if (__builtin_expect(__any_sync(0xffffffffu, most > lift + 6.f || lower), 0)) {
         if (__any_sync(0xffffffffu, lower)) {
           rescale(ref0 == kFirstRef ? ref0 : ref0 + lift + 4.f, ref1 == kFirstRef ? ref1 : ref1 + lift + 4.f);
           lift = -4.f;
@@ -763,7 +788,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
       copies_wait<kAttendStages - 2>();
       __syncwarp();  // this slot's rows are there for every lane, and every lane has left the slot before
       load(slot_before);
-      if (left >= 16 * kT && !holes) {
+      if (__builtin_expect(left >= 16 * kT && !holes, 1)) {
         tiles(std::true_type{}, std::integral_constant<int, kT>{}, slot, 0xffffu);
         left -= (int)sh.tokens;
       } else {

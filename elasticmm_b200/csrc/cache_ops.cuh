@@ -163,7 +163,6 @@ int attend_shape(const emm_pool *pool, int32_t D, int32_t B, int32_t group, int3
   s.warps = s.heads_cta * s.ntiles * s.subsets;
   // A tile's offsets within a block take 32 bits.
   s.block_shift = d.token_stride < 1 << 27 && d.block_stride <= 0xffffffffll ? shift_of(d.block_size) : -1;
-  if (s.block_shift < 4) s.block_shift = -1;
   s.stages = (uint32_t)emm::attend_stages(D);
   const int merge = (int)((s.subsets - 1) * s.heads_cta * s.ntiles * 8 * (uint32_t)(D + 2) * 4);
   *smem_out = (int)(s.warps * s.stages * (uint32_t)emm::attend_slot_bytes(D)) + merge;
@@ -199,34 +198,32 @@ AttendWorkspace attend_workspace(const emm::AttendShape &s, int32_t D, int32_t B
   return w;
 }
 
-// The kernel's dynamic shared memory is raised to the device's limit once per device.
-template <typename T, int D, bool kScores>
-int attend_smem(int device, int smem) {
+// Launches the main kernel; its dynamic shared memory is raised to the device's limit once per device.
+template <typename T, int D, bool kScores, bool kPages>
+int attend_main(emm_ctx *ctx, const emm::AttendArgs &a, int smem, cudaStream_t st) {
+  const int device = ctx->device;
   static std::atomic<int> limit[kMaxTrackedDevices];
   const bool tracked = device >= 0 && device < kMaxTrackedDevices;
-  if (tracked && limit[device].load(std::memory_order_acquire) >= smem) return EMM_OK;
-  int most = 0;
-  EMM_CUDA(cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, device));
-  cudaFuncAttributes fa;
-  EMM_CUDA(cudaFuncGetAttributes(&fa, emm::attend_q4<T, D, kScores>));
-  most -= (int)fa.sharedSizeBytes;
-  if (smem > most) return fail(EMM_ERR_TOO_LARGE, "q4_attend: %d bytes of shared memory, the device has %d", smem, most);
-  EMM_CUDA(cudaFuncSetAttribute(emm::attend_q4<T, D, kScores>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-  if (tracked) limit[device].store(most, std::memory_order_release);
+  if (!tracked || limit[device].load(std::memory_order_acquire) < smem) {
+    cudaFuncAttributes fa;
+    EMM_CUDA(cudaFuncGetAttributes(&fa, emm::attend_q4<T, D, kScores, kPages>));
+    const int most = ctx->max_smem_optin - (int)fa.sharedSizeBytes;
+    if (smem > most) return fail(EMM_ERR_TOO_LARGE, "q4_attend: %d bytes of shared memory, the device has %d", smem, most);
+    EMM_CUDA(cudaFuncSetAttribute(emm::attend_q4<T, D, kScores, kPages>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    if (tracked) limit[device].store(most, std::memory_order_release);
+  }
+  emm::attend_q4<T, D, kScores, kPages><<<a.sh.grid, a.sh.warps * 32, smem, st>>>(a);
+  EMM_CUDA(cudaGetLastError());
+  ctx->launches += 1;
   return EMM_OK;
 }
 
 template <typename T, int D>
 int attend_launch(emm_ctx *ctx, const emm::AttendArgs &a, int smem, cudaStream_t st) {
-  if (a.score_base) {
-    if (int rc = attend_smem<T, D, true>(ctx->device, smem)) return rc;
-    emm::attend_q4<T, D, true><<<a.sh.grid, a.sh.warps * 32, smem, st>>>(a);
-  } else {
-    if (int rc = attend_smem<T, D, false>(ctx->device, smem)) return rc;
-    emm::attend_q4<T, D, false><<<a.sh.grid, a.sh.warps * 32, smem, st>>>(a);
-  }
-  EMM_CUDA(cudaGetLastError());
-  ctx->launches += 1;
+  const bool pages = a.sh.block_shift >= 4;
+  const int rc = a.score_base ? (pages ? attend_main<T, D, true, true>(ctx, a, smem, st) : attend_main<T, D, true, false>(ctx, a, smem, st))
+                              : (pages ? attend_main<T, D, false, true>(ctx, a, smem, st) : attend_main<T, D, false, false>(ctx, a, smem, st));
+  if (rc) return rc;
   // The two small kernels behind it are placed while it drains.
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

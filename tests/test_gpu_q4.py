@@ -271,7 +271,8 @@ LENS = [0, 1, 15, 16, 17, 33, 64, 255, 700]
 @pytest.mark.parametrize("hnd", [False, True], ids=["nhd", "hnd"])
 @pytest.mark.parametrize("D,H,group,BS,dtype", [
     (128, 4, 7, 16, BF), (128, 8, 8, 16, FP), (128, 3, 1, 16, FP), (64, 8, 4, 16, BF), (64, 5, 2, 8, FP), (256, 2, 3, 32, BF),
-    (256, 1, 16, 16, FP), (128, 1, 64, 16, BF), (128, 2, 9, 5, BF), (64, 12, 1, 1, FP), (128, 9, 5, 48, FP)])
+    (256, 1, 16, 16, FP), (128, 1, 64, 16, BF), (128, 2, 9, 5, BF), (64, 12, 1, 1, FP), (128, 9, 5, 48, FP),
+    (128, 8, 2, 8, BF), (256, 2, 8, 8, FP), (128, 2, 4, 2, BF), (256, 1, 2, 1, BF), (128, 1, 8, 4, FP), (128, 4, 8, 64, BF)])
 def test_attend(ctx, D, H, group, BS, dtype, hnd):
     NB = sum(-(-n // BS) for n in LENS) + 3
     pool, bytes_ = random_pool(2, NB, BS, H, D, hnd, D + H)
