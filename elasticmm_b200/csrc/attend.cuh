@@ -251,6 +251,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
   const AttendShape &sh = a.sh;
   const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   grid_launch_dependents();
+  grid_dependency_wait();
   if (tid == 0) a.cta_item[blockIdx.x] = -1;
   // The line's length and this CTA's piece. A thread takes a run of consecutive sequences.
   {

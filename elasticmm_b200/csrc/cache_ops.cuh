@@ -7,6 +7,25 @@
 
 namespace {
 
+// Launches with programmatic stream serialisation (EMM_OPT_PDL): placed while the kernel before it in the stream drains.
+// Every kernel here waits for that one to complete before its first global access.
+template <typename... Params, typename... Args>
+int launch_after(emm_ctx *ctx, void (*kernel)(Params...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, const Args &...args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctx->pdl ? 1 : 0;
+  EMM_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+  ctx->launches += 1;
+  return EMM_OK;
+}
+
 bool q4_dim(int32_t D) { return D == 64 || D == 128 || D == 256; }
 
 // A pool whose rows are 4-bit rows of head_dim channels, in this GPU's memory, every row on a 16-byte boundary.
@@ -113,16 +132,13 @@ int q4_rows_impl(emm_pool *pool, bool append, int32_t D, int32_t dtype, int32_t 
   if (!guard.ok()) return fail(EMM_ERR_CUDA, "cannot select device %d", pool->ctx->device);
   const dim3 grid((unsigned)blocks, (unsigned)layer_count * 2);
   cudaStream_t st = (cudaStream_t)stream;
-#define EMM_Q4_ROWS(T_, D_)                                                                     \
-  do {                                                                                          \
-    if (append) {                                                                               \
-      if (wide) emm::q4_append_rows<T_, D_><<<grid, emm::kRowWarps * 32, 0, st>>>(a);           \
-      else emm::q4_append_units<T_, D_><<<grid, 256, 0, st>>>(a);                               \
-    } else {                                                                                    \
-      if (wide) emm::q4_read_rows<T_, D_><<<grid, emm::kRowWarps * 32, 0, st>>>(a);             \
-      else emm::q4_read_units<T_, D_><<<grid, 256, 0, st>>>(a);                                 \
-    }                                                                                           \
-  } while (0)
+  emm_ctx *ctx = pool->ctx;
+  const unsigned block = wide ? emm::kRowWarps * 32 : 256;
+#define EMM_Q4_ROWS(T_, D_)                                                                                    \
+  return append ? launch_after(ctx, wide ? emm::q4_append_rows<T_, D_> : emm::q4_append_units<T_, D_>, grid,   \
+                               block, 0, st, a)                                                                \
+                : launch_after(ctx, wide ? emm::q4_read_rows<T_, D_> : emm::q4_read_units<T_, D_>, grid, block, \
+                               0, st, a)
   if (dtype == EMM_DTYPE_FP16) {
     if (D == 64) EMM_Q4_ROWS(__half, 64);
     else if (D == 128) EMM_Q4_ROWS(__half, 128);
@@ -133,9 +149,6 @@ int q4_rows_impl(emm_pool *pool, bool append, int32_t D, int32_t dtype, int32_t 
     else EMM_Q4_ROWS(__nv_bfloat16, 256);
   }
 #undef EMM_Q4_ROWS
-  EMM_CUDA(cudaGetLastError());
-  pool->ctx->launches += 1;
-  return EMM_OK;
 }
 
 // How a call's work is laid out; see attend.cuh. A rule on heads and strides only.
@@ -212,10 +225,7 @@ int attend_main(emm_ctx *ctx, const emm::AttendArgs &a, int smem, cudaStream_t s
     EMM_CUDA(cudaFuncSetAttribute(emm::attend_q4<T, D, kScores, kPages>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     if (tracked) limit[device].store(most, std::memory_order_release);
   }
-  emm::attend_q4<T, D, kScores, kPages><<<a.sh.grid, a.sh.warps * 32, smem, st>>>(a);
-  EMM_CUDA(cudaGetLastError());
-  ctx->launches += 1;
-  return EMM_OK;
+  return launch_after(ctx, emm::attend_q4<T, D, kScores, kPages>, dim3(a.sh.grid), a.sh.warps * 32, (size_t)smem, st, a);
 }
 
 template <typename T, int D>
@@ -224,35 +234,20 @@ int attend_launch(emm_ctx *ctx, const emm::AttendArgs &a, int smem, cudaStream_t
   const int rc = a.score_base ? (pages ? attend_main<T, D, true, true>(ctx, a, smem, st) : attend_main<T, D, true, false>(ctx, a, smem, st))
                               : (pages ? attend_main<T, D, false, true>(ctx, a, smem, st) : attend_main<T, D, false, false>(ctx, a, smem, st));
   if (rc) return rc;
-  // The two small kernels behind it are placed while it drains.
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = ctx->pdl ? 1 : 0;
   if (a.sh.grid > 1) {  // one CTA splits nothing
     const bool by_cta = a.sh.items > a.sh.grid;
     const uint32_t rows = a.sh.heads_cta * a.group, x = by_cta ? a.sh.grid : a.sh.items;
-    cfg.blockDim = dim3(emm::kJoinWarps * 32);
     // Where items are few an item has many parts, and a head needs all warps of a block; else two.
-    if (x * 8 <= a.sh.grid) {
-      cfg.gridDim = dim3(x, rows);
-      EMM_CUDA(cudaLaunchKernelEx(&cfg, emm::attend_join<T, D, 1>, a, (uint32_t)by_cta));
-    } else {
-      cfg.gridDim = dim3(x, (rows + 7) / 8);
-      EMM_CUDA(cudaLaunchKernelEx(&cfg, emm::attend_join<T, D, 8>, a, (uint32_t)by_cta));
-    }
-    ctx->launches += 1;
+    const bool many = x * 8 <= a.sh.grid;
+    if (int rc2 = launch_after(ctx, many ? emm::attend_join<T, D, 1> : emm::attend_join<T, D, 8>,
+                               dim3(x, many ? rows : (rows + 7) / 8), emm::kJoinWarps * 32, 0, st, a, (uint32_t)by_cta))
+      return rc2;
   }
   if (a.score_base && a.max_len > 0) {
     const uint32_t chunks = (a.max_len + emm::kScoreTokens - 1) / emm::kScoreTokens;
     const uint64_t turns = (uint64_t)a.num_seqs * a.kv_heads * chunks;
-    cfg.gridDim = dim3((unsigned)std::min<uint64_t>((turns + 7) / 8, (uint64_t)ctx->sm_count * 6));
-    cfg.blockDim = dim3(256);
-    EMM_CUDA(cudaLaunchKernelEx(&cfg, emm::attend_scores, a, chunks));
-    ctx->launches += 1;
+    const unsigned grid = (unsigned)std::min<uint64_t>((turns + 7) / 8, (uint64_t)ctx->sm_count * 6);
+    return launch_after(ctx, emm::attend_scores, dim3(grid), 256, 0, st, a, chunks);
   }
   return EMM_OK;
 }
@@ -415,21 +410,13 @@ int emm_select_tokens(emm_pool *scores, const int32_t *d_block_tables, int64_t t
   const dim3 grid((unsigned)num_seqs * (unsigned)d.block_size, (unsigned)d.num_layers);
   const int64_t most = (int64_t)table_width * d.head_size;
   cudaStream_t st = (cudaStream_t)stream;
-  if (most * 4 <= kSelectSharedMax) {
-    if (most <= 4096) {
-      emm::select_tokens<256, true><<<grid, 256, (size_t)most * 4, st>>>(a);
-    } else if (most <= 11264) {  // 44 KB: fits the default limit
-      emm::select_tokens<512, true><<<grid, 512, (size_t)most * 4, st>>>(a);
-    } else {
-      EMM_CUDA(cudaFuncSetAttribute(emm::select_tokens<1024, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectSharedMax));
-      emm::select_tokens<1024, true><<<grid, 1024, (size_t)most * 4, st>>>(a);
-    }
-  } else {
-    emm::select_tokens<1024, false><<<grid, 1024, 0, st>>>(a);
-  }
-  EMM_CUDA(cudaGetLastError());
-  scores->ctx->launches += 1;
-  return EMM_OK;
+  emm_ctx *ctx = scores->ctx;
+  if (most * 4 > kSelectSharedMax) return launch_after(ctx, emm::select_tokens<1024, false>, grid, 1024, 0, st, a);
+  const size_t keys = (size_t)most * 4;
+  if (most <= 4096) return launch_after(ctx, emm::select_tokens<256, true>, grid, 256, keys, st, a);
+  if (most <= 11264) return launch_after(ctx, emm::select_tokens<512, true>, grid, 512, keys, st, a);  // 44 KB: the default limit
+  EMM_CUDA(cudaFuncSetAttribute(emm::select_tokens<1024, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectSharedMax));
+  return launch_after(ctx, emm::select_tokens<1024, true>, grid, 1024, keys, st, a);
 }
 
 int emm_keep_tokens(emm_pool *pool, const int32_t *d_index, int32_t index_heads, int32_t keep,
@@ -493,20 +480,15 @@ int emm_keep_tokens(emm_pool *pool, const int32_t *d_index, int32_t index_heads,
   const bool plain = a.row_bytes / vec <= (uint32_t)emm::kKeepThreads && a.pool.block_shift >= 0 &&
                      std::max(a.pool.block_stride, a.pool.token_stride) <= 0xffffffffull &&
                      (uint64_t)keep < (1ull << 31) - 64 * emm::kKeepThreads;
-#define EMM_KEEP(V_)                                                                  \
-  do {                                                                                \
-    if (plain) emm::keep_rows<V_, true><<<grid, emm::kKeepThreads, 0, st>>>(a);       \
-    else emm::keep_rows<V_, false><<<grid, emm::kKeepThreads, 0, st>>>(a);            \
-  } while (0)
+  emm_ctx *ctx = pool->ctx;
+#define EMM_KEEP(V_) \
+  return launch_after(ctx, plain ? emm::keep_rows<V_, true> : emm::keep_rows<V_, false>, grid, emm::kKeepThreads, 0, st, a)
   if (vec >= 16) EMM_KEEP(uint4);
-  else if (vec >= 8) EMM_KEEP(uint2);
-  else if (vec >= 4) EMM_KEEP(uint32_t);
-  else if (vec >= 2) EMM_KEEP(uint16_t);
-  else EMM_KEEP(uint8_t);
+  if (vec >= 8) EMM_KEEP(uint2);
+  if (vec >= 4) EMM_KEEP(uint32_t);
+  if (vec >= 2) EMM_KEEP(uint16_t);
+  EMM_KEEP(uint8_t);
 #undef EMM_KEEP
-  EMM_CUDA(cudaGetLastError());
-  pool->ctx->launches += 1;
-  return EMM_OK;
 }
 
 int emm_reset_scores(emm_pool *scores, const int64_t *d_slot_mapping, int32_t num_tokens, void *stream) {
@@ -521,12 +503,9 @@ int emm_reset_scores(emm_pool *scores, const int64_t *d_slot_mapping, int32_t nu
   if (blocks > 0x7fffffffull || d.num_layers > 65535) return fail(EMM_ERR_TOO_LARGE, "%s: %d tokens", what, num_tokens);
   DeviceGuard guard(scores->ctx->device);
   if (!guard.ok()) return fail(EMM_ERR_CUDA, "cannot select device %d", scores->ctx->device);
-  emm::reset_scores<<<dim3((unsigned)blocks, (unsigned)d.num_layers), 256, 0, (cudaStream_t)stream>>>(
-      scores->d_layers, (uint64_t)d.block_stride, (uint32_t)d.num_blocks, (uint32_t)d.head_size, (uint32_t)d.block_size,
-      d_slot_mapping, (uint64_t)num_tokens, scores->ctx->d_status);
-  EMM_CUDA(cudaGetLastError());
-  scores->ctx->launches += 1;
-  return EMM_OK;
+  return launch_after(scores->ctx, emm::reset_scores, dim3((unsigned)blocks, (unsigned)d.num_layers), 256, 0,
+                      (cudaStream_t)stream, (const uint64_t *)scores->d_layers, (uint64_t)d.block_stride, (uint32_t)d.num_blocks,
+                      (uint32_t)d.head_size, (uint32_t)d.block_size, d_slot_mapping, (uint64_t)num_tokens, scores->ctx->d_status);
 }
 
 }  // extern "C"

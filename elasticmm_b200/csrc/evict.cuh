@@ -42,6 +42,8 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 // barriers. So a digit is found by one warp, bins are cleared a pass ahead, and the index leaves after one more barrier.
 template <int kThreads, bool kShared>
 __global__ void __launch_bounds__(kThreads) select_tokens(const __grid_constant__ SelectArgs a) {
+  grid_launch_dependents();
+  grid_dependency_wait();
   constexpr int kWarps = kThreads / 32, kAhead = 8;
   extern __shared__ uint32_t keys[];  // kShared: one per position
   __shared__ uint32_t hist[2][256];
@@ -209,6 +211,8 @@ constexpr int kKeepThreads = 256, kKeepAhead = 4, kKeepStages = 3;
 
 template <typename V, bool kPlain>
 __global__ void __launch_bounds__(kKeepThreads) keep_rows(const __grid_constant__ KeepArgs a) {
+  grid_launch_dependents();
+  grid_dependency_wait();
   using Pos = typename std::conditional<kPlain, uint32_t, uint64_t>::type;
   __shared__ __align__(16) V ring[kKeepStages][kKeepAhead][kKeepThreads];
   const uint32_t piece = blockIdx.x % a.splits, pbh = blockIdx.x / a.splits;
@@ -316,6 +320,8 @@ __global__ void __launch_bounds__(kKeepThreads) keep_rows(const __grid_constant_
 __global__ void __launch_bounds__(256)
 reset_scores(const uint64_t *layers, uint64_t block_stride, uint32_t num_blocks, uint32_t block_size, uint32_t heads,
              const int64_t *slots, uint64_t num_tokens, int *status) {
+  grid_launch_dependents();
+  grid_dependency_wait();
   const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= num_tokens * heads) return;
   const uint64_t t = i / heads;

@@ -179,6 +179,8 @@ __device__ __noinline__ void encode_exact(uint64_t src, float s, float o, uint8_
 // grid.x * kRowWarps warps cover the T * H rows, 32 / (D/32) of them each; grid.y the layers and planes.
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowWarps * 32) q4_append_rows(const __grid_constant__ Q4RowsArgs a) {
+  grid_launch_dependents();
+  grid_dependency_wait();
   constexpr int G = q4_groups(D), R = q4_row_bytes(D), kRows = 32 / G, kPieces = kRows * R / 16;
   __shared__ __align__(16) uint8_t stage[kRowWarps][kRows * R];
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane % G;
@@ -259,6 +261,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) q4_append_rows(const __grid_co
 // The inverse: o + s * (c - 8), rounded once to T. A padding or reported slot gives a row of zeros.
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowWarps * 32) q4_read_rows(const __grid_constant__ Q4RowsArgs a) {
+  grid_launch_dependents();
+  grid_dependency_wait();
   constexpr int G = q4_groups(D), R = q4_row_bytes(D), kRows = 32 / G, kPieces = kRows * R / 16;
   __shared__ __align__(16) uint8_t stage[kRowWarps][kRows * R];
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane % G;
@@ -305,6 +309,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) q4_read_rows(const __grid_cons
 // of a group find its smallest and largest value by shuffles. grid.x * 256 threads cover T * H * D/4 units.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) q4_append_units(const __grid_constant__ Q4RowsArgs a) {
+  grid_launch_dependents();
+  grid_dependency_wait();
   constexpr uint32_t kUnits = D / 4, G = q4_groups(D);
   const uint64_t idx = (uint64_t)blockIdx.x * 256 + threadIdx.x;
   const uint32_t unit = (uint32_t)(idx % kUnits);
@@ -367,6 +373,8 @@ __global__ void __launch_bounds__(256) q4_append_units(const __grid_constant__ Q
 
 template <typename T, int D>
 __global__ void __launch_bounds__(256) q4_read_units(const __grid_constant__ Q4RowsArgs a) {
+  grid_launch_dependents();
+  grid_dependency_wait();
   constexpr uint32_t kUnits = D / 4, G = q4_groups(D);
   const uint64_t idx = (uint64_t)blockIdx.x * 256 + threadIdx.x;
   const uint32_t unit = (uint32_t)(idx % kUnits);
