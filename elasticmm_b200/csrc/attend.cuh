@@ -86,6 +86,7 @@ struct AttendArgs {
   int *cta_item;              // [grid]: the split item that this CTA finished, or -1
   float *lse;                 // [B, Hq], with scores
   float *logits;              // [B, Hq, logit_stride], with scores
+  uint32_t *longest;          // the batch's largest length, with scores
   uint64_t logit_stride;
   int *status;
 };
@@ -214,7 +215,7 @@ constexpr uint32_t kNib0 = 0x000f000fu, kNib1 = 0x00f000f0u;
 // prmt selectors, from two words: their low (high) halves; those halves shifted down by eight bits, with bits above that
 // the nibble masks drop
 constexpr uint32_t kLoHalves = 0x5410u, kHiHalves = 0x7632u, kLoUpper = 0x5511u, kHiUpper = 0x7733u;
-constexpr float kFirstRef = -1e30f;                            // reference before any token
+constexpr float kFirstRef = -3.40282347e38f;                  // reference before any token: no finite logit is less
 
 // A CTA's share. The batch is a line on which every item takes kItemCost and then one place per unit; a CTA has the units
 // whose places lie in its piece of the line.
@@ -246,7 +247,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
   constexpr int kTile = 32 * R, kWords = kT * kTile;  // bytes of a tile; where a slot's words begin
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Share share;
-  __shared__ uint32_t scan[kAttendWarps];
+  __shared__ uint32_t scan[kAttendWarps], tops[kAttendWarps];
 
   const AttendShape &sh = a.sh;
   const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -257,10 +258,11 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
   {
     const uint32_t per = (a.num_seqs + blockDim.x - 1) / blockDim.x;
     const uint32_t b0 = min(a.num_seqs, tid * per), b1 = min(a.num_seqs, b0 + per);
-    uint32_t mine = 0, n0 = 0;
+    uint32_t mine = 0, n0 = 0, top = 0;
     for (uint32_t b = b0; b < b1; ++b) {
       const uint32_t n = seq_length(a, b, blockIdx.x == 0);
       if (b == b0) n0 = n;
+      top = max(top, n);
       mine += (seq_units(a, n) + kItemCost) * sh.head_groups;
     }
     uint32_t upto = mine;
@@ -270,6 +272,10 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
       if (lane >= m) upto += other;
     }
     if (lane == 31) scan[warp] = upto;
+    if constexpr (kScores) {
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) tops[warp] = top;
+    }
     __syncthreads();
     uint32_t before = 0, total = 0;
     for (uint32_t w = 0; w < blockDim.x / 32; ++w) {
@@ -277,6 +283,10 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
       total += scan[w];
     }
     before += upto - mine;
+    if constexpr (kScores) {
+      for (uint32_t w = 0; w < blockDim.x / 32; ++w) top = max(top, tops[w]);
+      if (blockIdx.x == 0 && tid == 0) *a.longest = top;
+    }
     const uint32_t each = total / gridDim.x, extra = total - each * gridDim.x;
     const uint32_t first = each * blockIdx.x + min(blockIdx.x, extra);
     if (first >= total && tid == 0) share = Share{0, 0, 0, 0, 0, 0, 0};  // more CTAs than places
@@ -1031,15 +1041,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join(const __grid_cons
 }
 
 // Adds every token's weight to its score. A warp's turn is 128 tokens of a (sequence, KV head) pair, four a lane; turns go
-// chunk by chunk over all pairs, so that long and short sequences are spread over all warps. Nothing here needs the
+// chunk by chunk over all pairs up to the batch's largest length (max_len may be far more), so that long and short
+// sequences are spread over all warps. Nothing here needs the
 // latency hidden better than by many warps with few registers.
 constexpr uint32_t kScoreTokens = 128;
 
-__global__ void __launch_bounds__(256, 6) attend_scores(const __grid_constant__ AttendArgs a, const uint32_t chunks) {
+__global__ void __launch_bounds__(256, 6) attend_scores(const __grid_constant__ AttendArgs a) {
   grid_launch_dependents();
   grid_dependency_wait();
   const uint32_t lane = threadIdx.x % 32, pairs = a.num_seqs * a.kv_heads;
-  const uint64_t total = (uint64_t)pairs * chunks, step = (uint64_t)gridDim.x * 8;
+  const uint64_t total = (uint64_t)pairs * ((*a.longest + kScoreTokens - 1) / kScoreTokens), step = (uint64_t)gridDim.x * 8;
   for (uint64_t i = (uint64_t)blockIdx.x * 8 + threadIdx.x / 32; i < total; i += step) {
     const uint32_t c = (uint32_t)(i / pairs), bh = (uint32_t)(i - (uint64_t)c * pairs), b = bh / a.kv_heads, h = bh - b * a.kv_heads;
     const uint32_t n = seq_length(a, b, false), t = c * kScoreTokens + lane * 4;

@@ -187,7 +187,7 @@ int attend_shape(const emm_pool *pool, int32_t D, int32_t B, int32_t group, int3
 }
 
 struct AttendWorkspace {
-  uint64_t part_o, part_ml, item_span, cta_item, lse, logits, logit_stride, bytes;
+  uint64_t part_o, part_ml, item_span, cta_item, lse, longest, logits, logit_stride, bytes;
 };
 
 AttendWorkspace attend_workspace(const emm::AttendShape &s, int32_t D, int32_t B, int32_t Hq, int32_t group, int32_t max_len,
@@ -205,6 +205,7 @@ AttendWorkspace attend_workspace(const emm::AttendShape &s, int32_t D, int32_t B
   w.item_span = take((uint64_t)s.items * 8);
   w.cta_item = take((uint64_t)s.grid * 4);
   w.lse = take(scores ? (uint64_t)B * Hq * 4 : 0);
+  w.longest = take(scores ? 4 : 0);
   w.logit_stride = ((uint64_t)max_len + 7) / 8 * 8;
   w.logits = take(scores ? (uint64_t)B * Hq * w.logit_stride * 4 : 0);
   w.bytes = at;
@@ -247,7 +248,7 @@ int attend_launch(emm_ctx *ctx, const emm::AttendArgs &a, int smem, cudaStream_t
     const uint32_t chunks = (a.max_len + emm::kScoreTokens - 1) / emm::kScoreTokens;
     const uint64_t turns = (uint64_t)a.num_seqs * a.kv_heads * chunks;
     const unsigned grid = (unsigned)std::min<uint64_t>((turns + 7) / 8, (uint64_t)ctx->sm_count * 6);
-    return launch_after(ctx, emm::attend_scores, dim3(grid), 256, 0, st, a, chunks);
+    return launch_after(ctx, emm::attend_scores, dim3(grid), 256, 0, st, a);
   }
   return EMM_OK;
 }
@@ -305,7 +306,7 @@ int emm_q4_attend(emm_pool *pool, int32_t head_dim, int32_t dtype, int32_t layer
   if (max_len < 0 || (int64_t)max_len > (int64_t)table_width * d.block_size)
     return fail(EMM_ERR_LENGTH, "%s: max_len %d needs more than %d blocks of %d tokens", what, max_len, table_width,
                 d.block_size);
-  if (!(scale - scale == 0.0)) return fail(EMM_ERR_BAD_ARG, "%s: the scale is not finite", what);
+  if (!(std::fabs(scale) <= 1e38)) return fail(EMM_ERR_BAD_ARG, "%s: the scale is not finite in 32 bits", what);
   if (scores) {
     if (int rc = check_score_pool(scores, what)) return rc;
     if (scores->ctx != pool->ctx) return fail(EMM_ERR_BAD_ARG, "%s: pools of different contexts", what);
@@ -357,6 +358,7 @@ int emm_q4_attend(emm_pool *pool, int32_t head_dim, int32_t dtype, int32_t layer
   a.item_span = (int2 *)(ws + w.item_span);
   a.cta_item = (int *)(ws + w.cta_item);
   a.lse = (float *)(ws + w.lse);
+  a.longest = (uint32_t *)(ws + w.longest);
   a.logits = (float *)(ws + w.logits);
   a.logit_stride = w.logit_stride;
   a.status = pool->ctx->d_status;

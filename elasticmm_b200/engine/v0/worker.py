@@ -338,7 +338,8 @@ class V0Worker:
 
     def init_scores(self) -> ScorePool:
         """Starts to gather every cached token's attention weight, from zero. On a 16-bit pool the engine that computes
-        the attention adds to `scores.layers` itself."""
+        the attention adds to `scores.layers` itself. Weights follow evict_tokens and compact_blocks; where blocks are
+        swapped or go to another worker, the caller moves theirs (`scores.gather`, `scores.scatter`)."""
         self.scores = ScorePool.like(self._require_pool())
         return self.scores
 
@@ -367,10 +368,12 @@ class V0Worker:
         return {"seq_lens": lens, "index": index}
 
     def compact_blocks(self, move_src: Sequence[int], move_dst: Sequence[int]) -> Dict[str, Any]:
-        """Executes a compaction plan (V0BlockManager.compact) inside the pool."""
+        """Executes a compaction plan (V0BlockManager.compact) inside the pool; the blocks' weights move along."""
         pool = self._require_pool()
         try:
             pool.copy_blocks(pool, move_src, move_dst)
+            if self.scores is not None:
+                self.scores.copy_blocks(self.scores, move_src, move_dst)
         except _lib.EmmError as e:
             return {"error": str(e), "bytes": 0, "blocks": 0}
         return {"bytes": len(move_src) * pool.block_bytes(), "blocks": len(move_src)}

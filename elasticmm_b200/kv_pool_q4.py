@@ -20,6 +20,13 @@ from .kv_pool import Context, KVPool, _stream_ptr, check_block_tables
 
 _DTYPES = {torch.float16: _lib.DTYPE_FP16, torch.bfloat16: _lib.DTYPE_BF16}
 _MAX_SIGNATURES = 64
+_INT32_MAX = 0x7FFFFFFF
+
+
+def _remember(cache: Dict[tuple, tuple], sig: tuple, got: tuple) -> None:
+    if len(cache) >= _MAX_SIGNATURES:
+        cache.clear()
+    cache[sig] = got
 
 
 class ScorePool(KVPool):
@@ -65,8 +72,8 @@ class ScorePool(KVPool):
         """
         B, width = check_block_tables(self, block_tables, seq_lens)
         heads = self.block_size  # a block is [H, BS]
-        if keep <= 0:
-            raise ValueError("keep must be positive")
+        if keep <= 0 or max(keep, abs(recent), abs(sink)) > _INT32_MAX:
+            raise ValueError("keep must be positive, and the three counts fit 32 bits")
         index = torch.empty((self.num_layers, B, heads, keep), dtype=torch.int32, device=self.device)
         new_lens = torch.empty(B, dtype=torch.int32, device=self.device)
         rc = self.ctx._lib.emm_select_tokens(
@@ -153,12 +160,12 @@ class KVPoolQ4(KVPool):
             got = self._check_rows(key, value, slot_mapping, lead)
             if lead and key.shape[0] != self.num_layers:
                 raise ValueError(f"key has {key.shape[0]} layers, pool has {self.num_layers}")
-            if len(self._row_sigs) < _MAX_SIGNATURES:
-                self._row_sigs[sig] = got
+            _remember(self._row_sigs, sig, got)
         return got
 
     def append(self, layer: int, key: torch.Tensor, value: torch.Tensor, slot_mapping: torch.Tensor) -> None:
-        """Quantises one layer's new rows [T, H, D] (fp16 or bf16) into their slots; slot < 0 is skipped."""
+        """Quantises one layer's new rows [T, H, D] (fp16 or bf16) into their slots; slot < 0 is skipped.
+        The slots must be distinct: one that appears twice ends with bytes of both rows."""
         T, dt, (_, kts, _, vts) = self._rows_sig(key, value, slot_mapping, 0)
         rc = self._emm_q4_append(self._h, self.head_dim, dt, layer, 1, key.data_ptr(), value.data_ptr(), 0, kts, 0, vts,
                                  slot_mapping.data_ptr(), T, _stream_ptr(self.ctx.device))
@@ -243,7 +250,7 @@ class KVPoolQ4(KVPool):
                 raise ValueError(f"{name} heads must be contiguous ([heads, D] dense per sequence)")
         cap = width * self.block_size
         limit = cap if max_len is None else int(max_len)
-        if limit < 0 or limit > cap or limit > 0x7FFFFFFF:
+        if limit < 0 or limit > cap or limit > _INT32_MAX:
             raise ValueError(f"max_len {limit} outside [0, {cap}], what the tables can hold")
         nbytes = C.c_uint64()
         _lib.check(self.ctx._lib.emm_q4_attend_workspace(self._h, D, B, heads, limit, int(scores is not None),
@@ -274,8 +281,7 @@ class KVPoolQ4(KVPool):
         got = self._attend_sigs.get(sig)
         if got is None:
             got = self._check_attend(query, block_tables, seq_lens, out, scores, max_len)
-            if len(self._attend_sigs) < _MAX_SIGNATURES:
-                self._attend_sigs[sig] = got
+            _remember(self._attend_sigs, sig, got)
         dt, B, heads, width, limit, qs, os_, nbytes, default_scale = got
         device = self.ctx.device
         if out is None:

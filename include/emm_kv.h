@@ -357,8 +357,8 @@ int emm_q4_row_bytes(int32_t head_dim);
 /* emm_append / emm_append_all_layers with quantisation: 16-bit key/value rows
  * [layer_count, T, H, D] (heads dense, strides in bytes) go to their slots in
  * layers [layer_begin, layer_begin + layer_count). slot < 0 is skipped, a slot
- * outside the pool recorded in the status word and skipped; when a slot
- * appears twice, groups of either row may win. */
+ * outside the pool recorded in the status word and skipped. Slots must be
+ * distinct: one that appears twice ends with bytes of both rows. */
 int emm_q4_append(emm_pool *pool, int32_t head_dim, int32_t dtype, int32_t layer_begin, int32_t layer_count,
                   const void *d_key, const void *d_value, int64_t key_layer_stride, int64_t key_token_stride,
                   int64_t value_layer_stride, int64_t value_token_stride, const int64_t *d_slot_mapping,

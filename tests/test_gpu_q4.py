@@ -406,6 +406,8 @@ def test_attend_arguments(ctx):
     with pytest.raises(_lib.EmmError):
         pool.attend(0, q, tables_d, lens_d, scale=float("nan"))
     with pytest.raises(_lib.EmmError):
+        pool.attend(0, q, tables_d, lens_d, scale=1e39)  # infinite in 32 bits
+    with pytest.raises(_lib.EmmError):
         pool.attend(0, q, tables_d, lens_d, scores=ScorePool([torch.zeros(15, H, BS, device="cuda")], ctx))
     many = torch.zeros(3, 65 * H, D, dtype=BF, device="cuda")
     with pytest.raises(ValueError, match="at most 64"):
@@ -438,6 +440,78 @@ def test_attend_reports_bad_lengths_and_blocks(ctx):
     check_scores(scores.layers[0], np.zeros((16, H, BS), dtype=np.float32), short, [48, 32, 0], weights, spread, group)
     assert (out[2] == 0).all()
     assert_clean(ctx)
+
+
+def test_attend_logits_far_below_zero(ctx):
+    """Logits of -1e31 and less: the largest still takes all the weight, and its row comes out rounded once."""
+    D, H, BS, n = 128, 1, 16, 40
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((2, 4 * BS, H, D)).astype(np.float16).astype(np.float32)
+    x[0, :, 0, :32] = 0
+    x[0, :, 0, 0] = -4.0 - np.arange(4 * BS) % 7
+    x[0, 29, 0, 0] = -2.0  # position 29; nowhere else above -4
+    layer = np.stack([q4_oracle.encode_rows(p.reshape(-1, D)) for p in x]).reshape(2, 4, BS, H, -1)
+    pool = KVPoolQ4([dev(layer)], D, ctx)
+    tables = np.arange(4, dtype=np.int32)[None]
+    q = torch.zeros(1, 2, D, dtype=BF)
+    q[0, :, 0] = 1e32
+    scores = ScorePool.like(pool)
+    out = pool.attend(0, q.cuda(), dev(tables), dev(np.array([n], dtype=np.int32)), scores=scores)
+    # one weight is 1 and the others are 0 exactly, so nothing but the product p s c and the result are rounded
+    value = q4_oracle.decode_rows(layer[1].reshape(-1, layer.shape[-1]), D)[29]
+    tol = 2.0 ** -9 * np.abs(value) + 2.0 ** -11 * 16 * 0.5
+    assert (np.abs(out.double().cpu().numpy() - value) <= tol).all()
+    want = torch.zeros(4, H, BS)
+    want[1, 0, 13] = 2  # both query heads
+    assert torch.equal(scores.layers[0].cpu(), want)
+    assert_clean(ctx)
+
+
+def test_attend_many_short_sequences_in_wide_tables(ctx):
+    """More sequences than a block has threads, most of them empty, in tables for far longer ones (a padded batch)."""
+    D, H, group, BS = 64, 2, 2, 16
+    rng = np.random.default_rng(3)
+    lens = np.where(rng.random(700) < 0.6, 0, rng.integers(1, 50, 700)).tolist()
+    NB = sum(-(-n // BS) for n in lens)
+    pool, bytes_ = random_pool(1, NB, BS, H, D, False, 4)
+    tables = tables_for(lens, NB, BS, 4, extra=2000)
+    q = torch.randn(700, H * group, D, generator=torch.Generator().manual_seed(3)).to(BF)
+    before = rng.random((NB, H, BS), dtype=np.float32)
+    scores = ScorePool([dev(before)], ctx)
+    out = pool.attend(0, q.cuda(), dev(tables), dev(np.array(lens, dtype=np.int32)), scores=scores)
+    assert_clean(ctx)
+    ref, weights, bound, spread = q4_oracle.attend(bytes_[0], D, q.double().numpy(), tables, lens, D ** -0.5)
+    check_out(out, ref, bound, spread, BF)
+    check_scores(scores.layers[0], before, tables, lens, weights, spread, group)
+
+
+@pytest.mark.parametrize("hnd", [False, True], ids=["nhd", "hnd"])
+def test_offsets_past_32_bits(ctx, hnd):
+    """Blocks that begin more than 2^32 bytes into their plane hold, read and move what the same blocks of a small pool do."""
+    D, H, group, BS, n = 128, 8, 4, 16, 200
+    k = -(-n // BS)
+    NB = (5 << 30) // (BS * H * 80)
+    g = torch.Generator().manual_seed(1)
+    key, value = torch.randn(n, H, D, generator=g).to(BF).cuda(), torch.randn(n, H, D, generator=g).to(BF).cuda()
+    q = torch.randn(1, H * group, D, generator=g).to(BF).cuda()
+    lens = dev(np.array([n], dtype=np.int32))
+    got = []
+    for blocks, ids in ((k, np.arange(k)), (NB, np.concatenate([NB - 1 - np.arange(k - 2), [0, 1]]))):
+        pool = KVPoolQ4([t for t in new_layers(1, blocks, BS, H, D, hnd)], D, ctx)
+        scores = ScorePool.like(pool)
+        tables = dev(ids[None].astype(np.int32))
+        slots = (dev(ids)[:, None] * BS + torch.arange(BS, device="cuda")).flatten()[:n]
+        pool.append(0, key, value, slots)
+        rows = pool.read(slots, BF)
+        out = pool.attend(0, q, tables, lens, scores=scores)
+        index, _ = scores.select_tokens(tables, lens, 60, recent=5)
+        pool.keep_tokens(index, tables, lens)
+        kept = pool.read(slots[:60], BF)
+        got.append([*rows, out, index, *kept])
+        assert_clean(ctx)
+        pool.close()
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
 
 
 # ----------------------------------------------------------------------------------------------------------- eviction
@@ -518,7 +592,7 @@ def test_eviction_refusals_and_reports(ctx):
     scores = ScorePool([torch.rand(NB, H, BS, device="cuda")], ctx)
     pool = KVPool([torch.zeros(2, NB, BS, H, 64, dtype=BF, device="cuda")], ctx)
     tables, lens = dev(tables_for([40, 20], NB, BS, 1)), dev(np.array([40, 20], dtype=np.int32))
-    for keep, recent, sink in ((0, 0, 0), (-1, 0, 0), (8, 9, 0), (8, 4, 5), (8, -1, 0), (8, 0, -1)):
+    for keep, recent, sink in ((0, 0, 0), (-1, 0, 0), (8, 9, 0), (8, 4, 5), (8, -1, 0), (8, 0, -1), (2 ** 32 + 8, 0, 0), (8, 2 ** 32, 0)):
         with pytest.raises((ValueError, _lib.EmmError)):
             scores.select_tokens(tables, lens, keep, recent=recent, sink=sink)
     index, _ = scores.select_tokens(tables, lens, 8)

@@ -76,6 +76,19 @@ def test_swap_and_scores_move_with_blocks():
     assert (s.layers[1][8] == 3.0).all()
 
 
+def test_weights_follow_a_compaction():
+    w = _worker()
+    w.write_kv_blocks([6, 7], torch.randn(L, 2, 2, BS, H, D, dtype=torch.bfloat16, device="cuda"))
+    before = w.extract_kv_blocks([6, 7]).clone()
+    s = w.init_scores()
+    for layer in s.layers:
+        layer[6], layer[7] = 6.0, 7.0
+    assert w.compact_blocks([6, 7], [0, 1])["blocks"] == 2
+    assert torch.equal(w.extract_kv_blocks([0, 1]), before)
+    for layer in s.layers:
+        assert (layer[0] == 6.0).all() and (layer[1] == 7.0).all()
+
+
 def test_decode_evict_and_free():
     """Requests decode, are cut back, give blocks back, and decode on in what they kept."""
     w = _worker()
