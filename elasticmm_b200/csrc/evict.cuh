@@ -233,18 +233,18 @@ __global__ void __launch_bounds__(kKeepThreads) keep_rows(const __grid_constant_
   const uint64_t base = a.pool.layers[l] + p * a.pool.plane_stride + h * a.pool.head_stride + piece * a.row_bytes + part * sizeof(V);
   // Row segments in order; a thread that has none counts from behind the end.
   const Pos total = (Pos)a.keep * segments, step = (Pos)rows * kKeepAhead, own = mine < rows ? (Pos)mine : total;
-  auto row_at = [&](uint32_t t) -> uint64_t {
-    const uint32_t blk = kPlain ? t >> a.pool.block_shift : t / a.pool.block_size;
-    const uint32_t id = (uint32_t)table[blk];
+  auto block_of = [&](uint32_t t) -> int32_t { return table[kPlain ? t >> a.pool.block_shift : t / a.pool.block_size]; };
+  auto row_in = [&](uint32_t t, int32_t entry) -> uint64_t {
+    const uint32_t id = (uint32_t)entry;
     if (id >= a.pool.num_blocks) {
-      report(a.status, kStatusIdRange, (int32_t)id);
+      report(a.status, kStatusIdRange, entry);
       return 0;
     }
     if constexpr (kPlain)
       return base + (uint64_t)id * (uint32_t)a.pool.block_stride +
              (uint64_t)(t & ((1u << a.pool.block_shift) - 1u)) * (uint32_t)a.pool.token_stride;
     else
-      return base + (uint64_t)id * a.pool.block_stride + (uint64_t)(t - blk * a.pool.block_size) * a.pool.token_stride;
+      return base + (uint64_t)id * a.pool.block_stride + (uint64_t)(t % a.pool.block_size) * a.pool.token_stride;
   };
   // Bytes from a row's first segment to segment i's, or -1 where this thread has no vector in it.
   auto segment = [&](Pos i) -> int64_t {
@@ -252,12 +252,24 @@ __global__ void __launch_bounds__(kKeepThreads) keep_rows(const __grid_constant_
     const uint32_t seg = (uint32_t)(i % segments) * kKeepThreads;
     return part + seg < vecs ? (int64_t)seg * (int64_t)sizeof(V) : -1;
   };
-  int32_t from[kKeepAhead];  // positions of the next chunk to load
+  // What a row needs is fetched a chunk ahead of its use: its position, then the block of that, then its bytes.
+  int32_t next[kKeepAhead];                      // positions of the chunk after the next to load
+  int32_t from[kKeepAhead], from_block[kKeepAhead];  // the next to load: positions (-1: does not move) and blocks
   auto positions = [&](Pos first) {
 #pragma unroll
     for (int u = 0; u < kKeepAhead; ++u) {
       const Pos i = first + u * rows;
-      from[u] = i < total ? index[kPlain ? i : i / segments] : -1;
+      next[u] = i < total ? index[kPlain ? i : i / segments] : -1;
+    }
+  };
+  auto blocks = [&](Pos first) {
+#pragma unroll
+    for (int u = 0; u < kKeepAhead; ++u) {
+      const Pos i = first + u * rows;
+      // a row that stays, or that the index does not put behind its place and inside the sequence, is left alone
+      const bool on = next[u] > (int64_t)(kPlain ? i : i / segments) && next[u] < len && segment(i) >= 0;
+      from[u] = on ? next[u] : -1;
+      from_block[u] = on ? block_of((uint32_t)next[u]) : 0;
     }
   };
   uint32_t moves = 0;  // bit kKeepAhead s + u: row u of the chunk in stage s moves
@@ -265,12 +277,10 @@ __global__ void __launch_bounds__(kKeepThreads) keep_rows(const __grid_constant_
     moves &= ~(((1u << kKeepAhead) - 1u) << (s * kKeepAhead));
 #pragma unroll
     for (int u = 0; u < kKeepAhead; ++u) {
-      const Pos i = first + u * rows;
-      const uint32_t j = (uint32_t)(kPlain ? i : i / segments);
-      // a row that stays, or that the index does not put behind its place and inside the sequence, is left alone
-      if (from[u] > (int64_t)j && from[u] < len && segment(i) >= 0) {
-        const uint64_t src = row_at((uint32_t)from[u]);
+      if (from[u] >= 0) {
+        const uint64_t src = row_in((uint32_t)from[u], from_block[u]);
         if (src) {
+          const Pos i = first + u * rows;
           V *to = &ring[s][u][threadIdx.x];
           if constexpr (sizeof(V) >= 4)
             asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(to)), "l"(src + segment(i)), "n"((int)sizeof(V)) : "memory");
@@ -281,11 +291,25 @@ __global__ void __launch_bounds__(kKeepThreads) keep_rows(const __grid_constant_
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  auto ahead_of = [&](Pos first) {  // from here on `from` is of the chunk at first
+    blocks(first);
+    positions(first + step);
+  };
+  int32_t to_block[kKeepAhead];  // of the chunk to store
+  auto places = [&](Pos first) {
+#pragma unroll
+    for (int u = 0; u < kKeepAhead; ++u) {
+      const Pos i = first + u * rows;
+      to_block[u] = i < total ? block_of((uint32_t)(kPlain ? i : i / segments)) : 0;
+    }
+  };
   positions(own);
+  ahead_of(own);
+  places(own);
 #pragma unroll
   for (int s = 0; s < kKeepStages - 1; ++s) {
     load(own + s * step, s);
-    positions(own + (s + 1) * step);
+    ahead_of(own + (s + 1) * step);
   }
   int stage = 0, ahead = kKeepStages - 1;
   const Pos chunks = (total + step - 1) / step;
@@ -293,17 +317,18 @@ __global__ void __launch_bounds__(kKeepThreads) keep_rows(const __grid_constant_
 #pragma unroll 1
   for (Pos c = 0; c < chunks; ++c, first += step) {
     load(first + (kKeepStages - 1) * step, ahead);
-    positions(first + kKeepStages * step);
+    ahead_of(first + kKeepStages * step);
     uint64_t dst[kKeepAhead];
 #pragma unroll
     for (int u = 0; u < kKeepAhead; ++u) {
       const Pos i = first + u * rows;
       dst[u] = 0;
       if (moves >> (stage * kKeepAhead + u) & 1) {
-        dst[u] = row_at((uint32_t)(kPlain ? i : i / segments));
+        dst[u] = row_in((uint32_t)(kPlain ? i : i / segments), to_block[u]);
         if (!kPlain && dst[u]) dst[u] += segment(i);
       }
     }
+    places(first + step);
     asm volatile("cp.async.wait_group %0;" ::"n"(kKeepStages - 1) : "memory");
     __syncthreads();
 #pragma unroll
