@@ -60,6 +60,8 @@ struct AttendShape {
 // 1.2 us for a unit of 32 tokens and 8 heads). Without it the CTAs with many short sequences finish last.
 constexpr uint32_t kItemCost = 3;
 
+constexpr uint32_t kScoreTokens = 128;  // tokens of a warp's turn in attend_scores
+
 struct AttendArgs {
   TokenSide pool;
   uint64_t layer_base;        // this layer's base address
@@ -86,7 +88,7 @@ struct AttendArgs {
   int *cta_item;              // [grid]: the split item that this CTA finished, or -1
   float *lse;                 // [B, Hq], with scores
   float *logits;              // [B, Hq, logit_stride], with scores
-  uint32_t *longest;          // the batch's largest length, with scores
+  uint32_t *turns;            // [B + 1], with scores: turns of kScoreTokens tokens in all sequences before this one
   uint64_t logit_stride;
   int *status;
 };
@@ -247,7 +249,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
   constexpr int kTile = 32 * R, kWords = kT * kTile;  // bytes of a tile; where a slot's words begin
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Share share;
-  __shared__ uint32_t scan[kAttendWarps], tops[kAttendWarps];
+  __shared__ uint32_t scan[kAttendWarps];
 
   const AttendShape &sh = a.sh;
   const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -258,11 +260,10 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
   {
     const uint32_t per = (a.num_seqs + blockDim.x - 1) / blockDim.x;
     const uint32_t b0 = min(a.num_seqs, tid * per), b1 = min(a.num_seqs, b0 + per);
-    uint32_t mine = 0, n0 = 0, top = 0;
+    uint32_t mine = 0, n0 = 0;
     for (uint32_t b = b0; b < b1; ++b) {
       const uint32_t n = seq_length(a, b, blockIdx.x == 0);
       if (b == b0) n0 = n;
-      top = max(top, n);
       mine += (seq_units(a, n) + kItemCost) * sh.head_groups;
     }
     uint32_t upto = mine;
@@ -272,10 +273,6 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
       if (lane >= m) upto += other;
     }
     if (lane == 31) scan[warp] = upto;
-    if constexpr (kScores) {
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0) tops[warp] = top;
-    }
     __syncthreads();
     uint32_t before = 0, total = 0;
     for (uint32_t w = 0; w < blockDim.x / 32; ++w) {
@@ -283,10 +280,6 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
       total += scan[w];
     }
     before += upto - mine;
-    if constexpr (kScores) {
-      for (uint32_t w = 0; w < blockDim.x / 32; ++w) top = max(top, tops[w]);
-      if (blockIdx.x == 0 && tid == 0) *a.longest = top;
-    }
     const uint32_t each = total / gridDim.x, extra = total - each * gridDim.x;
     const uint32_t first = each * blockIdx.x + min(blockIdx.x, extra);
     if (first >= total && tid == 0) share = Share{0, 0, 0, 0, 0, 0, 0};  // more CTAs than places
@@ -308,6 +301,22 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
       share.extra = extra;
     }
     __syncthreads();
+    if (kScores && blockIdx.x == 0) {  // the same count for attend_scores
+      uint32_t turns = 0;
+      for (uint32_t b = b0; b < b1; ++b) turns += (seq_length(a, b, false) + kScoreTokens - 1) / kScoreTokens;
+      uint32_t at = turns;
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) {
+        const uint32_t other = __shfl_up_sync(0xffffffffu, at, m);
+        if (lane >= m) at += other;
+      }
+      if (lane == 31) scan[warp] = at;
+      __syncthreads();
+      at -= turns;
+      for (uint32_t w = 0; w < warp; ++w) at += scan[w];
+      if (tid == 0) a.turns[0] = 0;
+      for (uint32_t b = b0; b < b1; ++b) a.turns[b + 1] = at += (seq_length(a, b, false) + kScoreTokens - 1) / kScoreTokens;
+    }
   }
   const uint32_t end = share.end;
   uint32_t b = share.b, hg = share.hg, unit = share.unit, place = share.place;
@@ -1040,21 +1049,27 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join(const __grid_cons
     a.lse[(uint64_t)b * a.kv_heads * a.group + head] = sum == 0.f ? INFINITY : top + lg2(sum);
 }
 
-// Adds every token's weight to its score. A warp's turn is 128 tokens of a (sequence, KV head) pair, four a lane; turns go
-// chunk by chunk over all pairs up to the batch's largest length (max_len may be far more), so that long and short
-// sequences are spread over all warps. Nothing here needs the
-// latency hidden better than by many warps with few registers.
-constexpr uint32_t kScoreTokens = 128;
-
+// Adds every token's weight to its score. A warp's turn is 128 tokens of a (sequence, KV head) pair, four a lane. Turns are
+// counted over the tokens that there are (max_len may be far more), so every warp has the same number, give or take one: one
+// or two of them at 131 K tokens and 8 heads, whose latencies are what the kernel costs.
 __global__ void __launch_bounds__(256, 6) attend_scores(const __grid_constant__ AttendArgs a) {
   grid_launch_dependents();
   grid_dependency_wait();
-  const uint32_t lane = threadIdx.x % 32, pairs = a.num_seqs * a.kv_heads;
-  const uint64_t total = (uint64_t)pairs * ((*a.longest + kScoreTokens - 1) / kScoreTokens), step = (uint64_t)gridDim.x * 8;
+  const uint32_t lane = threadIdx.x % 32;
+  const uint64_t total = (uint64_t)a.turns[a.num_seqs] * a.kv_heads, step = (uint64_t)gridDim.x * 8;
   for (uint64_t i = (uint64_t)blockIdx.x * 8 + threadIdx.x / 32; i < total; i += step) {
-    const uint32_t c = (uint32_t)(i / pairs), bh = (uint32_t)(i - (uint64_t)c * pairs), b = bh / a.kv_heads, h = bh - b * a.kv_heads;
-    const uint32_t n = seq_length(a, b, false), t = c * kScoreTokens + lane * 4;
+    const uint32_t turn = (uint32_t)(i / a.kv_heads), h = (uint32_t)(i - (uint64_t)turn * a.kv_heads);
+    // The last sequence that begins at or before this turn: 32 are looked at together, then the 32 within a step of those.
+    uint32_t b = 0;
+    for (uint32_t width = a.num_seqs; width > 1;) {
+      const uint32_t each = (width + 31) / 32, from = min(b + lane * each, a.num_seqs);
+      const uint32_t below = __ballot_sync(0xffffffffu, lane * each < width && a.turns[from] <= turn);
+      b += (31 - __clz(below)) * each;
+      width = min(each, a.num_seqs - b);
+    }
+    const uint32_t n = seq_length(a, b, false), t = (turn - a.turns[b]) * kScoreTokens + lane * 4;
     if (t >= n) continue;
+    const uint32_t bh = b * a.kv_heads + h;
     const uint64_t head = (uint64_t)bh * a.group;
     float *sc[4];
     float old[4], w[4] = {0.f, 0.f, 0.f, 0.f};

@@ -187,7 +187,7 @@ int attend_shape(const emm_pool *pool, int32_t D, int32_t B, int32_t group, int3
 }
 
 struct AttendWorkspace {
-  uint64_t part_o, part_ml, item_span, cta_item, lse, longest, logits, logit_stride, bytes;
+  uint64_t part_o, part_ml, item_span, cta_item, lse, turns, logits, logit_stride, bytes;
 };
 
 AttendWorkspace attend_workspace(const emm::AttendShape &s, int32_t D, int32_t B, int32_t Hq, int32_t group, int32_t max_len,
@@ -205,7 +205,7 @@ AttendWorkspace attend_workspace(const emm::AttendShape &s, int32_t D, int32_t B
   w.item_span = take((uint64_t)s.items * 8);
   w.cta_item = take((uint64_t)s.grid * 4);
   w.lse = take(scores ? (uint64_t)B * Hq * 4 : 0);
-  w.longest = take(scores ? 4 : 0);
+  w.turns = take(scores ? (uint64_t)(B + 1) * 4 : 0);
   w.logit_stride = ((uint64_t)max_len + 7) / 8 * 8;
   w.logits = take(scores ? (uint64_t)B * Hq * w.logit_stride * 4 : 0);
   w.bytes = at;
@@ -358,7 +358,7 @@ int emm_q4_attend(emm_pool *pool, int32_t head_dim, int32_t dtype, int32_t layer
   a.item_span = (int2 *)(ws + w.item_span);
   a.cta_item = (int *)(ws + w.cta_item);
   a.lse = (float *)(ws + w.lse);
-  a.longest = (uint32_t *)(ws + w.longest);
+  a.turns = (uint32_t *)(ws + w.turns);
   a.logits = (float *)(ws + w.logits);
   a.logit_stride = w.logit_stride;
   a.status = pool->ctx->d_status;
