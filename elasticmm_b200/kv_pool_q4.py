@@ -285,7 +285,7 @@ class KVPoolQ4(KVPool):
         dt, B, heads, width, limit, qs, os_, nbytes, default_scale = got
         device = self.ctx.device
         if out is None:
-            out = torch.empty((B, heads, self.head_dim), dtype=query.dtype, device=device)
+            out = torch.empty_like(query)  # dense: the heads are, and a gap between sequences is not kept
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         rc = self._emm_q4_attend(
             self._h, self.head_dim, dt, layer, query.data_ptr(), qs, out.data_ptr(), os_, block_tables.data_ptr(),
