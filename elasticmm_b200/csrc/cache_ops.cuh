@@ -7,10 +7,11 @@
 
 namespace {
 
-// Launches with programmatic stream serialisation (EMM_OPT_PDL): placed while the kernel before it in the stream drains.
-// Every kernel here waits for that one to complete before its first global access.
+// Launches, if `early` with programmatic stream serialisation (EMM_OPT_PDL): placed while the kernel before it in the
+// stream drains. Every kernel here waits for that one to complete before its first global access.
 template <typename... Params, typename... Args>
-int launch_after(emm_ctx *ctx, void (*kernel)(Params...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, const Args &...args) {
+int launch_after(emm_ctx *ctx, void (*kernel)(Params...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, bool early,
+                 const Args &...args) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -20,7 +21,7 @@ int launch_after(emm_ctx *ctx, void (*kernel)(Params...), dim3 grid, unsigned bl
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = ctx->pdl ? 1 : 0;
+  cfg.numAttrs = early && ctx->pdl ? 1 : 0;
   EMM_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
   ctx->launches += 1;
   return EMM_OK;
@@ -136,9 +137,9 @@ int q4_rows_impl(emm_pool *pool, bool append, int32_t D, int32_t dtype, int32_t 
   const unsigned block = wide ? emm::kRowWarps * 32 : 256;
 #define EMM_Q4_ROWS(T_, D_)                                                                                    \
   return append ? launch_after(ctx, wide ? emm::q4_append_rows<T_, D_> : emm::q4_append_units<T_, D_>, grid,   \
-                               block, 0, st, a)                                                                \
+                               block, 0, st, true, a)                                                                \
                 : launch_after(ctx, wide ? emm::q4_read_rows<T_, D_> : emm::q4_read_units<T_, D_>, grid, block, \
-                               0, st, a)
+                               0, st, true, a)
   if (dtype == EMM_DTYPE_FP16) {
     if (D == 64) EMM_Q4_ROWS(__half, 64);
     else if (D == 128) EMM_Q4_ROWS(__half, 128);
@@ -226,7 +227,7 @@ int attend_main(emm_ctx *ctx, const emm::AttendArgs &a, int smem, cudaStream_t s
     EMM_CUDA(cudaFuncSetAttribute(emm::attend_q4<T, D, kScores, kPages>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     if (tracked) limit[device].store(most, std::memory_order_release);
   }
-  return launch_after(ctx, emm::attend_q4<T, D, kScores, kPages>, dim3(a.sh.grid), a.sh.warps * 32, (size_t)smem, st, a);
+  return launch_after(ctx, emm::attend_q4<T, D, kScores, kPages>, dim3(a.sh.grid), a.sh.warps * 32, (size_t)smem, st, true, a);
 }
 
 template <typename T, int D>
@@ -241,14 +242,14 @@ int attend_launch(emm_ctx *ctx, const emm::AttendArgs &a, int smem, cudaStream_t
     // Where items are few an item has many parts, and a head needs all warps of a block; else two.
     const bool many = x * 8 <= a.sh.grid;
     if (int rc2 = launch_after(ctx, many ? emm::attend_join<T, D, 1> : emm::attend_join<T, D, 8>,
-                               dim3(x, many ? rows : (rows + 7) / 8), emm::kJoinWarps * 32, 0, st, a, (uint32_t)by_cta))
+                               dim3(x, many ? rows : (rows + 7) / 8), emm::kJoinWarps * 32, 0, st, true, a, (uint32_t)by_cta))
       return rc2;
   }
   if (a.score_base && a.max_len > 0) {
     const uint32_t chunks = (a.max_len + emm::kScoreTokens - 1) / emm::kScoreTokens;
     const uint64_t turns = (uint64_t)a.num_seqs * a.kv_heads * chunks;
     const unsigned grid = (unsigned)std::min<uint64_t>((turns + 7) / 8, (uint64_t)ctx->sm_count * 6);
-    return launch_after(ctx, emm::attend_scores, dim3(grid), 256, 0, st, a);
+    return launch_after(ctx, emm::attend_scores, dim3(grid), 256, 0, st, true, a);
   }
   return EMM_OK;
 }
@@ -413,12 +414,14 @@ int emm_select_tokens(emm_pool *scores, const int32_t *d_block_tables, int64_t t
   const int64_t most = (int64_t)table_width * d.head_size;
   cudaStream_t st = (cudaStream_t)stream;
   emm_ctx *ctx = scores->ctx;
-  if (most * 4 > kSelectSharedMax) return launch_after(ctx, emm::select_tokens<1024, false>, grid, 1024, 0, st, a);
+  if (most * 4 > kSelectSharedMax) return launch_after(ctx, emm::select_tokens<1024, false>, grid, 1024, 0, st, true, a);
   const size_t keys = (size_t)most * 4;
-  if (most <= 4096) return launch_after(ctx, emm::select_tokens<256, true>, grid, 256, keys, st, a);
-  if (most <= 11264) return launch_after(ctx, emm::select_tokens<512, true>, grid, 512, keys, st, a);  // 44 KB: the default limit
-  EMM_CUDA(cudaFuncSetAttribute(emm::select_tokens<1024, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectSharedMax));
-  return launch_after(ctx, emm::select_tokens<1024, true>, grid, 1024, keys, st, a);
+  // Small CTAs where a thread has at most 16 keys: eight CTAs share an SM then, and one's barriers hide behind the others'
+  // (2 048 CTAs of 3 000-4 096 keys: 59 us, with 1 024 threads 74; 10 000 keys: 1 024 threads 11 us faster than 256).
+  if (most <= 4096) return launch_after(ctx, emm::select_tokens<256, true>, grid, 256, keys, st, true, a);
+  if (keys > 48 * 1024)
+    EMM_CUDA(cudaFuncSetAttribute(emm::select_tokens<1024, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectSharedMax));
+  return launch_after(ctx, emm::select_tokens<1024, true>, grid, 1024, keys, st, true, a);
 }
 
 int emm_keep_tokens(emm_pool *pool, const int32_t *d_index, int32_t index_heads, int32_t keep,
@@ -467,11 +470,12 @@ int emm_keep_tokens(emm_pool *pool, const int32_t *d_index, int32_t index_heads,
   for (uint64_t v : strides) align = std::min(align, pow2_align(v));
   DeviceGuard guard(pool->ctx->device);
   if (!guard.ok()) return fail(EMM_ERR_CUDA, "cannot select device %d", pool->ctx->device);
-  // Where an SM would have fewer than four CTAs, two or four share a row, down to 64 bytes each: a CTA's rows come one
-  // chunk after the other, so few CTAs cannot keep HBM busy.
+  // Two or four CTAs share a row, down to 64 bytes each, where all still fit the GPU at once (four an SM): a CTA's rows
+  // come one chunk after the other, so few CTAs cannot keep HBM busy (20 000 -> 10 000 tokens, 4 heads: 4 layers 134
+  // instead of 200 us, 16 layers 210 instead of 384).
   a.splits = 1;
   const uint64_t ctas = (uint64_t)num_seqs * a.heads * a.planes * (uint64_t)d.num_layers;
-  while (a.splits < 4 && ctas * a.splits < 4ull * pool->ctx->sm_count && a.row_bytes % 32 == 0 && a.row_bytes / 2 >= 64) {
+  while (a.splits < 4 && ctas * a.splits * 2 <= 4ull * pool->ctx->sm_count && a.row_bytes % 32 == 0 && a.row_bytes / 2 >= 64) {
     a.splits *= 2;
     a.row_bytes /= 2;
     align = std::min(align, pow2_align(a.row_bytes));
@@ -483,8 +487,12 @@ int emm_keep_tokens(emm_pool *pool, const int32_t *d_index, int32_t index_heads,
                      std::max(a.pool.block_stride, a.pool.token_stride) <= 0xffffffffull &&
                      (uint64_t)keep < (1ull << 31) - 64 * emm::kKeepThreads;
   emm_ctx *ctx = pool->ctx;
-#define EMM_KEEP(V_) \
-  return launch_after(ctx, plain ? emm::keep_rows<V_, true> : emm::keep_rows<V_, false>, grid, emm::kKeepThreads, 0, st, a)
+  // CTAs placed while the kernel before them drains are not spread evenly over the SMs. Where they are few, with long
+  // chains, that costs more than the start it saves (4 layers: 118 us, and 89 behind a finished kernel).
+  const bool early = ctas * a.splits >= 4ull * ctx->sm_count || (uint64_t)keep * a.row_bytes <= 128 * 1024;
+#define EMM_KEEP(V_)                                                                                                    \
+  return launch_after(ctx, plain ? emm::keep_rows<V_, true> : emm::keep_rows<V_, false>, grid, emm::kKeepThreads, 0, st, \
+                      early, a)
   if (vec >= 16) EMM_KEEP(uint4);
   if (vec >= 8) EMM_KEEP(uint2);
   if (vec >= 4) EMM_KEEP(uint32_t);
@@ -506,7 +514,7 @@ int emm_reset_scores(emm_pool *scores, const int64_t *d_slot_mapping, int32_t nu
   DeviceGuard guard(scores->ctx->device);
   if (!guard.ok()) return fail(EMM_ERR_CUDA, "cannot select device %d", scores->ctx->device);
   return launch_after(scores->ctx, emm::reset_scores, dim3((unsigned)blocks, (unsigned)d.num_layers), 256, 0,
-                      (cudaStream_t)stream, (const uint64_t *)scores->d_layers, (uint64_t)d.block_stride, (uint32_t)d.num_blocks,
+                      (cudaStream_t)stream, true, (const uint64_t *)scores->d_layers, (uint64_t)d.block_stride, (uint32_t)d.num_blocks,
                       (uint32_t)d.head_size, (uint32_t)d.block_size, d_slot_mapping, (uint64_t)num_tokens, scores->ctx->d_status);
 }
 
