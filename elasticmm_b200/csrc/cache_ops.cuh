@@ -237,7 +237,7 @@ int attend_launch(emm_ctx *ctx, const emm::AttendArgs &a, int smem, cudaStream_t
   const int rc = a.score_base ? (pages ? attend_main<T, D, true, true>(ctx, a, smem, st) : attend_main<T, D, true, false>(ctx, a, smem, st))
                               : (pages ? attend_main<T, D, false, true>(ctx, a, smem, st) : attend_main<T, D, false, false>(ctx, a, smem, st));
   if (rc) return rc;
-  if (a.sh.grid > 1) {  // one CTA splits nothing
+  if (a.max_len > a.sh.tokens) {  // else every item is one unit, which no CTA shares
     const bool by_cta = a.sh.items > a.sh.grid;
     const uint32_t rows = a.sh.heads_cta * a.group, x = by_cta ? a.sh.grid : a.sh.items;
     // Few items have many parts each; see attend_join.

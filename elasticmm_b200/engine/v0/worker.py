@@ -352,7 +352,8 @@ class V0Worker:
     def evict_tokens(self, block_tables: torch.Tensor, seq_lens: torch.Tensor, keep: int, recent: int = 0,
                      sink: int = 0) -> Dict[str, Any]:
         """Cuts every sequence to its `keep` tokens with the most weight, the first `sink` and the last `recent` among
-        them, per layer and KV head; rows and weights move to the front of the sequence's blocks. Returns
+        them, per layer and KV head; rows and weights move to the front of the sequence's blocks, none of which may belong
+        to another sequence of the call. Returns
         {"seq_lens": the new lengths (int32, on the device), "index": the kept positions}. The blocks behind
         ceil(keep / block size) can then be freed (V0BlockManager.truncate_blocks)."""
         pool = self._require_pool()

@@ -287,6 +287,8 @@ class KVPoolQ4(KVPool):
             got = self._check_attend(query, block_tables, seq_lens, out, scores, max_len)
             _remember(self._attend_sigs, sig, got)
         dt, B, heads, width, limit, qs, os_, nbytes, default_scale = got
+        if scores is not None and not scores._h:
+            raise ValueError("the score pool is closed")
         device = self.ctx.device
         if out is None:
             D = self.head_dim

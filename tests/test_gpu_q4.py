@@ -442,6 +442,25 @@ def test_attend_reports_bad_lengths_and_blocks(ctx):
     assert_clean(ctx)
 
 
+@pytest.mark.parametrize("D,group,dtype", [(64, 8, FP), (128, 3, BF), (256, 4, BF), (256, 1, FP)])
+def test_attend_one_head_long(ctx, D, group, dtype):
+    """One KV head, and tokens for every SM: all warps of a block work on the same head."""
+    BS, lens = 16, [40001, 5]
+    NB = sum(-(-n // BS) for n in lens)
+    pool, bytes_ = random_pool(1, NB, BS, 1, D, False, 6)
+    tables = tables_for(lens, NB, BS, 4)
+    q = torch.randn(2, group, D, generator=torch.Generator().manual_seed(3)).to(dtype)
+    scores = ScorePool.like(pool)
+    out = pool.attend(0, q.cuda(), dev(tables), dev(np.array(lens, dtype=np.int32)), scores=scores)
+    assert_clean(ctx)
+    ref, weights, bound, spread = q4_oracle.attend(bytes_[0], D, q.double().numpy(), tables, lens, D ** -0.5)
+    check_out(out, ref, bound, spread, dtype)
+    check_scores(scores.layers[0], np.zeros((NB, 1, BS), dtype=np.float32), tables, lens, weights, spread, group)
+    scores.close()
+    with pytest.raises(ValueError, match="closed"):
+        pool.attend(0, q.cuda(), dev(tables), dev(np.array(lens, dtype=np.int32)), scores=scores)
+
+
 def test_attend_logits_far_below_zero(ctx):
     """Logits of -1e31 and less: the largest still takes all the weight, and its row comes out rounded once."""
     D, H, BS, n = 128, 1, 16, 40
