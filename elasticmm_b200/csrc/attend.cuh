@@ -1061,6 +1061,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join(const __grid_cons
 // Adds every token's weight to its score. A warp's turn is 128 tokens of a (sequence, KV head) pair, four a lane. Turns are
 // counted over the tokens that there are (max_len may be far more), so every warp has the same number, give or take one: one
 // or two of them at 131 K tokens and 8 heads, whose latencies are what the kernel costs.
+// Six blocks an SM: with eight (32 registers) 160 sequences of up to 1 500 tokens take 33.7 instead of 30.5 us.
 __global__ void __launch_bounds__(256, 6) attend_scores(const __grid_constant__ AttendArgs a) {
   grid_launch_dependents();
   grid_dependency_wait();
