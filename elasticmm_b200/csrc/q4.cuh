@@ -106,6 +106,29 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   }
 }
 
+// Two 32-bit values in one register pair, an operation on both in one instruction, each rounded as the single one is.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(lo), "f"(hi));
+  return y;
+}
+__device__ __forceinline__ void split(uint64_t x, uint32_t &lo, uint32_t &hi) { asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(x)); }
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t y;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+  return y;
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t y;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+  return y;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t y;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+  return y;
+}
+
 // Address of a token's row of head 0, or 0 when the slot is padding or outside the pool (reported).
 __device__ __forceinline__ uint64_t slot_address(const TokenSide &s, uint32_t layer, uint32_t plane, int64_t slot,
                                                  bool reporter, int *status) {
@@ -122,18 +145,20 @@ __device__ __forceinline__ uint64_t slot_address(const TokenSide &s, uint32_t la
 // ---- one thread per group of 32 channels (64 bytes), where keys and values lie on 32-byte boundaries
 //
 // Append, 32 channels per thread: 64 bytes in, 20 out. At HBM's rate an SM has about 470 issue slots per warp for that, so
-// the bound is how few instructions a channel takes (7 here):
+// the bound is how few instructions a thread takes (393 here, 12 a channel) and that enough warps wait for their loads
+// (six blocks an SM; with the five that 43 registers allow the kernel below takes 5 us longer):
 //   * smallest and largest value on packed 16-bit pairs;
 //   * the quotient d / s, d = x - o, as d times an approximate 1/s and one step of correction with the fma's remainder:
 //     that is within 2^-45 of d / s before its rounding. It rounds to the same integer as the division does: a half-integer
 //     h times s is exact (5 and 11 bits), so d / s is h itself, which the corrected quotient then is too, or d is at least
 //     one unit in its last place away from h s, which is over half a unit of h (by 2^-11 of it or more). Every 50th
 //     group of bf16 values has such an exact half, so a test with divisions behind it would run in half of all warps;
+//   * these in instructions on pairs of channels, which round each half as the single ones do (7 us of 141);
 //   * rounding by adding 1.5 * 2^23 + 8, which leaves the code in the low bits; four make a unit by integer fma;
 //   * a group with a code outside 0..15 before the clamp (an offset much larger than its range), with s = 0, infinities or
 //     NaN goes through the definition step by step.
-// Rows are put together in shared memory and leave in 16-byte pieces. 4 099 tokens x 32 layers x 8 heads of 128, bf16: 146 us
-// (4.8 TB/s).
+// Rows are put together in shared memory and leave in 16-byte pieces. 4 099 tokens x 32 layers x 8 heads of 128, bf16: 134 us
+// (5.3 TB/s).
 constexpr int kRowWarps = 8;
 
 template <typename T>
@@ -179,7 +204,7 @@ __device__ __noinline__ void encode_exact(uint64_t src, float s, float o, uint8_
 
 // grid.x * kRowWarps warps cover the T * H rows, 32 / (D/32) of them each; grid.y the layers and planes.
 template <typename T, int D>
-__global__ void __launch_bounds__(kRowWarps * 32) q4_append_rows(const __grid_constant__ Q4RowsArgs a) {
+__global__ void __launch_bounds__(kRowWarps * 32, 6) q4_append_rows(const __grid_constant__ Q4RowsArgs a) {
   grid_launch_dependents();
   grid_dependency_wait();
   constexpr int G = q4_groups(D), R = q4_row_bytes(D), kRows = 32 / G, kPieces = kRows * R / 16;
@@ -220,17 +245,17 @@ __global__ void __launch_bounds__(kRowWarps * 32) q4_append_rows(const __grid_co
   float inv;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(sf));
   exact = exact || !((lo - of) * inv > -8.25f && (hi - of) * inv < 7.25f);  // also for s = 0 and NaN
+  const uint64_t inv2 = pair(inv, inv), minus_s = pair(-sf, -sf), minus_o = pair(-of, -of);
   uint32_t unit[8];
 #pragma unroll
   for (int u = 0; u < 8; ++u) {
-    float x[4];
-    unpack2<T>(w[2 * u], x[0], x[1]);
-    unpack2<T>(w[2 * u + 1], x[2], x[3]);
     uint32_t k[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float d = __fsub_rn(x[i], of), q = __fmul_rn(d, inv);
-      k[i] = __float_as_uint(__fadd_rn(__fmaf_rn(__fmaf_rn(-q, sf, d), inv, q), 12582920.f));
+    for (int i = 0; i < 2; ++i) {
+      float x0, x1;
+      unpack2<T>(w[2 * u + i], x0, x1);
+      const uint64_t d = add_pair(pair(x0, x1), minus_o), q = mul_pair(d, inv2);
+      split(add_pair(fma_pair(fma_pair(q, minus_s, d), inv2, q), pair(12582920.f, 12582920.f)), k[2 * i], k[2 * i + 1]);
     }
     unit[u] = ((k[3] * 16u + k[2]) * 16u + k[1]) * 16u + k[0];  // its low 16 bits: the constant's are zero but for the 8
   }
@@ -259,8 +284,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) q4_append_rows(const __grid_co
   }
 }
 
-// The inverse: o + s * (c - 8), rounded once to T. HBM's writes bound it: 16 383 tokens x 28 layers x 4 heads of 128 in 209 us
-// (5.9 TB/s). A padding or reported slot gives a row of zeros.
+// The inverse: o + s * (c - 8), rounded once to T. HBM's writes bound it: 16 383 tokens x 28 layers x 4 heads of 128 in 206 us
+// (6.0 TB/s). A padding or reported slot gives a row of zeros.
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowWarps * 32) q4_read_rows(const __grid_constant__ Q4RowsArgs a) {
   grid_launch_dependents();
@@ -288,16 +313,18 @@ __global__ void __launch_bounds__(kRowWarps * 32) q4_read_rows(const __grid_cons
   const uint8_t *mem = stage[warp] + lane / G * R;
   const float s = __half2float(*reinterpret_cast<const __half *>(mem + D / 2 + 2 * r));
   const float o = __half2float(*reinterpret_cast<const __half *>(mem + D / 2 + 2 * G + 2 * r));
+  const uint64_t s2 = pair(s, s), o2 = pair(o, o);
   uint32_t w[16];
 #pragma unroll
   for (int u = 0; u < 8; ++u) {
     const uint32_t unit = *reinterpret_cast<const uint16_t *>(mem + 2 * (u * G + r));
-    float v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)  // 2^23 + c less 2^23 + 8: exact
-      v[i] = fmaf(s, __uint_as_float(0x4b000000u | (unit >> (4 * i) & 15u)) - 8388616.f, o);
-    w[2 * u] = pack2<T>(v[0], v[1]);
-    w[2 * u + 1] = pack2<T>(v[2], v[3]);
+    for (int i = 0; i < 2; ++i) {  // 2^23 + c less 2^23 + 8: exact
+      const uint64_t c = pair(__uint_as_float(0x4b000000u | (unit >> (8 * i) & 15u)), __uint_as_float(0x4b000000u | (unit >> (8 * i + 4) & 15u)));
+      uint32_t v0, v1;
+      split(fma_pair(s2, add_pair(c, pair(-8388616.f, -8388616.f)), o2), v0, v1);
+      w[2 * u + i] = pack2<T>(__uint_as_float(v0), __uint_as_float(v1));
+    }
   }
   if (!mine) return;
   const uint64_t dst = (p ? a.value + lrel * a.value_layer_stride + t * a.value_token_stride
