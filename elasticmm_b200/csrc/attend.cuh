@@ -11,22 +11,28 @@
 // channels, columns heads). A tcgen05 tile has 64 rows at least, of which a decode step could fill eight, and takes
 // its operands from shared memory, where the codes would first have to be written out as 16-bit values.
 //
-// Codes are never converted. A nibble masked in place in a 16-bit lane IS an fp16 subnormal: c * 2^-24 from bits 0..3,
-// c * 2^-20 from bits 4..7, exact, and the tensor cores take subnormals at full rate. One AND (and half a shift) makes
-// two operand elements. The two powers of two are undone in q (keys) or when the result is written (values).
+// Codes are never converted. A nibble masked in place in a 16-bit lane IS a floating-point number: c * 2^-24 from bits
+// 0..3 and c * 2^-20 from bits 4..7 as fp16 (keys), c * 2^-133 and c * 2^-129 as bf16 (values; bit 7 belongs to the
+// exponent there, but the smallest normal numbers have the subnormals' step), exact, and the tensor cores take
+// subnormals at full rate. One AND (and half a shift) makes two operand elements. The powers of two are undone in q
+// (keys) or when the result is written (values).
 //
 // Scales and offsets, x = o + s (c - 8), group r of 32 channels:
 //   l[t]   = sum_r s_r[t] (sum_d q_d c_d) + sum_r (o_r[t] - 8 s_r[t]) Q_r,      Q_r = sum of q over the group
 //            the first bracket is two MMAs per group; the last sum is one MMA (two at D = 256) with a token's scales and
 //            offsets, which lie side by side in its row, as the row operand and Q in two fp16 halves (22 bits).
 //   out[d] = sum_t (p s_r) c_d + sum_t p (o_r - 8 s_r)
-//            p s_r is formed per group as the 16-bit operand; the last sum is one MMA with scales and offsets as rows.
+//            p s_r is formed in 32 bits and enters as two bf16 parts (below); the last sum has scales and offsets as rows.
 // p is held relative to a reference that only follows the running maximum when that outgrows it by 2^6, so the
-// accumulators are rarely rescaled and no maximum is taken across lanes in between. p is scaled by 2^8 (by 2^-4 from
-// the first scale >= 2 on), which keeps p s_r below 2^15 and above fp16's subnormals down to 2^-22 of the largest.
-// fp16 outputs: p and p s_r rounded to fp16 (2^-12 each, times up to 15 s) would cost several times the output's own
-// rounding, so their remainders (exact by an fma) go through the same MMAs. bf16 outputs are 8 times coarser: without.
-// Logits, sums and accumulators are 32 bits.
+// accumulators are rarely rescaled and no maximum is taken across lanes in between.
+// Rounding. p stays in 32 bits (its fragment is transposed in two halves of 16). p s_r is cut to its first 8 bits, and
+// what is left is rounded to 8 more: two MMAs on the same codes, off by 2^-16 of p s_r at most. bf16 has the range of 32
+// bits, so no scale, however large, takes bits from a smaller one or from a lesser weight. One part would be 2^-8, more
+// than a result's own rounding; fp16 parts run out of range: with p held below 2^14 for the sake of scales of 2^13, p s_r
+// of thousands of tokens with a small scale and a small weight each was 0. Against the offsets p enters as two 11-bit
+// parts, the second times 2^12 into sums of its own: 2^-22, down to 2^-45 of the largest p.
+// Logits, sums and accumulators are 32 bits. Against 64 bits the result is off by its own rounding: 1.7e-3 (bf16) and
+// 2.1e-4 (fp16), as where all of it is computed in 32 bits.
 //
 // Work. A unit is 16 (x token subsets) tokens of one sequence for the KV heads of a CTA, one warp per head, tile of
 // query heads and subset. The units of the whole batch, counted on the device, are split evenly over the CTAs, whatever
@@ -37,10 +43,11 @@
 // SM completed one in 28 (38) ns whatever was in flight, which held the loads alone to 3.4 (4.7) TB/s; tensor boxes of 16
 // rows of 80 bytes came to 3.7 TB/s. The 16-byte copies alone reach 6 TB/s.
 //
-// Measured, D = 128, 8 KV heads, 8 query heads each, bf16: one sequence of 131 071 tokens 53 us (168 MB: 3.1 TB/s), 64 of 128
-// to 8 191 tokens 58 us, with weights 71 (the first kernel, scalar: 288 ms and 14 ms). 39 us of the 53 are the loop, whose loads alone take 27.7 and whose arithmetic alone 30.8: no unit is full (issue 39 % of cycles, ALU 39 %,
-// tensor cores 19 %), two warps a scheduler do not hide all of one another's chain from codes to products. The rest is the
-// share, the first loads, the queries and the join.
+// Measured, D = 128, 8 KV heads, 8 query heads each, bf16: one sequence of 131 071 tokens 61 us (168 MB: 2.75 TB/s), 64 of
+// 128 to 8 191 tokens with weights 81 (the first kernel, scalar: 288 ms and 14 ms). With one 16-bit part for p s_r these
+// took 53 and 71 us. Then no unit was full (issue 39 % of cycles, ALU 39 %, tensor cores 19 %): two warps a scheduler do
+// not hide all of one another's chain from codes to products, to which the second part adds. The share, the first loads,
+// the queries and the join take about 15 us.
 #pragma once
 #include "q4.cuh"
 
@@ -131,6 +138,13 @@ __device__ __forceinline__ void mma_k16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
+__device__ __forceinline__ void mma_bf16_k16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -147,10 +161,20 @@ __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
   return y;
 }
-__device__ __forceinline__ uint32_t fma_half2(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t y;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(a), "r"(b), "r"(c));
-  return y;
+// Two 32-bit values of lanes (row, 2 columns) of an 8x8 tile -> those of its transpose.
+__device__ __forceinline__ void transpose8(float &x, float &y) {
+  const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+  const uint32_t lo = transpose8(__byte_perm(a, b, 0x5410)), hi = transpose8(__byte_perm(a, b, 0x7632));
+  x = __uint_as_float(__byte_perm(lo, hi, 0x5410));
+  y = __uint_as_float(__byte_perm(lo, hi, 0x7632));
+}
+// Two 32-bit values as bf16 pairs whose sum they are to 2^-16: the first cut, the second what is left, rounded.
+__device__ __forceinline__ void split_bf16(uint64_t x, uint32_t &hi, uint32_t &lo) {
+  uint32_t a, b;
+  split(x, a, b);
+  hi = __byte_perm(a, b, 0x7632);
+  split(add_pair(x, pair(__uint_as_float((a & 0xffff0000u) ^ 0x80000000u), __uint_as_float((b & 0xffff0000u) ^ 0x80000000u))), a, b);
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(__uint_as_float(b)), "f"(__uint_as_float(a)));
 }
 // N words from shared memory at a + kOff (aligned to N words, as the row format guarantees).
 template <int N, int kOff>
@@ -225,6 +249,10 @@ constexpr uint32_t kNib0 = 0x000f000fu, kNib1 = 0x00f000f0u;
 // the nibble masks drop
 constexpr uint32_t kLoHalves = 0x5410u, kHiHalves = 0x7632u, kLoUpper = 0x5511u, kHiUpper = 0x7733u;
 constexpr float kFirstRef = -3.40282347e38f;                  // reference before any token: no finite logit is less
+constexpr float kLift = 8.f;            // p is held times 2^kLift, and is at most 2^6 of that: in fp16's range
+constexpr float kWeightUnit = 0x1p96f;  // and times this in the products p s of the values
+// What undoes the units of the value sums: a masked nibble is c * 2^-133 or c * 2^-129 as a bf16 subnormal.
+constexpr float kUnitLo = 0x1p37f, kUnitHi = 0x1p33f;
 
 // A CTA's share. The batch is a line on which every item takes kItemCost and then one place per unit; a CTA has the units
 // whose places lie in its piece of the line.
@@ -243,7 +271,7 @@ __host__ __device__ constexpr int attend_tiles(int D) { return D == 256 ? 1 : 2;
 __host__ __device__ constexpr int attend_stages(int D) { return D == 64 ? 6 : 4; }
 __host__ __device__ constexpr int attend_slot_bytes(int D) { return attend_tiles(D) * 32 * q4_row_bytes(D) + 16; }
 
-// Decode attention; see the top of the file. kPrecise: carry the remainder of p s_r (fp16 outputs).
+// Decode attention; see the top of the file.
 // kPages: blocks of 2^k >= 16 tokens (sh.block_shift >= 4), so that a tile lies in one; the branch for smaller ones in the
 // loop costs 24 sequences of 2 048-4 096 tokens and 32 heads 100.7 instead of 95.3 us.
 template <typename T, int D, bool kScores, bool kPages>
@@ -252,7 +280,6 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
   constexpr int KW = D / 32;  // words of codes per lane and token, keys (two units of every group)
   constexpr int VW = D / 64;  // words of codes per lane and token, values (one unit of every group)
   constexpr int SW = (G + 1) / 2;  // words of a token's scales
-  constexpr bool kPrecise = std::is_same<T, __half>::value;
   constexpr int kT = attend_tiles(D), kSlotBytes = attend_slot_bytes(D), kAttendStages = attend_stages(D);
   constexpr int kTile = 32 * R, kWords = kT * kTile;  // bytes of a tile; where a slot's words begin
   extern __shared__ __align__(128) unsigned char smem[];
@@ -514,7 +541,6 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
   const uint32_t mi = lane / 8, mt = lane % 8;
   const uint32_t km_at = (mt + 8 * (mi & 1)) * R + (G == 8 && mi >= 2 ? 2 * G : 0);
   const uint32_t vm_at = (16 + mt + 8 * (mi >> 1)) * R + (G == 8 && (mi & 1) ? 2 * G : 0);
-  const uint32_t scale_bits = G == 8 || g < (uint32_t)G ? 0x40004000u : 0u;  // >= 2, where this lane's rows are scales
   uint32_t slot = ring, slot_before = ring_end - kSlotBytes;  // the slot to compute on, and the one before it
 
   float *merge = reinterpret_cast<float *>(smem + sh.warps * kAttendStages * kSlotBytes);  // [(warps - warps/subsets)][8][D + 2]
@@ -594,7 +620,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
       c1 = __shfl_sync(0xffffffffu, c, 8 * q4 + 4);
     }
 
-    float acc[G][2][4], accx[4] = {0.f, 0.f, 0.f, 0.f};
+    float acc[G][2][4], accx[4] = {0.f, 0.f, 0.f, 0.f}, accy[4] = {0.f, 0.f, 0.f, 0.f};  // accy: times 2^12
 #pragma unroll
     for (int r = 0; r < G; ++r)
 #pragma unroll
@@ -602,7 +628,6 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
 #pragma unroll
         for (int k = 0; k < 4; ++k) acc[r][i][k] = 0.f;
     float ref0 = kFirstRef, ref1 = kFirstRef, sum0 = 0.f, sum1 = 0.f;
-    float lift = 8.f;  // p is held times 2^lift
     float *lg = nullptr;  // logits of head 2 q4; head 2 q4 + 1 lies one row further
     if constexpr (kScores)
       lg = a.logits + ((uint64_t)b * a.kv_heads * a.group + (uint64_t)h * a.group + j0 + 2 * q4) * a.logit_stride;
@@ -624,32 +649,36 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
           acc[r][i][2] *= f0;
           acc[r][i][3] *= f1;
         }
-      accx[0] *= f0;
-      accx[1] *= f1;
-      accx[2] *= f0;
-      accx[3] *= f1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        accx[i] *= i % 2 ? f1 : f0;
+        accy[i] *= i % 2 ? f1 : f0;
+      }
     };
+    // Row r of accx holds the sums of p s_r, the offsets' row those of p o_r.
+    auto side_sum = [&](int i) { return fmaf(accy[i], 0x1p-12f, accx[i]); };
 
     // Takes the -8 s of x = o + s (c - 8) out of the value sums so far. The tensor cores cut each sum of theirs short
     // rather than round it, by a share of its size, and sum p s c alone is much larger than what is left of it when the
     // values have no common sign: with a fixed number of tiles between two calls the loss stays below 2^-20 of sum p s c
-    // however long the sequence (24 sequences of 2 048-4 096 tokens, fp16: the result's error 2.1e-4, that of its own
-    // rounding, instead of 3.4e-4).
+    // however long the sequence. Every 64 tokens: one sequence of 131 071 tokens is off what 32-bit sums give by 2.4e-4
+    // (two bf16 results that round a few values apart; every 256 tokens 4.9e-4, and 60.3 instead of 61.0 us).
     auto recentre = [&]() {
+      const float s0 = -8.f * side_sum(0), s1 = -8.f * side_sum(1);
 #pragma unroll
       for (int r = 0; r < G; ++r) {
-        const float x0 = -8.f * __shfl_sync(0xffffffffu, accx[0], 4 * r + q4), x1 = -8.f * __shfl_sync(0xffffffffu, accx[1], 4 * r + q4);
+        const float x0 = __shfl_sync(0xffffffffu, s0, 4 * r + q4), x1 = __shfl_sync(0xffffffffu, s1, 4 * r + q4);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          acc[r][i][0] = fmaf(x0, 0x1p-24f, acc[r][i][0]);
-          acc[r][i][1] = fmaf(x1, 0x1p-24f, acc[r][i][1]);
-          acc[r][i][2] = fmaf(x0, 0x1p-20f, acc[r][i][2]);
-          acc[r][i][3] = fmaf(x1, 0x1p-20f, acc[r][i][3]);
+          acc[r][i][0] = fmaf(x0, 1.f / kUnitLo, acc[r][i][0]);
+          acc[r][i][1] = fmaf(x1, 1.f / kUnitLo, acc[r][i][1]);
+          acc[r][i][2] = fmaf(x0, 1.f / kUnitHi, acc[r][i][2]);
+          acc[r][i][3] = fmaf(x1, 1.f / kUnitHi, acc[r][i][3]);
         }
       }
-      if (g < (uint32_t)G) accx[0] = accx[1] = 0.f;  // the scales' rows
+      if (g < (uint32_t)G) accx[0] = accx[1] = accy[0] = accy[1] = 0.f;  // the scales' rows
     };
-    constexpr uint32_t kRecentre = 16 / kT;  // slots between two calls
+    constexpr uint32_t kRecentre = 4 / kT;  // slots between two calls
 
     int left = active ? (int)n - (int)(unit0 * sh.tokens + t_sub) : 0;  // tokens from this warp's next tile on
     // N tiles, the first at position n - left. kWhole: all their tokens count (mask is not read; else N = 1).
@@ -735,25 +764,17 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
           }
         }
       }
-      // ---- weights; the reference follows the maximum only when it is left 2^6 behind. From the first scale >= 2 (bit 14
-      // of an fp16) on p is held smaller.
+      // ---- weights; the reference follows the maximum only when it is left 2^6 behind
       float p[N][4], most = kFirstRef;
-      uint32_t big = 0;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        big |= m[i][0] | m[i][2];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           p[i][k] = l[i][k] - (k % 2 ? ref1 : ref0);
           most = fmaxf(most, p[i][k]);
         }
       }
-      const bool lower = (big & scale_bits) != 0 && lift > 0.f;
-      if (__builtin_expect(__any_sync(0xffffffffu, most > lift + 6.f || lower), 0)) {
-        if (__any_sync(0xffffffffu, lower)) {
-          rescale(ref0 == kFirstRef ? ref0 : ref0 + lift + 4.f, ref1 == kFirstRef ? ref1 : ref1 + lift + 4.f);
-          lift = -4.f;
-        }
+      if (__builtin_expect(__any_sync(0xffffffffu, most > kLift + 6.f), 0)) {
         float m0 = l[0][0], m1 = l[0][1];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -765,49 +786,53 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
           m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, s));
           m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, s));
         }
-        rescale(fmaxf(ref0, m0 - lift), fmaxf(ref1, m1 - lift));
+        rescale(fmaxf(ref0, m0 - kLift), fmaxf(ref1, m1 - kLift));
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
           for (int k = 0; k < 4; ++k) p[i][k] = l[i][k] - (k % 2 ? ref1 : ref0);
       }
-      uint32_t b0[N], b1[N], bl0[N], bl1[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) p[i][k] = ex2(p[i][k]);
         sum0 += p[i][0] + p[i][2];
         sum1 += p[i][1] + p[i][3];
-        const uint32_t h01 = pack_half2(p[i][0], p[i][1]), h23 = pack_half2(p[i][2], p[i][3]);
-        b0[i] = transpose8(h01);
-        b1[i] = transpose8(h23);
-        if constexpr (kPrecise) {
-          const float2 r01 = unpack_half2(h01), r23 = unpack_half2(h23);
-          bl0[i] = transpose8(pack_half2(p[i][0] - r01.x, p[i][1] - r01.y));
-          bl1[i] = transpose8(pack_half2(p[i][2] - r23.x, p[i][3] - r23.y));
-        }
+        transpose8(p[i][0], p[i][1]);  // from here on tokens tv0, tv1, tv0 + 8, tv1 + 8 of head g
+        transpose8(p[i][2], p[i][3]);
       }
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        // ---- sums of p s_r and p o_r: rows r and G + r of accx
-        mma_k16(accx, m[i][0], m[i][1], m[i][2], m[i][3], b0[i], b1[i], accx);
-        if constexpr (kPrecise) mma_k16(accx, m[i][0], m[i][1], m[i][2], m[i][3], bl0[i], bl1[i], accx);
+        // ---- sums of p s_r and p o_r: rows r and G + r of accx and accy, p in two 11-bit parts
+        {
+          const uint32_t h01 = pack_half2(p[i][0], p[i][1]), h23 = pack_half2(p[i][2], p[i][3]);
+          const float2 r01 = unpack_half2(h01), r23 = unpack_half2(h23);
+          const uint32_t l01 = pack_half2((p[i][0] - r01.x) * 0x1p12f, (p[i][1] - r01.y) * 0x1p12f);
+          const uint32_t l23 = pack_half2((p[i][2] - r23.x) * 0x1p12f, (p[i][3] - r23.y) * 0x1p12f);
+          mma_k16(accx, m[i][0], m[i][1], m[i][2], m[i][3], h01, h23, accx);
+          mma_k16(accy, m[i][0], m[i][1], m[i][2], m[i][3], l01, l23, accy);
+        }
         // ---- values
+        const uint64_t p01 = mul_pair(pair(p[i][0], p[i][1]), pair(kWeightUnit, kWeightUnit));
+        const uint64_t p23 = mul_pair(pair(p[i][2], p[i][3]), pair(kWeightUnit, kWeightUnit));
 #pragma unroll
         for (int r = 0; r < G; ++r) {
           const uint32_t sel = r % 2 ? kHiHalves : kLoHalves, up = r % 2 ? kHiUpper : kLoUpper;
-          const uint32_t s01 = __byte_perm(sv[i][0][r / 2], sv[i][1][r / 2], sel), s23 = __byte_perm(sv[i][2][r / 2], sv[i][3][r / 2], sel);
-          const uint32_t e0 = mul_half2(b0[i], s01), e1 = mul_half2(b1[i], s23);
+          float sc[4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const float2 f = unpack_half2(sv[i][t][r / 2]);
+            sc[t] = r % 2 ? f.y : f.x;
+          }
+          uint32_t e0, e1, f0, f1;
+          split_bf16(mul_pair(p01, pair(sc[0], sc[1])), e0, f0);
+          split_bf16(mul_pair(p23, pair(sc[2], sc[3])), e1, f1);
           const uint32_t u01 = __byte_perm(w[i][0][r / 2], w[i][1][r / 2], sel), u23 = __byte_perm(w[i][2][r / 2], w[i][3][r / 2], sel);
           const uint32_t y01 = __byte_perm(w[i][0][r / 2], w[i][1][r / 2], up), y23 = __byte_perm(w[i][2][r / 2], w[i][3][r / 2], up);
-          mma_k16(acc[r][0], u01 & kNib0, u01 & kNib1, u23 & kNib0, u23 & kNib1, e0, e1, acc[r][0]);
-          mma_k16(acc[r][1], y01 & kNib0, y01 & kNib1, y23 & kNib0, y23 & kNib1, e0, e1, acc[r][1]);
-          if constexpr (kPrecise) {
-            const uint32_t f0 = fma_half2(bl0[i], s01, fma_half2(b0[i], s01, e0 ^ 0x80008000u));
-            const uint32_t f1 = fma_half2(bl1[i], s23, fma_half2(b1[i], s23, e1 ^ 0x80008000u));
-            mma_k16(acc[r][0], u01 & kNib0, u01 & kNib1, u23 & kNib0, u23 & kNib1, f0, f1, acc[r][0]);
-            mma_k16(acc[r][1], y01 & kNib0, y01 & kNib1, y23 & kNib0, y23 & kNib1, f0, f1, acc[r][1]);
-          }
+          mma_bf16_k16(acc[r][0], u01 & kNib0, u01 & kNib1, u23 & kNib0, u23 & kNib1, e0, e1);
+          mma_bf16_k16(acc[r][1], y01 & kNib0, y01 & kNib1, y23 & kNib0, y23 & kNib1, e0, e1);
+          mma_bf16_k16(acc[r][0], u01 & kNib0, u01 & kNib1, u23 & kNib0, u23 & kNib1, f0, f1);
+          mma_bf16_k16(acc[r][1], y01 & kNib0, y01 & kNib1, y23 & kNib0, y23 & kNib1, f0, f1);
         }
       }
     };
@@ -845,14 +870,14 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
 #pragma unroll
     for (int r = 0; r < G; ++r) {
       const int so = G == 8 ? 4 * r : 4 * (G + r);  // lanes that hold the offsets' sums
-      const float x0 = __shfl_sync(0xffffffffu, accx[G == 8 ? 2 : 0], so + q4) - 8.f * __shfl_sync(0xffffffffu, accx[0], 4 * r + q4);
-      const float x1 = __shfl_sync(0xffffffffu, accx[G == 8 ? 3 : 1], so + q4) - 8.f * __shfl_sync(0xffffffffu, accx[1], 4 * r + q4);
+      const float x0 = __shfl_sync(0xffffffffu, side_sum(G == 8 ? 2 : 0), so + q4) - 8.f * __shfl_sync(0xffffffffu, side_sum(0), 4 * r + q4);
+      const float x1 = __shfl_sync(0xffffffffu, side_sum(G == 8 ? 3 : 1), so + q4) - 8.f * __shfl_sync(0xffffffffu, side_sum(1), 4 * r + q4);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        acc[r][i][0] = fmaf(acc[r][i][0], 0x1p24f, x0);
-        acc[r][i][1] = fmaf(acc[r][i][1], 0x1p24f, x1);
-        acc[r][i][2] = fmaf(acc[r][i][2], 0x1p20f, x0);
-        acc[r][i][3] = fmaf(acc[r][i][3], 0x1p20f, x1);
+        acc[r][i][0] = fmaf(acc[r][i][0], kUnitLo, x0);
+        acc[r][i][1] = fmaf(acc[r][i][1], kUnitLo, x1);
+        acc[r][i][2] = fmaf(acc[r][i][2], kUnitHi, x0);
+        acc[r][i][3] = fmaf(acc[r][i][3], kUnitHi, x1);
       }
     }
     if (sh.subsets > 1) {
