@@ -491,10 +491,9 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
     if (__builtin_expect(run == 0 && after > 0, 0)) {
       begin_run();
       if (run == 0) load_rest(slot);
-    } else if (__builtin_expect(run > 0 && holes, 0)) {
-      by_length(slot);
     }
     if (run > 0) {
+      if (__builtin_expect(holes, 0)) by_length(slot);  // the words may be an earlier tile's masks
 #pragma unroll
       for (int i = 0; i < kT; ++i) {
         const uint32_t t = it + 16 * i;
