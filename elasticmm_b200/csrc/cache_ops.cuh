@@ -214,20 +214,27 @@ AttendWorkspace attend_workspace(const emm::AttendShape &s, int32_t D, int32_t B
   return w;
 }
 
-// Launches the main kernel; its dynamic shared memory is raised to the device's limit once per device.
-template <typename T, int D, bool kScores, bool kPages>
-int attend_main(emm_ctx *ctx, const emm::AttendArgs &a, int smem, cudaStream_t st) {
+// Raises a kernel's dynamic shared memory to the device's limit, once per device. Without it a block's static and dynamic
+// shared memory together have 48 KiB, so a kernel whose dynamic part comes near that needs it too.
+template <auto kKernel>
+int allow_smem(emm_ctx *ctx, int smem, const char *what) {
   const int device = ctx->device;
   static std::atomic<int> limit[kMaxTrackedDevices];
   const bool tracked = device >= 0 && device < kMaxTrackedDevices;
   if (!tracked || limit[device].load(std::memory_order_acquire) < smem) {
     cudaFuncAttributes fa;
-    EMM_CUDA(cudaFuncGetAttributes(&fa, emm::attend_q4<T, D, kScores, kPages>));
+    EMM_CUDA(cudaFuncGetAttributes(&fa, kKernel));
     const int most = ctx->max_smem_optin - (int)fa.sharedSizeBytes;
-    if (smem > most) return fail(EMM_ERR_TOO_LARGE, "q4_attend: %d bytes of shared memory, the device has %d", smem, most);
-    EMM_CUDA(cudaFuncSetAttribute(emm::attend_q4<T, D, kScores, kPages>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    if (smem > most) return fail(EMM_ERR_TOO_LARGE, "%s: %d bytes of shared memory, the device has %d", what, smem, most);
+    EMM_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     if (tracked) limit[device].store(most, std::memory_order_release);
   }
+  return EMM_OK;
+}
+
+template <typename T, int D, bool kScores, bool kPages>
+int attend_main(emm_ctx *ctx, const emm::AttendArgs &a, int smem, cudaStream_t st) {
+  if (int rc = allow_smem<emm::attend_q4<T, D, kScores, kPages>>(ctx, smem, "q4_attend")) return rc;
   return launch_after(ctx, emm::attend_q4<T, D, kScores, kPages>, dim3(a.sh.grid), a.sh.warps * 32, (size_t)smem, st, true, a);
 }
 
@@ -421,8 +428,7 @@ int emm_select_tokens(emm_pool *scores, const int32_t *d_block_tables, int64_t t
   // Small CTAs where a thread has at most 16 keys: eight CTAs share an SM then, and one's barriers hide behind the others'
   // (2 048 CTAs of 3 000-4 096 keys: 61 us, with 1 024 threads 76; 10 000 keys: 1 024 threads 11 us faster than 256).
   if (most <= 4096) return launch_after(ctx, emm::select_tokens<256, true>, grid, 256, keys, st, true, a);
-  if (keys > 48 * 1024)
-    EMM_CUDA(cudaFuncSetAttribute(emm::select_tokens<1024, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectSharedMax));
+  if (int rc = allow_smem<emm::select_tokens<1024, true>>(ctx, (int)keys, what)) return rc;
   return launch_after(ctx, emm::select_tokens<1024, true>, grid, 1024, keys, st, true, a);
 }
 

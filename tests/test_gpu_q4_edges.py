@@ -1,4 +1,8 @@
 """Calls of the 4-bit cache and of token eviction at the edges of what their documents allow, against the restatement."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -56,3 +60,32 @@ def test_a_bad_block_hides_no_later_tokens_of_its_sequence(ctx, D, BS, dtype, ba
     ref, _, bound, spread = q4_oracle.attend(bytes_[0], D, q.double().numpy(), np.delete(table, bad_place, 1), [n - BS], D ** -0.5)
     check_out(out, ref, bound, spread, dtype)
     assert_clean(ctx)
+
+
+# ------------------------------------------------------------------------------------------------- token selection
+_FIRST_SELECTION = """
+import sys
+import numpy as np, torch
+from elasticmm_b200 import ScorePool
+from oracle import q4_oracle
+n, BS = int(sys.argv[1]), int(sys.argv[2])
+values = np.random.default_rng(n).random((1, n // BS, 1, BS), dtype=np.float32)
+scores = ScorePool([torch.from_numpy(values[0]).cuda()])
+tables = np.random.default_rng(1).permutation(n // BS).astype(np.int32)[None]
+index, lens = scores.select_tokens(torch.from_numpy(tables).cuda(), torch.tensor([n], dtype=torch.int32, device="cuda"),
+                                   500, recent=20, sink=3)
+assert (index.cpu().numpy() == q4_oracle.select_tokens(values, tables, [n], 500, 20, 3)).all()
+assert lens.tolist() == [500]
+scores.ctx.check_status()
+print("selected")
+"""
+
+
+@pytest.mark.parametrize("n,BS", [(11680, 16), (11681, 1), (12288, 16), (12289, 1), (51200, 16), (51201, 1)])
+def test_the_first_selection_of_a_process(n, BS):
+    """Tables of every capacity launch without a larger call before them: around 48 KiB of keys, with and without the
+    kernel's static shared memory, and around the most keys that are held at all."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", _FIRST_SELECTION, str(n), str(BS)], cwd=root, capture_output=True, text=True,
+                         timeout=300, env={**os.environ, "PYTHONPATH": root})
+    assert run.returncode == 0 and "selected" in run.stdout, run.stderr[-2000:]
