@@ -186,17 +186,18 @@ class KVPoolQ4(KVPool):
 
     def bind_append(self, key: torch.Tensor, value: torch.Tensor, slot_mapping: torch.Tensor):
         """Pre-validated per-layer append over static [L, T, H, D] buffers (see KVPool.bind_append):
-        returns append(layer, stream=None)."""
+        returns append(layer, stream=None), which is refused once the pool is closed or `append.release()` was called."""
         T, dt, (kls, kts, vls, vts) = self._check_rows(key, value, slot_mapping, 1)
         if key.shape[0] != self.num_layers:
             raise ValueError(f"key has {key.shape[0]} layers, pool has {self.num_layers}")
-        fn, h, device, L = self._emm_q4_append, self._h, self.ctx.device, self.num_layers
+        fn, device, L, pool = self._emm_q4_append, self.ctx.device, self.num_layers, self
         D, k, v, s = self.head_dim, key.data_ptr(), value.data_ptr(), slot_mapping.data_ptr()
 
         def raw(layer: int, stream: int) -> int:
             if not 0 <= layer < L:  # the addresses below are per layer
                 return _lib.ERR_BAD_ARG
-            return fn(h, D, dt, layer, 1, k + layer * kls, v + layer * vls, 0, kts, 0, vts, s, T, stream)
+            # the pool's handle is looked up in each call: a closed pool's is null, which the library refuses
+            return fn(pool and pool._h, D, dt, layer, 1, k + layer * kls, v + layer * vls, 0, kts, 0, vts, s, T, stream)
 
         def append(layer: int, stream: Optional[int] = None) -> None:
             if not 0 <= layer < L:
@@ -205,8 +206,13 @@ class KVPoolQ4(KVPool):
             if rc:
                 _lib.check(rc)
 
+        def release() -> int:
+            nonlocal pool
+            pool = None
+            return _lib.OK
+
         append.buffers = (key, value, slot_mapping, self)
-        append.release = lambda: _lib.OK
+        append.release = release
         append.raw = raw
         return append
 

@@ -135,3 +135,40 @@ def test_truncated_tables_give_their_blocks_back():
         bm.truncate_blocks("b", 3)
     with pytest.raises(ValueError):
         bm.truncate_blocks("a", -1)
+
+
+def _bound_append(L=2, H=1, D=64):
+    """A bound append of a pool without a GPU: (append, pool, calls that reached the library with the pool's handle)."""
+    calls, lib = [], _lib.load()
+
+    def entry(handle, *args):
+        if handle is None:
+            return lib.emm_q4_append(handle, *args)
+        calls.append((handle, *args))
+        return _lib.OK
+
+    pool = KVPoolQ4.__new__(KVPoolQ4)
+    pool._h, pool.num_layers, pool.num_kv_heads, pool.head_dim = 77, L, H, D
+    pool.ctx = types.SimpleNamespace(device=torch.device("cpu"), _lib=types.SimpleNamespace(emm_pool_destroy=lambda h: _lib.OK))
+    pool._emm_q4_append = entry
+    kv = torch.zeros(L, 3, H, D, dtype=torch.float16)
+    return pool.bind_append(kv, kv.clone(), torch.arange(3)), pool, calls
+
+
+def test_a_bound_append_ends_with_its_pool():
+    append, pool, calls = _bound_append()
+    append(1, 0)
+    assert append.raw(0, 0) == _lib.OK and [c[0] for c in calls] == [77, 77]
+    pool.close()
+    with pytest.raises(_lib.EmmError, match="null pool"):
+        append(0, 0)
+    assert append.raw(1, 0) == _lib.ERR_BAD_ARG and len(calls) == 2
+
+
+def test_a_released_append_is_refused():
+    append, pool, calls = _bound_append()
+    assert append.release() == _lib.OK and append.release() == _lib.OK
+    with pytest.raises(_lib.EmmError, match="null pool"):
+        append(0, 0)
+    assert append.raw(1, 0) == _lib.ERR_BAD_ARG and calls == []
+    pool.close()
