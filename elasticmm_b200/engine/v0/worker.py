@@ -201,6 +201,8 @@ class V0Worker:
             return self._require_pool().gather(block_indices)
 
     def write_kv_blocks(self, block_indices: List[int], kv_data: torch.Tensor) -> None:
+        """Writes packed blocks into the pool. After init_scores the blocks' weights start from zero, whoever had the
+        blocks before; a caller that brings weights along scatters them behind this call."""
         pool = self._require_pool()
         assert kv_data.shape[2] == len(block_indices), (
             f"Block count mismatch: {kv_data.shape[2]} vs {len(block_indices)}")
@@ -209,6 +211,18 @@ class V0Worker:
                 self._quantize_kv_blocks(block_indices, kv_data)
             else:
                 pool.scatter(block_indices, kv_data)
+            self._reset_block_scores(block_indices)
+
+    def _block_slots(self, block_indices) -> torch.Tensor:
+        """The slots of the blocks' tokens, in order (int64, on the device)."""
+        pool = self._require_pool()
+        on_device = isinstance(block_indices, torch.Tensor) and block_indices.is_cuda
+        first = (block_indices if on_device else pool.upload_ids(_as_host_ids(block_indices))).long() * pool.block_size
+        return (first[:, None] + torch.arange(pool.block_size, device=self.device)).flatten()
+
+    def _reset_block_scores(self, block_indices) -> None:
+        if self.scores is not None and len(block_indices):
+            self.scores.reset(self._block_slots(block_indices))
 
     def _quantize_kv_blocks(self, block_indices: List[int], kv_data: torch.Tensor) -> None:
         """write_kv_blocks of a 16-bit worker's blocks into a 4-bit pool: [L, 2, n, BS, H, D] fp16 or bf16."""
@@ -217,9 +231,7 @@ class V0Worker:
         want = (pool.num_layers, 2, n, bs, pool.num_kv_heads, pool.head_dim)
         if tuple(kv_data.shape) != want:
             raise ValueError(f"packed tensor has shape {tuple(kv_data.shape)}, expected {want}")
-        host = pool._validated(_as_host_ids(block_indices), unique=True)
-        first = pool.upload_ids(host).long() * bs
-        slots = (first[:, None] + torch.arange(bs, device=self.device)).flatten()
+        slots = self._block_slots(pool._validated(_as_host_ids(block_indices), unique=True))
         # a head-major worker's blocks are a permuted view: made token-major first
         rows = kv_data if kv_data.is_contiguous() else kv_data.contiguous()
         pool.append_all_layers(rows[:, 0].flatten(1, 2), rows[:, 1].flatten(1, 2), slots)
@@ -231,9 +243,7 @@ class V0Worker:
         if self.kv_bits != 4:
             raise RuntimeError("read_kv_blocks is for a 4-bit pool; use extract_kv_blocks")
         n, bs = len(block_indices), pool.block_size
-        host = pool._validated(_as_host_ids(block_indices))
-        first = pool.upload_ids(host).long() * bs
-        slots = (first[:, None] + torch.arange(bs, device=self.device)).flatten()
+        slots = self._block_slots(pool._validated(_as_host_ids(block_indices)))
         key, value = pool.read(slots, _DTYPES[self.dtype])
         shape = (pool.num_layers, n, bs, pool.num_kv_heads, pool.head_dim)
         return torch.stack([key.view(shape), value.view(shape)], dim=1)
@@ -250,6 +260,8 @@ class V0Worker:
             assert data.shape[2] == len(ids), f"Block count mismatch: {data.shape[2]} vs {len(ids)}"
         with _range("emm.write_kv_blocks_many"):
             self._require_pool().scatter_many(block_index_lists, kv_data)
+            if self.scores is not None:
+                self._reset_block_scores([i for ids in block_index_lists for i in ids])
 
     def get_kv_cache_layout(self) -> Dict[str, Any]:
         if not self.kv_cache:
