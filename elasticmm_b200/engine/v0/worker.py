@@ -19,6 +19,7 @@ import os
 import time
 from typing import Any, Dict, List, Optional, Sequence, Tuple
 
+import numpy as np
 import torch
 import torch.distributed as dist
 
@@ -208,7 +209,7 @@ class V0Worker:
             f"Block count mismatch: {kv_data.shape[2]} vs {len(block_indices)}")
         with _range("emm.write_kv_blocks"):
             if self.kv_bits == 4 and kv_data.dtype != torch.uint8:
-                self._quantize_kv_blocks(block_indices, kv_data)
+                self._quantize_kv_blocks([block_indices], [kv_data])
             else:
                 pool.scatter(block_indices, kv_data)
             self._reset_block_scores(block_indices)
@@ -224,17 +225,25 @@ class V0Worker:
         if self.scores is not None and len(block_indices):
             self.scores.reset(self._block_slots(block_indices))
 
-    def _quantize_kv_blocks(self, block_indices: List[int], kv_data: torch.Tensor) -> None:
-        """write_kv_blocks of a 16-bit worker's blocks into a 4-bit pool: [L, 2, n, BS, H, D] fp16 or bf16."""
+    def _quantize_kv_blocks(self, block_index_lists: Sequence[List[int]], kv_data: Sequence[torch.Tensor]) -> None:
+        """16-bit workers' blocks, [L, 2, n, BS, H, D] fp16 or bf16 per request, into a 4-bit pool: all are checked first."""
         pool = self._require_pool()
-        n, bs = len(block_indices), pool.block_size
-        want = (pool.num_layers, 2, n, bs, pool.num_kv_heads, pool.head_dim)
-        if tuple(kv_data.shape) != want:
-            raise ValueError(f"packed tensor has shape {tuple(kv_data.shape)}, expected {want}")
-        slots = self._block_slots(pool._validated(_as_host_ids(block_indices), unique=True))
-        # a head-major worker's blocks are a permuted view: made token-major first
-        rows = kv_data if kv_data.is_contiguous() else kv_data.contiguous()
-        pool.append_all_layers(rows[:, 0].flatten(1, 2), rows[:, 1].flatten(1, 2), slots)
+        if len(block_index_lists) != len(kv_data):
+            raise ValueError(f"{len(kv_data)} packed tensors for {len(block_index_lists)} id lists")
+        hosts = [_as_host_ids(ids) for ids in block_index_lists]
+        for host, data in zip(hosts, kv_data):
+            want = (pool.num_layers, 2, len(host), pool.block_size, pool.num_kv_heads, pool.head_dim)
+            if tuple(data.shape) != want:
+                raise ValueError(f"packed tensor has shape {tuple(data.shape)}, expected {want}")
+            if data.dtype not in (torch.float16, torch.bfloat16) or data.device != pool.device:
+                raise ValueError("packed tensors that are quantised are float16 or bfloat16 on the worker's device, got "
+                                 f"{data.dtype} on {data.device}")
+        all_slots = self._block_slots(pool._validated(np.concatenate(hosts), unique=True))
+        for slots, data in zip(all_slots.split([len(host) * pool.block_size for host in hosts]), kv_data):
+            # a head-major worker's blocks are a permuted view: made token-major first
+            rows = data if data.is_contiguous() else data.contiguous()
+            if slots.numel():
+                pool.append_all_layers(rows[:, 0].flatten(1, 2), rows[:, 1].flatten(1, 2), slots)
 
     def read_kv_blocks(self, block_indices: List[int]) -> torch.Tensor:
         """The blocks of a 4-bit pool as [L, 2, n, BS, H, D] of the worker's dtype, for a 16-bit consumer
@@ -255,11 +264,15 @@ class V0Worker:
 
     def write_kv_blocks_many(self, block_index_lists: Sequence[List[int]], kv_data: Sequence[torch.Tensor]) -> None:
         """write_kv_blocks for several requests with one launch; `kv_data` as returned by
-        extract_kv_blocks_many (possibly of another worker on the same GPU)."""
+        extract_kv_blocks_many (possibly of another worker on the same GPU). A 4-bit worker takes 16-bit blocks too,
+        with one launch per request."""
         for ids, data in zip(block_index_lists, kv_data):
             assert data.shape[2] == len(ids), f"Block count mismatch: {data.shape[2]} vs {len(ids)}"
         with _range("emm.write_kv_blocks_many"):
-            self._require_pool().scatter_many(block_index_lists, kv_data)
+            if self.kv_bits == 4 and any(data.dtype != torch.uint8 for data in kv_data):
+                self._quantize_kv_blocks(block_index_lists, kv_data)
+            else:
+                self._require_pool().scatter_many(block_index_lists, kv_data)
             if self.scores is not None:
                 self._reset_block_scores([i for ids in block_index_lists for i in ids])
 

@@ -1,9 +1,11 @@
 """Blocks that enter a 4-bit worker: whose weights they have, one request or several at a time, from 16 bits or 4."""
+import asyncio
+
 import numpy as np
 import pytest
 import torch
 
-from elasticmm_b200.engine.v0 import V0Worker
+from elasticmm_b200.engine.v0 import TransferMethod, V0KVTransferManager, V0Worker
 from test_gpu_q4_worker import BS, D, H, L, NB, _worker
 
 pytestmark = pytest.mark.gpu
@@ -59,3 +61,53 @@ def test_an_eviction_after_a_hand_over_goes_by_the_new_requests_weights():
         layer[17, :, 5] = 1e-3  # position 37 was looked at, no other
     res = w.evict_tokens(tables, torch.tensor([3 * BS], dtype=torch.int32, device="cuda"), 2)
     assert (res["index"].cpu() == torch.tensor([0, 37])).all()
+
+
+@pytest.mark.parametrize("layout", ["nhd", "hnd"])
+@pytest.mark.parametrize("source", ["nhd", "hnd"])
+def test_several_requests_of_a_16_bit_worker_enter_together(layout, source):
+    """write_kv_blocks_many holds what write_kv_blocks does request by request, and takes all of a call or nothing."""
+    wide = V0Worker(dtype="bfloat16", device="cuda:0", block_size=BS)
+    wide.init_kvcache(NB, L, H, D, layout=source)
+    for t in wide.kv_cache:
+        t.normal_()
+    one, many = _worker(layout), _worker(layout)
+    src, dst = [[5, 0, 23], [], [7], [1, 2]], [[1, 22, 3], [], [9], [0, 14]]
+    parts = wide.extract_kv_blocks_many(src)
+    many.write_kv_blocks_many(dst, parts)
+    for s, d in zip(src, dst):
+        if s:
+            one.write_kv_blocks(d, wide.extract_kv_blocks(s))
+    for a, b in zip(one.kv_cache, many.kv_cache):
+        assert torch.equal(a, b)
+    held = [t.clone() for t in many.kv_cache]
+    other = wide.extract_kv_blocks_many([[3], [4, 6]])
+    for ids, data in (([[3], [3, 4]], other), ([[3], [4, NB]], other), ([[3], [4]], other), ([[3]], other),
+                      ([[3], [4, 6]], [other[0], other[1].float()]), ([[3], [4, 6]], [other[0], other[1].cpu()]),
+                      ([[3], [4, 6]], [other[0], many.extract_kv_blocks([4, 6])])):
+        with pytest.raises(Exception):
+            many.write_kv_blocks_many(ids, data)
+        assert all(torch.equal(a, b) for a, b in zip(held, many.kv_cache))
+    many.write_kv_blocks_many([], [])
+    many.write_kv_blocks_many([[3], [4]], one.extract_kv_blocks_many([[22], [0]]))  # bytes, as before
+    assert torch.equal(many.extract_kv_blocks([3, 4]), one.extract_kv_blocks([22, 0]))
+    many.ctx.check_status()
+
+
+def test_a_transfer_into_4_bits_does_the_same_with_and_without_batching():
+    wide = V0Worker(dtype="bfloat16", device="cuda:0", block_size=BS)
+    wide.init_kvcache(NB, L, H, D)
+    for t in wide.kv_cache:
+        t.normal_()
+    got = []
+    for batching in (False, True):
+        w = _worker()
+        mgr = V0KVTransferManager(transfer_method=TransferMethod.P2P_COPY, enable_batching=batching, batch_size=2,
+                                  batch_timeout=3600.0)
+        mgr.register_worker(0, wide, "prefill")
+        mgr.register_worker(1, w, "decoding")
+        for i, (s, d) in enumerate((([0, 4], [8, 1]), ([2], [3]), ([9, 7, 6], [0, 2, 20]))):
+            assert asyncio.run(mgr.transfer_kv_cache(f"r{i}", 0, 1, s, d)), mgr.last_result
+        assert mgr.flush(), mgr.last_result
+        got.append([t.clone() for t in w.kv_cache])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
