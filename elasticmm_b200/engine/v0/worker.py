@@ -594,14 +594,15 @@ class V0Worker:
         sender gathers its blocks into one flat message and broadcasts it from `root`; a
         receiver takes the broadcast and scatters it into `block_indices`. `group_name` is a
         torch.distributed process group (or None for the default group) where the reference
-        passes the name of a Ray collective group.
+        passes the name of a Ray collective group. The blocks of a 4-bit pool are sent as the bytes they are
+        (dtype "uint8"); a 4-bit receiver takes a 16-bit sender's blocks too and quantises them.
         """
         key = dtype.replace("torch.", "").lower()
         names = {"float16": torch.float16, "half": torch.float16, "fp16": torch.float16,
                  "bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32,
-                 "fp32": torch.float32}
-        if key not in names:
-            raise ValueError(f"[V0Worker] Unsupported dtype for collective transfer: {dtype}")
+                 "fp32": torch.float32, "uint8": torch.uint8}
+        if key not in names or (key == "uint8" if self.kv_bits != 4 else key != "uint8" and mode == "send"):
+            raise ValueError(f"[V0Worker] Unsupported dtype for collective transfer: {dtype} ({self.kv_bits}-bit pool)")
         group = None if isinstance(group_name, str) else group_name
         shape = tuple(int(d) for d in tensor_shape)
         if mode == "send":

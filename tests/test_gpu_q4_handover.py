@@ -111,3 +111,38 @@ def test_a_transfer_into_4_bits_does_the_same_with_and_without_batching():
         assert mgr.flush(), mgr.last_result
         got.append([t.clone() for t in w.kv_cache])
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_the_broadcast_form_moves_4_bit_blocks_as_bytes(monkeypatch):
+    message = []
+
+    def broadcast(t, src, group):
+        if sending:
+            message.append(t.clone())
+        else:
+            assert t.dtype == message[-1].dtype
+            t.copy_(message[-1])
+
+    monkeypatch.setattr("torch.distributed.broadcast", broadcast)
+    a, b = _worker(), _worker("hnd")
+    wide = V0Worker(dtype="bfloat16", device="cuda:0", block_size=BS)
+    wide.init_kvcache(NB, L, H, D)
+    for t in wide.kv_cache:
+        t.normal_()
+    a.write_kv_blocks([1, 2, 3], _blocks(3, 7))
+    packed = a.extract_kv_blocks([3, 1])
+    sending = True
+    res = a.collective_transfer_kv(None, 0, [3, 1], packed.shape, "torch.uint8", "send")
+    assert res["bytes"] == packed.numel()
+    sending = False
+    a.collective_transfer_kv(None, 0, [8, 9], packed.shape, a.get_kv_cache_layout()["dtype"], "recv")
+    assert torch.equal(a.extract_kv_blocks([8, 9]), packed)
+    sending = True
+    wide.collective_transfer_kv(None, 0, [4, 0], (L, 2, 2, BS, H, D), "bfloat16", "send")
+    sending = False
+    b.collective_transfer_kv(None, 0, [5, 6], (L, 2, 2, BS, H, D), "bfloat16", "recv")
+    a.write_kv_blocks([5, 6], wide.extract_kv_blocks([4, 0]))
+    assert torch.equal(b.read_kv_blocks([5, 6]), a.read_kv_blocks([5, 6]))
+    for worker, dtype, mode in ((a, "bfloat16", "send"), (wide, "uint8", "send"), (wide, "uint8", "recv"), (a, "int8", "recv")):
+        with pytest.raises(ValueError, match="Unsupported dtype"):
+            worker.collective_transfer_kv(None, 0, [0], (1,), dtype, mode)
