@@ -70,9 +70,9 @@ struct AttendShape {
 };
 
 // What an item costs besides its units, in units: queries, the subsets' meeting, the result (measured: 3 us against
-// 1.2 us for a unit of 32 tokens and 8 heads). With 1 the CTAs with many short sequences finish last: 64 sequences of
-// 128-8 191 tokens 74.6 instead of 71.4 us.
-constexpr uint32_t kItemCost = 3;
+// 1.8 us for a unit of 32 tokens and 8 heads). 64 sequences of 128-8 191 tokens 80.6 us, 160 of up to 1 500 31.4; with 1
+// 81.7 and 32.5, with 3 81.6 and 32.1.
+constexpr uint32_t kItemCost = 2;
 
 constexpr uint32_t kScoreTokens = 128;  // tokens of a warp's turn in attend_scores
 
@@ -272,9 +272,7 @@ __host__ __device__ constexpr int attend_stages(int D) { return D == 64 ? 6 : 4;
 __host__ __device__ constexpr int attend_slot_bytes(int D) { return attend_tiles(D) * 32 * q4_row_bytes(D) + 16; }
 
 // Decode attention; see the top of the file.
-// kPages: blocks of 2^k >= 16 tokens (sh.block_shift >= 4), so that a tile lies in one; the branch for smaller ones in the
-// loop costs 24 sequences of 2 048-4 096 tokens and 32 heads 100.7 instead of 95.3 us.
-template <typename T, int D, bool kScores, bool kPages>
+template <typename T, int D, bool kScores>
 __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_constant__ AttendArgs a) {
   constexpr int G = q4_groups(D), R = q4_row_bytes(D);
   constexpr int KW = D / 32;  // words of codes per lane and token, keys (two units of every group)
@@ -375,7 +373,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
   }
   const uint32_t tail_lane = R % 32 == 0 || lane < R % 32;  // has a chunk in the last, partial round
   const uint32_t shift = (uint32_t)sh.block_shift & 31u, block_mask = (1u << shift) - 1u;
-  const bool paged = kPages || sh.block_shift >= 0;
+  const bool paged = sh.block_shift >= 0;
   bool holes = false;              // a block outside the pool was met
   // Where the next slot's tokens lie. `run` slots from here on hold whole tiles of one block each, their blocks at hand
   // in `ids`; `after` more units of the item follow in the share.
@@ -416,7 +414,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
     if (!paged || !ireal || it + 16 * kT > in) return;
     const uint32_t far = (it >> shift) - window;
     if (far >= 32) {
-      if (kPages || far < 64) {  // a unit has at most 256 tokens: 32 blocks of 8
+      if (far < 64) {  // a unit has at most 256 tokens: 32 blocks of 8
         window += 32;
         ids = ids_next;
       } else {
@@ -427,7 +425,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
     }
     if (__any_sync(0xffffffffu, (uint32_t)ids >= a.pool.num_blocks)) return;
     // slots begin at multiples of 16 kT tokens, so a slot's blocks (32 at most) lie in one window
-    if (!kPages && shift < 4) {
+    if (shift < 4) {
       small = true;
       return;
     }
@@ -442,7 +440,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
     for (uint32_t i = 0; i < kT; ++i) {
       const uint32_t t = it + 16 * i, to = slot + i * kTile;
       uint32_t word = kByLength;
-      if (!kPages && small) {
+      if (small) {
 #pragma unroll
         for (int j = 0; j < kCopies; ++j) {
           const uint32_t c = min(lane + 32 * j, (uint32_t)(16 * kChunks - 1)), at = t + c / kChunks;
@@ -457,7 +455,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
       } else if (t < in && ireal) {
         const uint32_t count = min(16u, in - t);
         auto row_at = [&](uint32_t row) -> uint64_t {
-          const uint32_t blk = kPages ? (t + row) >> shift : (t + row) / a.pool.block_size;
+          const uint32_t blk = paged ? (t + row) >> shift : (t + row) / a.pool.block_size;
           const int32_t id = itab[blk];
           if ((uint32_t)id >= a.pool.num_blocks) {
             report(a.status, kStatusIdRange, id);
@@ -979,8 +977,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 1) attend_q4(const __grid_c
 
 // Adds the partial results of the items that several CTAs worked on. grid.x: items, or (by_cta) the CTAs that finished
 // one; grid.y x kHeads: the query heads of an item. kJoinWarps / kHeads warps share a head's parts, all 16 where few items
-// have many parts (131 071 tokens: the whole call 53.9 us, with two warps 62.0), two where many have few (64 sequences: 71.4
-// us, with 16 warps 100.8). One round of loads each: latency bounds it.
+// have many parts (131 071 tokens: the whole call 61.4 us, with two warps 69.5), two where many have few (64 sequences: 81
+// us, with 16 warps 110.5). One round of loads each: latency bounds it.
 constexpr int kJoinWarps = 16;
 
 template <typename T, int D, int kHeads>
@@ -1085,7 +1083,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join(const __grid_cons
 // Adds every token's weight to its score. A warp's turn is 128 tokens of a (sequence, KV head) pair, four a lane. Turns are
 // counted over the tokens that there are (max_len may be far more), so every warp has the same number, give or take one: one
 // or two of them at 131 K tokens and 8 heads, whose latencies are what the kernel costs.
-// Six blocks an SM: with eight (32 registers) 160 sequences of up to 1 500 tokens take 33.7 instead of 30.5 us.
+// Six blocks an SM: with eight (32 registers) 160 sequences of up to 1 500 tokens take 35.1 instead of 32.1 us.
 __global__ void __launch_bounds__(256, 6) attend_scores(const __grid_constant__ AttendArgs a) {
   grid_launch_dependents();
   grid_dependency_wait();

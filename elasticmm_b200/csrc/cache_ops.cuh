@@ -172,7 +172,7 @@ int attend_shape(const emm_pool *pool, int32_t D, int32_t B, int32_t group, int3
     const uint32_t tokens = 16 * (uint32_t)emm::attend_tiles(D) * s.subsets;
     return std::max<uint64_t>(1, ((uint64_t)max_len + tokens - 1) / tokens) * s.items;
   };
-  // Little work is spread over more, smaller CTAs (577 tokens of one sequence: the call 14.0 us, otherwise 19.5).
+  // Little work is spread over more, smaller CTAs (577 tokens of one sequence, in a graph: 8.9 us, otherwise 10.0).
   while (s.subsets > 1 && units() < sms) s.subsets /= 2;
   s.tokens = 16 * (uint32_t)emm::attend_tiles(D) * s.subsets;
   s.warps = s.heads_cta * s.ntiles * s.subsets;
@@ -232,17 +232,15 @@ int allow_smem(emm_ctx *ctx, int smem, const char *what) {
   return EMM_OK;
 }
 
-template <typename T, int D, bool kScores, bool kPages>
+template <typename T, int D, bool kScores>
 int attend_main(emm_ctx *ctx, const emm::AttendArgs &a, int smem, cudaStream_t st) {
-  if (int rc = allow_smem<emm::attend_q4<T, D, kScores, kPages>>(ctx, smem, "q4_attend")) return rc;
-  return launch_after(ctx, emm::attend_q4<T, D, kScores, kPages>, dim3(a.sh.grid), a.sh.warps * 32, (size_t)smem, st, true, a);
+  if (int rc = allow_smem<emm::attend_q4<T, D, kScores>>(ctx, smem, "q4_attend")) return rc;
+  return launch_after(ctx, emm::attend_q4<T, D, kScores>, dim3(a.sh.grid), a.sh.warps * 32, (size_t)smem, st, true, a);
 }
 
 template <typename T, int D>
 int attend_launch(emm_ctx *ctx, const emm::AttendArgs &a, int smem, cudaStream_t st) {
-  const bool pages = a.sh.block_shift >= 4;
-  const int rc = a.score_base ? (pages ? attend_main<T, D, true, true>(ctx, a, smem, st) : attend_main<T, D, true, false>(ctx, a, smem, st))
-                              : (pages ? attend_main<T, D, false, true>(ctx, a, smem, st) : attend_main<T, D, false, false>(ctx, a, smem, st));
+  const int rc = a.score_base ? attend_main<T, D, true>(ctx, a, smem, st) : attend_main<T, D, false>(ctx, a, smem, st);
   if (rc) return rc;
   if (a.max_len > a.sh.tokens) {  // else every item is one unit, which no CTA shares
     const bool by_cta = a.sh.items > a.sh.grid;
