@@ -44,10 +44,12 @@
 // rows of 80 bytes came to 3.7 TB/s. The 16-byte copies alone reach 6 TB/s.
 //
 // Measured, D = 128, 8 KV heads, 8 query heads each, bf16: one sequence of 131 071 tokens 61 us (168 MB: 2.75 TB/s), 64 of
-// 128 to 8 191 tokens with weights 81 (the first kernel, scalar: 288 ms and 14 ms). With one 16-bit part for p s_r these
-// took 53 and 71 us. Then no unit was full (issue 39 % of cycles, ALU 39 %, tensor cores 19 %): two warps a scheduler do
-// not hide all of one another's chain from codes to products, to which the second part adds. The share, the first loads,
-// the queries and the join take about 15 us.
+// 128 to 8 191 tokens 65 us, with weights 81 (the first kernel, scalar: 288 ms and 14 ms). With one 16-bit part for p s_r
+// these took 53, 58 and 71. 49 us of the 61 are the loop, whose loads alone take 28 and whose arithmetic alone 39: no unit
+// is full (issue 43 % of cycles, ALU 40 %, tensor cores 24 %), two warps a scheduler do not hide all of one another's
+// chain from codes to products. The rest is the share, the first loads, the queries and the join.
+// More than eight query heads on a KV head are several tiles, each of whose warps fetches and unpacks the rows for itself
+// (131 071 tokens, 8 KV heads: 16 query heads each 109 us, 64 each 433).
 #pragma once
 #include "q4.cuh"
 

@@ -363,8 +363,9 @@ class V0Worker:
 
     def init_scores(self) -> ScorePool:
         """Starts to gather every cached token's attention weight, from zero. On a 16-bit pool the engine that computes
-        the attention adds to `scores.layers` itself. Weights follow evict_tokens and compact_blocks; where blocks are
-        swapped or go to another worker, the caller moves theirs (`scores.gather`, `scores.scatter`)."""
+        the attention adds to `scores.layers` itself. Weights follow evict_tokens and compact_blocks, and start from zero
+        in blocks that write_kv_blocks fills; where blocks are swapped or go to another worker, the caller moves theirs
+        behind them (`scores.gather`, `scores.scatter`)."""
         self.scores = ScorePool.like(self._require_pool())
         return self.scores
 

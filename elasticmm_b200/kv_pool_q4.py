@@ -282,7 +282,7 @@ class KVPoolQ4(KVPool):
         where given, must not overlap the query unless it is the same tensor.
 
         With `scores`, each token's weight, summed over the query heads of its KV head, is added to its entry of this
-        layer; a block may then belong to one sequence only. `max_len` (default: what the tables can hold) bounds the
+        layer; a block may then appear once in the tables, and in no call that overlaps on the GPU. `max_len` (default: what the tables can hold) bounds the
         lengths and sizes the workspace; a length outside is clamped and reported by Context.check_status.
         """
         sig = (query.shape, query.stride(), query.dtype, query.device, block_tables.shape, block_tables.stride(),

@@ -381,12 +381,14 @@ int emm_q4_read(emm_pool *pool, int32_t head_dim, int32_t dtype, int32_t layer_b
  * last block are not read. A sequence of length 0 gives zeros. A length
  * outside [0, max_len] is recorded (EMM_ERR_LENGTH) and clamped; a block id
  * outside the pool is recorded and its tokens are left out. max_len bounds the
- * workspace and must not exceed table_width * BS.
+ * workspace and must not exceed table_width * BS. An fp16 result saturates at
+ * +-65504.
  *
  * With `scores` (a single-plane pool of fp32 [NB, H, BS] with the KV pool's
  * layers, emm_pool_desc_blocks(L, NB, H, BS, 4)) each token's weight, summed
  * over the query heads of its KV head, is added to its entry of that layer.
- * No block may then belong to two of the call's sequences (each block has one
+ * No block may then appear twice in the tables of the call, nor in those of
+ * another call with this pool that may overlap on the GPU (each block has one
  * owner, as V0BlockManager hands them out).
  *
  * The workspace (emm_q4_attend_workspace bytes, 16-byte aligned) is scratch of

@@ -146,3 +146,16 @@ def test_the_broadcast_form_moves_4_bit_blocks_as_bytes(monkeypatch):
     for worker, dtype, mode in ((a, "bfloat16", "send"), (wide, "uint8", "send"), (wide, "uint8", "recv"), (a, "int8", "recv")):
         with pytest.raises(ValueError, match="Unsupported dtype"):
             worker.collective_transfer_kv(None, 0, [0], (1,), dtype, mode)
+
+
+@pytest.mark.parametrize("layout", ["nhd", "hnd"])
+def test_4_bit_blocks_swap_in_both_layouts(layout):
+    w = _worker(layout, cpu=4)
+    w.write_kv_blocks([2, 3], _blocks(2, 5))
+    before = w.extract_kv_blocks([2, 3]).clone()
+    w.swap_blocks(["r"], [2, 3], [1, 0], is_swap_in=False)
+    w.wait_for_all_swap_out()
+    w.write_kv_blocks([2, 3], _blocks(2, 6))
+    w.swap_blocks(["r"], [0, 1], [8, 9], is_swap_in=True)
+    w.wait_for_all_swap_in()
+    assert torch.equal(w.extract_kv_blocks([9, 8]), before)
